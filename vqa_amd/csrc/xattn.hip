@@ -329,7 +329,7 @@ __device__ __forceinline__ void xa_block_reduce(float (&v)[HP], float (*red)[HP]
 
 typedef float xa_f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ xa_f32x2 xa_fma2(float w, xa_f32x2 x, xa_f32x2 a) {
-  // two FMAs in one packed instruction (v_pk_fma_f32): each element is the same correctly rounded fmaf
+  // one FMA per element, each a correctly rounded fmaf
   return __builtin_elementwise_fma(xa_f32x2{w, w}, x, a);
 }
 // A token row piece (8 columns) as it arrives from memory: bf16 rows stay packed until they are multiplied.
