@@ -715,6 +715,46 @@ int vqaf_scale_cast(const float* in, const float* scale, size_t n, int out_dtype
                     vqaf_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
+ * Answer scores: what vqaf_ce_conf's loss and confidence (attack/metric_src.py:302-426) leave out of a row of logits.
+ * With z = x / temperature: logprobs (R,T) f32 = log softmax(z) at targets (R,T) int64; entropy (R) f32 of softmax(z);
+ * top_logprobs / top_indices (R,K) f32 / int64, the K largest in falling order, ties to the lowest index, NaN first.
+ * logits (R,C) `dtype`, rows `ld` >= 0 elements apart (0: one row repeated), inner stride 1, any element alignment.
+ * T, K <= 128, K <= C; either may be 0, entropy may be NULL.  stats (R,2) f32, or NULL, receives what the backward
+ * needs.  temperature in [2^-20, 2^20].
+ * A negative target is none (log probability 0, no gradient); one past the classes gives NaN.  -inf logits have
+ * probability 0.  A row of nothing but -inf has log probabilities -inf, entropy 0 and a zero gradient; a row with a
+ * NaN or +inf is NaN throughout.
+ * Backward: grad (R,C) `dtype` of g_logprobs (R,T), g_entropy (R) and g_top (R,K) f32, each may be NULL, from the
+ * forward's stats and entropy; an entry named more than once gets all its terms.  grad rows have to lie on their
+ * 16-byte grid as the logits' rows do: (grad - logits) a multiple of 16 bytes, and (ld_grad - ld) too. */
+int vqaf_token_logprobs(const void* logits, long ld, const int64_t* targets, int R, int C, int T, int K, int dtype,
+                        double temperature, float* logprobs, float* entropy, float* top_logprobs,
+                        int64_t* top_indices, float* stats, vqaf_stream_t stream);
+int vqaf_token_logprobs_bwd(const void* logits, long ld, const int64_t* targets, const int64_t* top_indices, int R,
+                            int C, int T, int K, int dtype, double temperature, const float* stats,
+                            const float* entropy, const float* g_logprobs, const float* g_entropy,
+                            const float* g_top, void* grad, long ld_grad, vqaf_stream_t stream);
+
+/* Distillation from a teacher's top answers, in the place of the hard-label loss of utils/src.py:96.  teacher (R,K)
+ * f32: the teacher's log probabilities AT THE TEMPERATURE of the answers indices (R,K) int64 (top_logprobs /
+ * top_indices of vqaf_token_logprobs); a negative index is no answer, one past the classes makes its row NaN.
+ * q_k = exp(teacher_k), divided by their sum (tail 0) or as they are with the remaining mass r = 1 - sum q as one more
+ * event, met by all classes outside the list together (tail 1; r <= 2^-20 is taken for the rounding it is, and a list
+ * of all classes or of none has no rest).  p = softmax(x / temperature):
+ *   row_loss = temperature^2 [ sum_k q_k (log q_k - log p_{i_k}) + r (log r - log sum_{j outside} p_j) ].
+ * row_loss (R) f32.  grad, if non-NULL, receives scale * d(sum of rows)/dx in `dtype` (layout as above), formed from
+ * the same read of the logits.  loss, if non-NULL, receives scale * sum of rows, added in a fixed order.  stats (R,5)
+ * f64, or NULL, receives what vqaf_distill_bwd needs: the gradient for an incoming gradient `up` in device memory, one
+ * for each row (up_step 1) or a scalar (0), times scale.  skip_unit (scalar only): leave grad as it is where up[0] is
+ * exactly 1, for a caller who has the forward's gradient in it.  K in [1, 128].  With tail at most 393000 classes. */
+int vqaf_distill(const void* logits, long ld, const float* teacher, const int64_t* indices, int R, int C, int K,
+                 int dtype, double temperature, int tail, float* row_loss, double* stats, void* grad, long ld_grad,
+                 double scale, float* loss, vqaf_stream_t stream);
+int vqaf_distill_bwd(const void* logits, long ld, const float* teacher, const int64_t* indices, int R, int C, int K,
+                     int dtype, double temperature, const double* stats, const float* up, int up_step, int skip_unit,
+                     double scale, void* grad, long ld_grad, vqaf_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
  * Encoder blocks: the transformer layers of the vision and text encoders whose outputs feed the
  * fusion (model/vision_encoder.py:83-127 and model/text_encoder.py:14-48 wrap Hugging Face
  * models; these are the per-layer operations of those models that are not plain GEMMs).

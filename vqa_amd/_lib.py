@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_long, c_size_t, c_uint64, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_long, c_size_t, c_uint64, c_void_p
 
 import torch
 
@@ -174,6 +174,13 @@ SIGNATURES = {
     "vqaf_ce_conf": (c_int, [_P, _P, c_int, c_int, c_int, _P, _P, _P, _P, c_int, c_float, _P]),
     "vqaf_ce_mean": (c_int, [_P, _P, c_int, c_int, c_int, _P, _P, c_long, c_int, c_float, _P, _P, _P]),
     "vqaf_scale_cast": (c_int, [_P, _P, c_size_t, c_int, _P, _P]),
+    "vqaf_token_logprobs": (c_int, [_P, c_long, _P, c_int, c_int, c_int, c_int, c_int, c_double, _P, _P, _P, _P, _P, _P]),
+    "vqaf_token_logprobs_bwd": (c_int, [_P, c_long, _P, _P, c_int, c_int, c_int, c_int, c_int, c_double, _P, _P, _P, _P,
+                                        _P, _P, c_long, _P]),
+    "vqaf_distill": (c_int, [_P, c_long, _P, _P, c_int, c_int, c_int, c_int, c_double, c_int, _P, _P, _P, c_long,
+                             c_double, _P, _P]),
+    "vqaf_distill_bwd": (c_int, [_P, c_long, _P, _P, c_int, c_int, c_int, c_int, c_double, _P, _P, c_int, c_int, c_double,
+                                 _P, c_long, _P]),
     "vqaf_attn_fwd": (c_int, [_P, _P, _P, c_long, _P, c_int, c_int, c_int, c_int, c_float, c_float, _P, _P, c_long,
                               _P, _P]),
     "vqaf_attn_bwd": (c_int, [_P, _P, _P, c_long, _P, _P, c_long, _P, c_int, c_int, c_int, c_int, c_float, c_float,

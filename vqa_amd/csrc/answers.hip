@@ -1,0 +1,1410 @@
+// What a model answers with: log probabilities of given tokens, the entropy of the answer distribution and its top
+// alternatives (forward and backward), and the distillation loss against a teacher's top answers with its gradient.
+// They score the answers for the membership attacks (attack/metric_src.py:302-426 reads a loss and a maximum per
+// sample; these are the finer scores) and train a student on them in place of hard labels (utils/src.py:96).
+//
+// With z = x / T, m = max z, e_j = exp(z_j - m), S = sum_j e_j, p_j = e_j / S:
+//   log p_t = z_t - m - log S            H = log S - sum_j e_j (z_j - m) / S
+//   d log p_t / dx_j = (1{j = t} - p_j) / T            dH / dx_j = -p_j (log p_j + H) / T
+// and for a teacher's answers i_k with probabilities q_k (rest r, held by no answer of the list):
+//   L = T^2 [ sum_k q_k (log q_k - log p_{i_k}) + r (log r - log P) ],     P = sum of p_j outside the list
+//   dL / dx_j = T [ p_j (sum q + r) - sum_{k: i_k = j} q_k ] on the list,  T p_j [ sum q + r - r / P ] elsewhere.
+//
+// All of it is bound by the row of logits: read once (and its gradient written once).  A row therefore stays in
+// registers from its one read to its last use: rows of up to 1024 classes in one wave (four rows to a workgroup),
+// longer ones in a workgroup of 256 to 1024 threads, which covers 65536 classes; longer rows are read again for each
+// use.  Loads are whole 16-byte pieces on 16-byte addresses, whatever the row's own alignment (a vocabulary of 50265
+// puts every second bf16 row on an odd address): the row is cut at the pieces' borders and what lies outside it is
+// masked in registers.
+//
+// Precision.  The divergence of two close distributions is a small difference of large terms, so the normaliser, the
+// entropy's sum and the loss are carried in 64 bits: sums of eight in f32, sums of those in f64; the exponent
+// (x - m) log2(e) / T is formed with the two-term constant, because the rounding of a single one would shift every
+// term of a row the same way.  Rows of one wave, whose few terms do not average their rounding out, take the
+// exponential itself in f64 (a Taylor polynomial after range reduction; the f64 vector rate of this chip is the f32
+// one).  Probabilities, and with them the gradients, are f32 and rounded once into their type.
+
+#include <type_traits>
+
+#include "common.h"
+
+namespace {
+
+constexpr int AN_TOP_MAX = 128;     // alternatives / teacher answers per row
+constexpr int AN_WAVE_C = 1024;     // classes up to which a row belongs to one wave
+constexpr int AN_CAP = 1024;        // candidates for the top alternatives that fit in shared memory
+constexpr float AN_NO_REST = 9.5367431640625e-07f;  // 2^-20: a smaller remainder of f32 log probabilities is rounding
+
+constexpr double AN_LN2 = 0.69314718055994530942;
+constexpr double AN_LOG2E = 1.44269504088896340736;
+
+typedef unsigned long long u64;
+
+// ---------------------------------------------------------------------------------------------
+// Order of the alternatives: larger value first, then lower index; NaN above everything (as torch.topk has it)
+// and the two zeros equal.
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ unsigned an_key(float x) {
+  const unsigned u = __float_as_uint(x + 0.0f);   // -0 + 0 = +0
+  const unsigned k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return x != x ? 0xffffffffu : k;
+}
+__device__ __forceinline__ float an_unkey(unsigned k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+constexpr unsigned AN_KEY_MINF = 0x007fffffu;   // an_key(-inf): the lowest key of any value
+__device__ __forceinline__ u64 an_pack(unsigned key, int idx) { return ((u64)key << 32) | (unsigned)~idx; }
+__device__ __forceinline__ int an_index(u64 c) { return (int)~(unsigned)c; }
+
+// ---------------------------------------------------------------------------------------------
+// Wave reductions through DPP; the result is in every lane (read from lane 63).
+// ---------------------------------------------------------------------------------------------
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned an_dpp(unsigned idle, unsigned x) {
+  return (unsigned)__builtin_amdgcn_update_dpp((int)idle, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <class F>
+__device__ __forceinline__ unsigned an_wave_u32(unsigned x, unsigned idle, F f) {
+  x = f(x, an_dpp<0x111, 0xf>(idle, x));
+  x = f(x, an_dpp<0x112, 0xf>(idle, x));
+  x = f(x, an_dpp<0x114, 0xf>(idle, x));
+  x = f(x, an_dpp<0x118, 0xf>(idle, x));
+  x = f(x, an_dpp<0x142, 0xa>(idle, x));
+  x = f(x, an_dpp<0x143, 0xc>(idle, x));
+  return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ float an_wave_max(float v) {
+  return __uint_as_float(an_wave_u32(__float_as_uint(v), 0xff800000u, [](unsigned a, unsigned b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+__device__ __forceinline__ unsigned an_wave_umax(unsigned v) {
+  return an_wave_u32(v, 0u, [](unsigned a, unsigned b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ unsigned an_wave_umin(unsigned v) {
+  return an_wave_u32(v, 0xffffffffu, [](unsigned a, unsigned b) { return a < b ? a : b; });
+}
+__device__ __forceinline__ unsigned an_wave_uadd(unsigned v) {
+  return an_wave_u32(v, 0u, [](unsigned a, unsigned b) { return a + b; });
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double an_dadd(double x) {
+  const u64 u = __builtin_bit_cast(u64, x);
+  const u64 o = ((u64)an_dpp<CTRL, ROWS>(0u, (unsigned)(u >> 32)) << 32) | an_dpp<CTRL, ROWS>(0u, (unsigned)u);
+  return x + __builtin_bit_cast(double, o);   // idle lanes contribute +0
+}
+__device__ __forceinline__ double an_wave_sum(double x) {
+  x = an_dadd<0x111, 0xf>(x);
+  x = an_dadd<0x112, 0xf>(x);
+  x = an_dadd<0x114, 0xf>(x);
+  x = an_dadd<0x118, 0xf>(x);
+  x = an_dadd<0x142, 0xa>(x);
+  x = an_dadd<0x143, 0xc>(x);
+  const u64 u = __builtin_bit_cast(u64, x);
+  const u64 r = ((u64)(unsigned)__builtin_amdgcn_readlane((int)(u >> 32), 63) << 32) |
+                (unsigned)__builtin_amdgcn_readlane((int)(unsigned)u, 63);
+  return __builtin_bit_cast(double, r);
+}
+
+// exp(t) for t <= 0 to about 2^-40: t = k ln 2 + f with |f| <= ln 2 / 2, Taylor's polynomial of degree 10 in f
+// (the first term left out is f^11 / 11! < 2^-41).  NaN stays NaN; below -700 the result is zero.
+__device__ __forceinline__ double an_exp(double t) {
+  const double c = t < -700.0 ? -700.0 : t;
+  const double k = __builtin_rint(c * AN_LOG2E);
+  const double f = fma(-k, AN_LN2, c);   // |k| < 1100: the constant's own rounding stays below 2^-42
+  double p = 1.0 / 3628800.0;
+  p = fma(p, f, 1.0 / 362880.0);
+  p = fma(p, f, 1.0 / 40320.0);
+  p = fma(p, f, 1.0 / 5040.0);
+  p = fma(p, f, 1.0 / 720.0);
+  p = fma(p, f, 1.0 / 120.0);
+  p = fma(p, f, 1.0 / 24.0);
+  p = fma(p, f, 1.0 / 6.0);
+  p = fma(p, f, 0.5);
+  p = fma(p, f, 1.0);
+  p = fma(p, f, 1.0);
+  return t < -700.0 ? 0.0 : ldexp(p, (int)k);
+}
+
+// the exponent's factor log2(e) / T in two f32 terms
+struct AnTemp {
+  float hi, lo;
+  double inv_t;
+};
+inline AnTemp an_temp(double temperature) {
+  AnTemp t;
+  t.inv_t = 1.0 / temperature;
+  const double c = AN_LOG2E * t.inv_t;
+  t.hi = (float)c;
+  t.lo = (float)(c - (double)t.hi);
+  return t;
+}
+// (x - m) log2(e) / T.  x = -inf gives -inf (the second term, of either sign, stays finite); NaN comes through the first.
+__device__ __forceinline__ float an_arg(float x, float m, float hi, float lo) {
+  const float d = x - m;
+  return fmaf(d, hi, fmaxf(d, -3.402823466e38f) * lo);
+}
+__device__ __forceinline__ float an_exp2(float t) { return __builtin_amdgcn_exp2f(t); }
+// the factor of e in the entropy's sum: finite where e is zero, so that 0 * t stays 0
+__device__ __forceinline__ float an_floor(float t) { return fmaxf(t, -4096.f); }
+
+// ---------------------------------------------------------------------------------------------
+// A row cut into 16-byte pieces.
+// ---------------------------------------------------------------------------------------------
+template <bool BF16>
+struct Piece {
+  static constexpr int V = BF16 ? 8 : 4;
+};
+template <bool BF16>
+__device__ __forceinline__ void an_unpack(const u32x4 r, float (&v)[Piece<BF16>::V]) {
+  if constexpr (BF16) {
+    v[0] = bf16_lo(r.x); v[1] = bf16_hi(r.x); v[2] = bf16_lo(r.y); v[3] = bf16_hi(r.y);
+    v[4] = bf16_lo(r.z); v[5] = bf16_hi(r.z); v[6] = bf16_lo(r.w); v[7] = bf16_hi(r.w);
+  } else {
+    v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y);
+    v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+  }
+}
+
+// Geometry of one row: its first element lies `shift` elements into piece 0.  `lo` and `hi` bound the memory of the
+// whole matrix: a piece that reaches outside it (at the very first or last row only) is read element by element.
+struct Span {
+  const unsigned char* first;   // address of piece 0
+  const unsigned char* lo;
+  const unsigned char* hi;
+  int shift, pieces, C;
+};
+template <bool BF16>
+__device__ __forceinline__ Span an_span(const void* base, long ld, long row, long rows, int C) {
+  constexpr int ES = BF16 ? 2 : 4;
+  Span s;
+  const unsigned char* b = reinterpret_cast<const unsigned char*>(base);
+  const unsigned char* r = b + row * ld * ES;
+  s.shift = (int)((reinterpret_cast<uintptr_t>(r) & 15u) / ES);
+  s.first = r - s.shift * ES;
+  s.lo = b;
+  s.hi = b + ((rows - 1) * ld + C) * ES;
+  s.pieces = (s.shift + C + Piece<BF16>::V - 1) / Piece<BF16>::V;
+  s.C = C;
+  return s;
+}
+// Elements of piece c outside the row become -inf.  `el` = column of the piece's first element.
+template <bool BF16>
+__device__ __forceinline__ u32x4 an_mask(u32x4 r, int el, int C) {
+  constexpr int V = Piece<BF16>::V;
+  if (el < 0 || el + V > C) {
+    unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const bool out = el + j < 0 || el + j >= C;
+      if constexpr (BF16) {
+        const unsigned keep = (j & 1) ? 0x0000ffffu : 0xffff0000u, put = (j & 1) ? 0xff800000u : 0x0000ff80u;
+        w[j >> 1] = out ? ((w[j >> 1] & keep) | put) : w[j >> 1];
+      } else {
+        w[j] = out ? 0xff800000u : w[j];
+      }
+    }
+    r = u32x4{w[0], w[1], w[2], w[3]};
+  }
+  return r;
+}
+// A piece that reaches outside the matrix, element by element.
+template <bool BF16>
+__device__ __forceinline__ u32x4 an_load_edge(const Span& s, int el) {
+  constexpr int V = Piece<BF16>::V;
+  const unsigned char* row = s.first + s.shift * (BF16 ? 2 : 4);
+  unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (el + j >= 0 && el + j < s.C) {
+      if constexpr (BF16) w[j >> 1] |= (unsigned)reinterpret_cast<const bf16_t*>(row)[el + j] << (16 * (j & 1));
+      else w[j] = reinterpret_cast<const unsigned*>(row)[el + j];
+    }
+  }
+  return u32x4{w[0], w[1], w[2], w[3]};
+}
+
+// The pieces tid, tid + NT, ... of a row, in registers (E > 0) or read again on every walk (E == 0).
+template <bool BF16, int NT, int E>
+struct RowPieces {
+  static constexpr int V = Piece<BF16>::V;
+  Span s;
+  u32x4 raw[E > 0 ? E : 1];
+
+  // one piece; pieces past the row read piece 1, which lies inside it (rows here have more than 1024 classes)
+  __device__ __forceinline__ u32x4 fetch(int c) const {
+    const unsigned char* p = s.first + (long)c * 16;
+    const bool safe = c < s.pieces && p >= s.lo && p + 16 <= s.hi;
+    return *reinterpret_cast<const u32x4*>(safe ? p : s.first + 16);
+  }
+  __device__ __forceinline__ u32x4 finish(u32x4 r, int c) const {
+    const unsigned char* p = s.first + (long)c * 16;
+    const int el = c * V - s.shift;
+    if (c < s.pieces && (p < s.lo || p + 16 > s.hi)) r = an_load_edge<BF16>(s, el);
+    return an_mask<BF16>(r, el, s.C);
+  }
+  __device__ __forceinline__ void load() {
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) raw[i] = fetch((int)threadIdx.x + i * NT);
+#pragma unroll
+      for (int i = 0; i < E; ++i) raw[i] = finish(raw[i], (int)threadIdx.x + i * NT);
+    }
+  }
+  // f(v, c, el): the V values of piece c, the first of them in column el; columns outside [0, C) hold -inf
+  template <class F>
+  __device__ __forceinline__ void walk(F f) const {
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        float v[V];
+        an_unpack<BF16>(raw[i], v);
+        f(v, (int)threadIdx.x + i * NT, ((int)threadIdx.x + i * NT) * V - s.shift);
+      }
+    } else {
+      for (int c = threadIdx.x; c < s.pieces; c += NT) {
+        float v[V];
+        an_unpack<BF16>(finish(fetch(c), c), v);
+        f(v, c, c * V - s.shift);
+      }
+    }
+  }
+};
+
+// whether the row holds a NaN (every thread of the workgroup calls)
+template <int NT, class ROW>
+__device__ __forceinline__ bool an_block_nan(const ROW& row) {
+  int nan = 0;
+  row.walk([&](const float (&v)[ROW::V], int, int) {
+#pragma unroll
+    for (int j = 0; j < ROW::V; ++j) nan |= v[j] != v[j] ? 1 : 0;
+  });
+  return __syncthreads_or(nan) != 0;
+}
+
+template <int V>
+__device__ __forceinline__ float an_tree(const float (&v)[V]) {
+  if constexpr (V == 8) return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+  else return (v[0] + v[1]) + (v[2] + v[3]);
+}
+
+template <bool BF16>
+__device__ __forceinline__ float an_at(const void* row, long j) { return load1<BF16>(row, (size_t)j); }
+template <bool BF16>
+__device__ __forceinline__ const void* an_row(const void* base, long ld, long row) {
+  return reinterpret_cast<const unsigned char*>(base) + row * ld * (BF16 ? 2 : 4);
+}
+
+// What a row's statistics give for one logit.  A row without a live entry (m = -inf) has log probability -inf
+// everywhere; a NaN or +inf in the row makes all of it NaN.
+__device__ __forceinline__ float an_logprob(float x, float m, double log_s, double inv_t) {
+  if (m == -INFINITY) return -INFINITY;
+  return (float)(((double)x - (double)m) * inv_t - log_s);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Log probabilities: one workgroup per row
+// ---------------------------------------------------------------------------------------------
+struct LogprobArgs {
+  const void* x;
+  const int64_t* targets;
+  float* logprobs;
+  float* entropy;
+  float* top_logprobs;
+  int64_t* top_indices;
+  float* stats;   // (R,2): m, S
+  long ld, R;
+  int C, T, K;
+  AnTemp temp;
+};
+
+template <int NT>
+struct TopShared {
+  float tmax[NT];
+  u64 cand[AN_CAP];
+  int rank[AN_CAP];
+  int n;
+  float thr;
+  int cnt[2];
+};
+
+// how many of the workgroup's elements pass `f` (all threads call; two barriers)
+template <int NT, class ROW, class F>
+__device__ __forceinline__ int an_block_count(const ROW& row, int* cnt, F f) {
+  constexpr int V = ROW::V;
+  __syncthreads();
+  if (threadIdx.x == 0) cnt[0] = 0;
+  __syncthreads();
+  unsigned n = 0;
+  row.walk([&](const float (&v)[V], int, int el) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) n += (el + j >= 0 && el + j < row.s.C && f(v[j], el + j)) ? 1u : 0u;
+  });
+  n = an_wave_uadd(n);
+  if ((threadIdx.x & 63) == 0) atomicAdd(&cnt[0], (int)n);
+  __syncthreads();
+  return cnt[0];
+}
+
+// The K best of a row into sh.cand, by counting alone: the K-th key bit by bit, then the index up to which elements
+// equal to it belong.  For rows whose candidates overflow the list (long ties: a masked row has nothing but) and rows
+// with NaN; 63 passes at most.
+template <bool BF16, int NT>
+__device__ __forceinline__ void an_top_by_counting(const Span& span, TopShared<NT>& sh, int K) {
+  constexpr int V = Piece<BF16>::V;
+  RowPieces<BF16, NT, 0> row;   // reads the row again: the common path's registers stay its own
+  row.s = span;
+  unsigned t = 0;
+  for (int b = 31; b >= 0; --b) {
+    const unsigned mid = t | (1u << b);
+    if (an_block_count<NT>(row, sh.cnt, [&](float x, int) { return an_key(x) >= mid; }) >= K) t = mid;
+  }
+  const int above = an_block_count<NT>(row, sh.cnt, [&](float x, int) { return an_key(x) > t; });
+  const int need = K - above;   // of the elements equal to t, >= 1
+  int last = 0;                 // the lowest index bound that admits `need` of them: [0, last]
+  {
+    int lo = 0, hi = row.s.C - 1;
+    while (lo < hi) {
+      const int mid = lo + ((hi - lo) >> 1);
+      if (an_block_count<NT>(row, sh.cnt, [&](float x, int j) { return an_key(x) == t && j <= mid; }) >= need) hi = mid;
+      else lo = mid + 1;
+    }
+    last = lo;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) sh.n = 0;
+  __syncthreads();
+  row.walk([&](const float (&v)[V], int, int el) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int col = el + j;
+      if (col < 0 || col >= row.s.C) continue;
+      const unsigned k = an_key(v[j]);
+      if (k > t || (k == t && col <= last)) sh.cand[atomicAdd(&sh.n, 1) & (AN_CAP - 1)] = an_pack(k, col);
+    }
+  });
+  __syncthreads();
+}
+
+// Wave 0: a value that at least K, and not many more than K, of the threads' maxima reach.  At least K elements of the
+// row reach it then, and the elements that do lie with few threads.
+template <int NT>
+__device__ __forceinline__ float an_threshold(const float* tmax, int threads_with_data, int K) {
+  constexpr int PER = NT / 64;
+  const int lane = threadIdx.x & 63;
+  unsigned k[PER];
+  unsigned lo = 0xffffffffu, hi = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = i * 64 + lane;
+    k[i] = t < threads_with_data ? an_key(tmax[t]) : 0u;
+  }
+  unsigned best = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) best = k[i] > best ? k[i] : best;
+  hi = an_wave_umax(best);
+  lo = an_wave_umin(best);                      // 64 maxima reach it if every lane has one
+  if (K > 64 || lo < AN_KEY_MINF) lo = AN_KEY_MINF;
+  const int most = K + (K >> 1) + 16;
+  // invariant: at least K maxima are >= lo; fewer than K are >= hi + 1
+  unsigned up = hi;
+  while (lo < up) {
+    const unsigned mid = lo + ((up - lo) >> 1) + 1;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) c += __popcll(__ballot(k[i] >= mid));
+    if (c >= K) {
+      lo = mid;
+      if (c <= most) break;
+    } else {
+      up = mid - 1;
+    }
+  }
+  return an_unkey(lo);
+}
+
+template <bool BF16, int NT, int E>
+__global__ __launch_bounds__(NT) void logprob_block_kernel(const LogprobArgs a) {
+  constexpr int V = Piece<BF16>::V, NW = NT / 64;
+  __shared__ TopShared<NT> sh;
+  __shared__ float s_max[NW];
+  __shared__ double s_sum[2][NW];
+  const long r = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  RowPieces<BF16, NT, E> row;
+  row.s = an_span<BF16>(a.x, a.ld, r, a.R, a.C);
+  row.load();
+
+  float m = -INFINITY;
+  row.walk([&](const float (&v)[V], int, int) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) m = fmaxf(m, v[j]);
+  });
+  if (a.K > 0) {
+    sh.tmax[tid] = m;
+    if (tid == 0) sh.n = 0;
+    for (int i = tid; i < AN_CAP; i += NT) sh.rank[i] = 0;
+  }
+  m = an_wave_max(m);
+  if (lane == 0) s_max[wave] = m;
+  __syncthreads();
+  m = s_max[0];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) m = fmaxf(m, s_max[i]);
+  if (m == -INFINITY && an_block_nan<NT>(row)) m = NAN;   // (the maximum leaves NaN out)
+
+  double S = 0.0, W = 0.0;
+  const float hi = a.temp.hi, lo = a.temp.lo;
+  row.walk([&](const float (&v)[V], int, int) {
+    float e[V], w[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float t = an_arg(v[j], m, hi, lo);
+      e[j] = an_exp2(t);
+      w[j] = e[j] * an_floor(t);
+    }
+    S += (double)an_tree<V>(e);
+    W += (double)an_tree<V>(w);
+  });
+  S = an_wave_sum(S);
+  W = an_wave_sum(W);
+  if (lane == 0) {
+    s_sum[0][wave] = S;
+    s_sum[1][wave] = W;
+  }
+  if (a.K > 0 && wave == 0) {
+    const float t = an_threshold<NT>(sh.tmax, row.s.pieces < NT ? row.s.pieces : NT, a.K);
+    if (lane == 0) sh.thr = t;
+  }
+  __syncthreads();
+  S = s_sum[0][0];
+  W = s_sum[1][0];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) {
+    S += s_sum[0][i];
+    W += s_sum[1][i];
+  }
+  const bool empty = m == -INFINITY;
+  const bool broken = !empty && !(S == S);   // a NaN or +inf in the row
+  const double log_s = empty ? -INFINITY : log(S);
+  const void* xr = an_row<BF16>(a.x, a.ld, r);
+  if (tid == 0) {
+    if (a.entropy != nullptr) a.entropy[r] = empty ? 0.f : (float)(log_s - AN_LN2 * (W / S));
+    if (a.stats != nullptr) {
+      a.stats[2 * r] = m;
+      a.stats[2 * r + 1] = empty ? 1.f : (float)S;
+    }
+  }
+  for (int i = tid; i < a.T; i += NT) {
+    const int64_t t = a.targets[r * a.T + i];
+    float lp = 0.f;                                         // a negative target is none
+    if (t >= a.C) lp = NAN;
+    else if (t >= 0) lp = an_logprob(an_at<BF16>(xr, t), m, log_s, a.temp.inv_t);
+    a.logprobs[r * a.T + i] = lp;
+  }
+  if (a.K == 0) return;
+
+  // candidates: what reaches the threshold
+  bool counted = broken;
+  if (!broken) {
+    const float thr = sh.thr;
+    if (sh.tmax[tid] >= thr) {
+      row.walk([&](const float (&v)[V], int, int el) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (v[j] >= thr && el + j >= 0 && el + j < a.C) {
+            const int at = atomicAdd(&sh.n, 1);
+            if (at < AN_CAP) sh.cand[at] = an_pack(an_key(v[j]), el + j);
+          }
+        }
+      });
+    }
+    __syncthreads();
+    counted = sh.n > AN_CAP;   // uniform
+  }
+  if (counted) an_top_by_counting<BF16, NT>(row.s, sh, a.K);
+  const int n = sh.n;
+  // rank of each candidate: how many are before it.  The list is cut among the threads left over.
+  int npad = 64;
+  while (npad < n) npad <<= 1;
+  if (npad <= NT) {
+    const int parts = NT / npad, i = tid & (npad - 1), p = tid / npad;
+    if (i < n) {
+      const u64 mine = sh.cand[i];
+      int before = 0;
+      for (int j = p; j < n; j += parts) before += sh.cand[j] > mine ? 1 : 0;
+      if (before > 0) atomicAdd(&sh.rank[i], before);
+    }
+  } else {
+    for (int i = tid; i < n; i += NT) {
+      const u64 mine = sh.cand[i];
+      int before = 0;
+      for (int j = 0; j < n; ++j) before += sh.cand[j] > mine ? 1 : 0;
+      sh.rank[i] = before;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += NT) {
+    const int k = sh.rank[i];
+    if (k < a.K) {
+      const int j = an_index(sh.cand[i]);
+      a.top_indices[r * a.K + k] = j;
+      a.top_logprobs[r * a.K + k] = an_logprob(an_at<BF16>(xr, j), m, log_s, a.temp.inv_t);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Log probabilities: one wave per row of up to 1024 classes, column lane + 64 i in register i
+// ---------------------------------------------------------------------------------------------
+constexpr int AN_WAVES = 4;   // rows per workgroup
+
+// maximum over the wave; NaN for a row that holds nothing else but -inf (the maximum leaves NaN out)
+template <int E>
+__device__ __forceinline__ float an_wave_row_max(const float (&v)[E], float m) {
+  m = an_wave_max(m);
+  if (m == -INFINITY) {
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < E; ++i) nan |= v[i] != v[i];
+    if (__ballot(nan) != 0) m = NAN;
+  }
+  return m;
+}
+
+// K rounds of "the largest left, the lowest index of it": cheaper than a threshold while K is small
+constexpr int AN_ROUNDS = 12;
+
+template <bool BF16, int E>
+__global__ __launch_bounds__(64 * AN_WAVES) void logprob_wave_kernel(const LogprobArgs a) {
+  __shared__ u64 s_cand[AN_WAVES][AN_TOP_MAX];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long r = (long)blockIdx.x * AN_WAVES + wave;
+  if (r >= a.R) return;   // no barrier below: a wave keeps to its own row
+  const void* xr = an_row<BF16>(a.x, a.ld, r);
+  float v[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int c = lane + 64 * i;
+    v[i] = c < a.C ? an_at<BF16>(xr, c) : -INFINITY;
+  }
+  int64_t t = -1;
+  if (lane < a.T) t = a.targets[r * a.T + lane];   // the first 64; more are read below
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < E; ++i) m = fmaxf(m, v[i]);
+  m = an_wave_row_max<E>(v, m);
+  const bool empty = m == -INFINITY;
+  double S = 0.0, W = 0.0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const double d = ((double)v[i] - (double)m) * a.temp.inv_t;
+    const double e = an_exp(d);
+    S += e;
+    W += e * (d < -4096.0 ? -4096.0 : d);
+  }
+  S = an_wave_sum(S);
+  W = an_wave_sum(W);
+  const double log_s = empty ? -INFINITY : log(S);
+  if (lane == 0) {
+    if (a.entropy != nullptr) a.entropy[r] = empty ? 0.f : (float)(log_s - W / S);
+    if (a.stats != nullptr) {
+      a.stats[2 * r] = m;
+      a.stats[2 * r + 1] = empty ? 1.f : (float)S;
+    }
+  }
+  for (int i = lane; i < a.T; i += 64) {
+    if (i >= 64) t = a.targets[r * a.T + i];
+    float lp = 0.f;
+    if (t >= a.C) lp = NAN;
+    else if (t >= 0) lp = an_logprob(an_at<BF16>(xr, t), m, log_s, a.temp.inv_t);
+    a.logprobs[r * a.T + i] = lp;
+  }
+  if (a.K == 0) return;
+
+  unsigned key[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) key[i] = lane + 64 * i < a.C ? an_key(v[i]) : 0u;
+  if (a.K <= AN_ROUNDS) {
+    for (int k = 0; k < a.K; ++k) {
+      unsigned best = key[0];
+#pragma unroll
+      for (int i = 1; i < E; ++i) best = key[i] > best ? key[i] : best;
+      best = an_wave_umax(best);
+      int at = -1;
+#pragma unroll
+      for (int i = E - 1; i >= 0; --i) {
+        const u64 who = __ballot(key[i] == best);
+        if (who != 0) at = i * 64 + __ffsll((long long)who) - 1;
+      }
+      // (K <= C, so a live element is left: best > 0)
+#pragma unroll
+      for (int i = 0; i < E; ++i) key[i] = at == lane + 64 * i ? 0u : key[i];
+      if (lane == 0) {
+        a.top_indices[r * a.K + k] = at;
+        a.top_logprobs[r * a.K + k] = an_logprob(an_unkey(best), m, log_s, a.temp.inv_t);
+      }
+    }
+    return;
+  }
+  // the K-th key by bisection, from the smallest of the lanes' maxima where that is sure to be reached K times
+  unsigned best = key[0];
+#pragma unroll
+  for (int i = 1; i < E; ++i) best = key[i] > best ? key[i] : best;
+  unsigned up = an_wave_umax(best), low = an_wave_umin(best);
+  if (a.K > 64 || low < AN_KEY_MINF) low = AN_KEY_MINF;
+  while (low < up) {
+    const unsigned mid = low + ((up - low) >> 1) + 1;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) c += __popcll(__ballot(key[i] >= mid));
+    if (c >= a.K) {
+      low = mid;
+      if (c == a.K) break;
+    } else {
+      up = mid - 1;
+    }
+  }
+  // all elements above it, then the first of those equal to it: exactly K, in shared memory
+  int n = 0, above = 0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) above += __popcll(__ballot(key[i] > low));
+  int ties = a.K - above;
+  const u64 below_lane = (1ull << lane) - 1ull;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const u64 eq = __ballot(key[i] == low);
+    const bool take = key[i] > low || (key[i] == low && __popcll(eq & below_lane) < ties);
+    const u64 who = __ballot(take);
+    if (take) s_cand[wave][n + __popcll(who & below_lane)] = an_pack(key[i], lane + 64 * i);
+    n += __popcll(who);
+    ties -= __popcll(eq);
+    ties = ties < 0 ? 0 : ties;
+  }
+  __builtin_amdgcn_wave_barrier();
+  __threadfence_block();
+  for (int i = lane; i < a.K; i += 64) {
+    const u64 mine = s_cand[wave][i];
+    int before = 0;
+    for (int j = 0; j < a.K; ++j) before += s_cand[wave][j] > mine ? 1 : 0;
+    a.top_indices[r * a.K + before] = an_index(mine);
+    a.top_logprobs[r * a.K + before] = an_logprob(an_unkey((unsigned)(mine >> 32)), m, log_s, a.temp.inv_t);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Gradients, streamed: the row's statistics are known, every logit is read once and its gradient written once.
+// Entries of the row that something names (targets, alternatives, the teacher's answers) are written a second time,
+// whole, after a barrier: a few 2- or 4-byte stores into lines that the workgroup has just written.  An entry named
+// more than once is written by its first mention, which adds the others' terms in order.
+// ---------------------------------------------------------------------------------------------
+struct LogprobGrad {
+  const int64_t* targets;
+  const int64_t* top_indices;
+  const float* stats;
+  const float* entropy;
+  const float* g_lp;
+  const float* g_ent;
+  const float* g_top;
+  int T, K;
+  AnTemp temp;
+  // of the row
+  struct Row {
+    float m, inv_s, log_s, A, h, H, hi, lo, inv_t;
+    bool empty;
+  };
+  __device__ __forceinline__ bool done() const { return false; }
+  __device__ __forceinline__ int named() const { return (g_lp != nullptr ? T : 0) + (g_top != nullptr ? K : 0); }
+  __device__ __forceinline__ void mention(long r, int s, int C, int& idx, float& add) const {
+    const int t = g_lp != nullptr ? T : 0;
+    int64_t j;
+    float g;
+    if (s < t) {
+      j = targets[r * T + s];
+      g = g_lp[r * T + s];
+      if (j < 0) g = 0.f;        // no target: no gradient
+      if (j >= C) g = NAN;       // outside the classes: the row says so
+    } else {
+      j = top_indices[r * K + (s - t)];
+      g = g_top[r * K + (s - t)];
+    }
+    idx = j >= 0 && j < C ? (int)j : -1;
+    add = g;
+  }
+  __device__ __forceinline__ Row row(long r, int lane, int C) const {
+    Row w;
+    w.m = stats[2 * r];
+    const float S = stats[2 * r + 1];
+    w.inv_s = 1.0f / S;
+    w.log_s = logf(S);
+    w.H = entropy != nullptr ? entropy[r] : 0.f;
+    w.h = g_ent != nullptr ? g_ent[r] : 0.f;
+    double sum = 0.0;
+    for (int s = lane; s < named(); s += 64) {
+      int j;
+      float g;
+      mention(r, s, C, j, g);
+      sum += (double)g;
+    }
+    w.A = (float)an_wave_sum(sum);
+    w.hi = temp.hi;
+    w.lo = temp.lo;
+    w.inv_t = (float)temp.inv_t;
+    w.empty = w.m == -INFINITY;
+    return w;
+  }
+  static __device__ __forceinline__ float dense(const Row& w, float x) {
+    if (w.empty) return 0.f;
+    const float t = an_arg(x, w.m, w.hi, w.lo);
+    const float p = an_exp2(t) * w.inv_s;
+    const float lp = fmaf(an_floor(t), (float)AN_LN2, -w.log_s);
+    return -w.inv_t * (p * fmaf(w.h, lp + w.H, w.A));
+  }
+  static __device__ __forceinline__ float base(const Row& w, float x) { return dense(w, x); }
+  static __device__ __forceinline__ float term(const Row& w, float g) { return w.empty ? 0.f : w.inv_t * g; }
+};
+
+// (R,5) f64: m, S, mass = sum q + r, slope = mass - r / P, log Q (q_k = exp(v_k - log Q))
+struct DistillStat {
+  double m, S, mass, slope, log_q;
+};
+
+// a row that is all masked, or that no answer teaches (whatever its logits hold)
+__device__ __forceinline__ bool an_no_gradient(const DistillStat& s) {
+  return s.m == -INFINITY || (s.mass == 0.0 && s.slope == 0.0);
+}
+
+struct DistillGrad {
+  const float* teacher;
+  const int64_t* indices;
+  const DistillStat* stats;
+  const float* up;     // gradient of the loss, one per row (up_step 1) or one (0)
+  int up_step, K, skip_unit;   // skip_unit: nothing is left to do where up[0] is 1 (the gradient is there already)
+  float scale;         // T * (1 for a sum, 1 / R for a mean)
+  AnTemp temp;
+  struct Row {
+    float m, mass, slope, hi, lo, g;
+    double log_q;
+    bool empty;
+  };
+  __device__ __forceinline__ bool done() const { return skip_unit && up[0] == 1.0f; }
+  __device__ __forceinline__ int named() const { return K; }
+  __device__ __forceinline__ void mention(long r, int s, int C, int& idx, float& add) const {
+    const int64_t j = indices[r * K + s];
+    idx = j >= 0 && j < C ? (int)j : -1;
+    add = (float)an_exp((double)teacher[r * K + s] - stats[r].log_q);
+  }
+  __device__ __forceinline__ Row row(long r, int, int) const {
+    Row w;
+    const DistillStat s = stats[r];
+    w.m = (float)s.m;
+    w.empty = an_no_gradient(s);
+    const double inv = w.empty ? 0.0 : 1.0 / s.S;
+    w.mass = (float)(s.mass * inv);
+    w.slope = (float)(s.slope * inv);
+    w.hi = temp.hi;
+    w.lo = temp.lo;
+    w.g = scale * up[r * up_step];
+    return w;
+  }
+  static __device__ __forceinline__ float dense(const Row& w, float x) {
+    return w.empty ? 0.f : w.g * (an_exp2(an_arg(x, w.m, w.hi, w.lo)) * w.slope);
+  }
+  static __device__ __forceinline__ float base(const Row& w, float x) {
+    return w.empty ? 0.f : w.g * (an_exp2(an_arg(x, w.m, w.hi, w.lo)) * w.mass);
+  }
+  static __device__ __forceinline__ float term(const Row& w, float q) { return w.empty ? 0.f : -w.g * q; }
+};
+
+// the V gradients of a piece, into the row of the gradient that starts at the same place of its 16-byte grid
+template <bool BF16>
+__device__ __forceinline__ void an_store(unsigned char* grow, int el, int C, const float (&g)[Piece<BF16>::V]) {
+  constexpr int V = Piece<BF16>::V;
+  if (el >= 0 && el + V <= C) {
+    u32x4 w;
+    if constexpr (BF16) {
+      w.x = pack_bf16x2(g[0], g[1]); w.y = pack_bf16x2(g[2], g[3]);
+      w.z = pack_bf16x2(g[4], g[5]); w.w = pack_bf16x2(g[6], g[7]);
+      *reinterpret_cast<u32x4*>(grow + (long)el * 2) = w;
+    } else {
+      w.x = __float_as_uint(g[0]); w.y = __float_as_uint(g[1]); w.z = __float_as_uint(g[2]); w.w = __float_as_uint(g[3]);
+      *reinterpret_cast<u32x4*>(grow + (long)el * 4) = w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (el + j >= 0 && el + j < C) store1<BF16>(grow, (size_t)(el + j), g[j]);
+  }
+}
+
+// Mentions in shared memory, `count` threads with number `id` share them: writes the entries in [from, to).
+template <bool BF16, class F, class G>
+__device__ __forceinline__ void an_write_named(const int* idx, const float* add, int ns, int id, int count, int from, int to,
+                                               const void* xr, unsigned char* grow, F base, G term) {
+  for (int s = id; s < ns; s += count) {
+    const int j = idx[s];
+    if (j < from || j >= to) continue;
+    bool first = true;
+    float t = 0.f;
+    for (int o = 0; o < ns; ++o) {
+      const bool same = idx[o] == j;
+      if (same && o < s) first = false;
+      if (same) t += add[o];
+    }
+    if (first) store1<BF16>(grow, (size_t)j, base(an_at<BF16>(xr, j)) + term(t));
+  }
+}
+
+constexpr int AN_ST = 256, AN_SP = 4;   // threads, pieces per thread of a streamed segment
+constexpr int AN_NAMED = 2 * AN_TOP_MAX;
+
+template <bool BF16, class OP>
+__global__ __launch_bounds__(AN_ST) void answer_grad_block_kernel(const OP op, const void* x, long ld, long R, int C, int segments,
+                                                                  void* grad, long ldg) {
+  constexpr int V = Piece<BF16>::V;
+  __shared__ int s_idx[AN_NAMED];
+  __shared__ float s_add[AN_NAMED];
+  if (op.done()) return;   // uniform
+  const long r = blockIdx.x / segments;
+  const int seg = (int)(blockIdx.x - r * segments), tid = threadIdx.x;
+  RowPieces<BF16, AN_ST, 0> row;
+  row.s = an_span<BF16>(x, ld, r, R, C);
+  const int c0 = seg * (AN_ST * AN_SP);
+  u32x4 raw[AN_SP];
+#pragma unroll
+  for (int i = 0; i < AN_SP; ++i) raw[i] = row.fetch(c0 + i * AN_ST + tid);
+  const int ns = op.named();
+  for (int s = tid; s < ns; s += AN_ST) op.mention(r, s, C, s_idx[s], s_add[s]);
+  const typename OP::Row w = op.row(r, tid & 63, C);
+  unsigned char* grow = reinterpret_cast<unsigned char*>(grad) + r * ldg * (BF16 ? 2 : 4);
+#pragma unroll
+  for (int i = 0; i < AN_SP; ++i) {
+    const int c = c0 + i * AN_ST + tid, el = c * V - row.s.shift;
+    if (c < row.s.pieces) {
+      float v[V], g[V];
+      an_unpack<BF16>(row.finish(raw[i], c), v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) g[j] = OP::dense(w, v[j]);
+      an_store<BF16>(grow, el, C, g);
+    }
+  }
+  __syncthreads();
+  const int from = c0 * V - row.s.shift;
+  an_write_named<BF16>(s_idx, s_add, ns, tid, AN_ST, from < 0 ? 0 : from, min(C, from + AN_ST * AN_SP * V),
+                       an_row<BF16>(x, ld, r), grow, [&](float v) { return OP::base(w, v); },
+                       [&](float t) { return OP::term(w, t); });
+}
+
+template <bool BF16, int E, class OP>
+__global__ __launch_bounds__(64 * AN_WAVES) void answer_grad_wave_kernel(const OP op, const void* x, long ld, long R, int C,
+                                                                         void* grad, long ldg) {
+  __shared__ int s_idx[AN_WAVES][AN_NAMED];
+  __shared__ float s_add[AN_WAVES][AN_NAMED];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long r = (long)blockIdx.x * AN_WAVES + wave;
+  if (r >= R || op.done()) return;   // no barrier below: a wave keeps to its own row
+  const void* xr = an_row<BF16>(x, ld, r);
+  float v[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int c = lane + 64 * i;
+    v[i] = c < C ? an_at<BF16>(xr, c) : 0.f;
+  }
+  const int ns = op.named();
+  for (int s = lane; s < ns; s += 64) op.mention(r, s, C, s_idx[wave][s], s_add[wave][s]);
+  const typename OP::Row w = op.row(r, lane, C);
+  unsigned char* grow = reinterpret_cast<unsigned char*>(grad) + r * ldg * (BF16 ? 2 : 4);
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int c = lane + 64 * i;
+    if (c < C) store1<BF16>(grow, (size_t)c, OP::dense(w, v[i]));
+  }
+  __threadfence_block();
+  __builtin_amdgcn_wave_barrier();
+  an_write_named<BF16>(s_idx[wave], s_add[wave], ns, lane, 64, 0, C, xr, grow, [&](float u) { return OP::base(w, u); },
+                       [&](float t) { return OP::term(w, t); });
+}
+
+// ---------------------------------------------------------------------------------------------
+// Distillation loss, with the gradient of the sum (or mean) in the same pass
+// ---------------------------------------------------------------------------------------------
+struct DistillArgs {
+  const void* x;
+  const float* teacher;
+  const int64_t* indices;
+  float* row_loss;
+  DistillStat* stats;   // or NULL
+  void* grad;           // or NULL
+  long ld, ldg, R;
+  int C, K, tail;
+  float scale;          // of the gradient: T * (1 or 1 / R)
+  double t2;            // T^2
+  AnTemp temp;
+};
+
+// One wave: the row's loss and statistics.  lane holds the teacher's answers lane and lane + 64: value v, student logit
+// x, `live` where there is one.  s_all: sum of e over the row, s_out: over the classes outside the list (tail only),
+// `all`: the list covers every class.  q[] receives the teacher's probabilities.
+__device__ __forceinline__ DistillStat an_distill_row(const float (&v)[2], const float (&x)[2], const bool (&live)[2], bool bad,
+                                                      float m, double s_all, double s_out, bool all, int tail, double inv_t,
+                                                      double (&q)[2], double& loss) {
+  DistillStat st;
+  st.m = m;
+  st.S = s_all;
+  const bool empty = m == -INFINITY;
+  const double log_s = log(s_all);
+  st.log_q = 0.0;
+  bool some = true;
+  if (!tail) {
+    float vm = fmaxf(live[0] ? v[0] : -INFINITY, live[1] ? v[1] : -INFINITY);
+    vm = an_wave_max(vm);
+    // (a NaN among the values is left out of the maximum and comes back through the sum)
+    const bool nan = __ballot((live[0] && v[0] != v[0]) || (live[1] && v[1] != v[1])) != 0;
+    some = vm != -INFINITY || nan;
+    if (some) {
+      double sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sum += live[i] ? an_exp((double)v[i] - (double)vm) : 0.0;
+      st.log_q = (double)vm + log(an_wave_sum(sum));
+    }
+  }
+  double mass = 0.0, l = 0.0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const double lq = (double)v[i] - st.log_q;
+    q[i] = live[i] && some ? an_exp(lq) : 0.0;
+    mass += q[i];
+    const double lp = empty ? -INFINITY : ((double)x[i] - (double)m) * inv_t - log_s;
+    if (q[i] != 0.0) l += q[i] * (lq - lp);   // (NaN goes in)
+  }
+  mass = an_wave_sum(mass);
+  l = an_wave_sum(l);
+  double rest = 0.0, slope_cut = 0.0;
+  if (tail) {
+    const bool any = __ballot(live[0] || live[1]) != 0;
+    rest = all || !any ? 0.0 : 1.0 - mass;   // (a row without answers teaches nothing)
+    if (!(rest > (double)AN_NO_REST)) rest = 0.0;
+    mass += rest;
+    if (rest > 0.0) {
+      if (empty) {
+        l += INFINITY;
+      } else {
+        const double P = s_out / s_all;
+        l += rest * (log(rest) - log(P));
+        slope_cut = P > 0.0 ? rest / P : (P == 0.0 ? mass : P);
+      }
+    }
+  } else if (some) {
+    mass = mass / mass;   // 1, or NaN
+  }
+  if (bad) l = mass = NAN;
+  st.mass = mass;
+  st.slope = mass - slope_cut;
+  loss = l;
+  return st;
+}
+
+template <int NT, bool BF16>
+struct DistillShared {
+  float v[AN_TOP_MAX], x[AN_TOP_MAX], add[AN_TOP_MAX];
+  int idx[AN_TOP_MAX];
+  float s_max[NT / 64];
+  double s_sum[2][NT / 64];
+  int bad;
+  DistillStat st;
+};
+
+// MARK: the classes of the list are marked in a bitmap (in units of pieces) so that the others can be summed apart:
+// 1 - sum p would lose what is left of it where the student agrees with its teacher.
+template <bool BF16, int NT, int E, bool TAIL>
+__global__ __launch_bounds__(NT) void distill_block_kernel(const DistillArgs a) {
+  constexpr int V = Piece<BF16>::V, NW = NT / 64;
+  __shared__ DistillShared<NT, BF16> sh;
+  extern __shared__ unsigned s_mark[];   // TAIL: one bit per element of the pieces
+  const long r = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  RowPieces<BF16, NT, E> row;
+  row.s = an_span<BF16>(a.x, a.ld, r, a.R, a.C);
+  row.load();
+  const void* xr = an_row<BF16>(a.x, a.ld, r);
+  if (TAIL)
+    for (int i = tid; i < (row.s.pieces * V + 31) / 32; i += NT) s_mark[i] = 0u;
+  if (tid == 0) sh.bad = 0;
+  __syncthreads();
+  if (tid < a.K) {
+    const int64_t j = a.indices[r * a.K + tid];
+    const bool live = j >= 0 && j < a.C;
+    sh.idx[tid] = live ? (int)j : -1;
+    sh.v[tid] = a.teacher[r * a.K + tid];
+    sh.x[tid] = live ? an_at<BF16>(xr, j) : 0.f;
+    if (j >= a.C) sh.bad = 1;
+    if (TAIL && live) {
+      const int b = (int)j + row.s.shift;
+      atomicOr(&s_mark[b >> 5], 1u << (b & 31));
+    }
+  }
+  float m = -INFINITY;
+  row.walk([&](const float (&v)[V], int, int) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) m = fmaxf(m, v[j]);
+  });
+  m = an_wave_max(m);
+  if (lane == 0) sh.s_max[wave] = m;
+  __syncthreads();
+  m = sh.s_max[0];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) m = fmaxf(m, sh.s_max[i]);
+  if (m == -INFINITY && an_block_nan<NT>(row)) m = NAN;
+
+  double S = 0.0, O = 0.0;
+  const float hi = a.temp.hi, lo = a.temp.lo;
+  row.walk([&](const float (&v)[V], int c, int) {
+    float e[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) e[j] = an_exp2(an_arg(v[j], m, hi, lo));
+    S += (double)an_tree<V>(e);
+    if constexpr (TAIL) {
+      // the piece's bits: a byte (bf16) or a nibble (f32); pieces past the row have none and hold zeros
+      unsigned b = 0;
+      if (c < row.s.pieces) b = s_mark[(c * V) >> 5] >> ((c * V) & 31);
+#pragma unroll
+      for (int j = 0; j < V; ++j) e[j] = (b >> j) & 1u ? 0.f : e[j];
+      O += (double)an_tree<V>(e);
+    }
+  });
+  S = an_wave_sum(S);
+  if (TAIL) O = an_wave_sum(O);
+  if (lane == 0) {
+    sh.s_sum[0][wave] = S;
+    if (TAIL) sh.s_sum[1][wave] = O;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    S = O = 0.0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      S += sh.s_sum[0][i];
+      if (TAIL) O += sh.s_sum[1][i];
+    }
+    float v[2], x[2];
+    bool live[2];
+    double q[2], loss;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int k = lane + 64 * i;
+      live[i] = k < a.K && sh.idx[k < a.K ? k : 0] >= 0;
+      v[i] = live[i] ? sh.v[k] : 0.f;
+      x[i] = live[i] ? sh.x[k] : 0.f;
+    }
+    // (more than 1024 classes and at most 128 answers: never all of them)
+    const DistillStat st = an_distill_row(v, x, live, sh.bad != 0, m, S, O, false, TAIL ? 1 : 0, a.temp.inv_t, q, loss);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int k = lane + 64 * i;
+      if (k < a.K) sh.add[k] = (float)q[i];
+    }
+    if (lane == 0) {
+      sh.st = st;
+      a.row_loss[r] = (float)(a.t2 * loss);
+      if (a.stats != nullptr) a.stats[r] = st;
+    }
+  }
+  if (a.grad == nullptr) return;   // uniform
+  __syncthreads();
+  const DistillStat st = sh.st;
+  const bool empty = an_no_gradient(st);
+  const double inv = empty ? 0.0 : 1.0 / st.S;
+  const float mass = (float)(st.mass * inv), slope = (float)(st.slope * inv) * a.scale;
+  unsigned char* grow = reinterpret_cast<unsigned char*>(a.grad) + r * a.ldg * (BF16 ? 2 : 4);
+  row.walk([&](const float (&v)[V], int c, int el) {
+    if (c >= row.s.pieces) return;
+    float g[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) g[j] = empty ? 0.f : an_exp2(an_arg(v[j], m, hi, lo)) * slope;
+    an_store<BF16>(grow, el, a.C, g);
+  });
+  __syncthreads();
+  const float sc = a.scale;
+  an_write_named<BF16>(sh.idx, sh.add, a.K, tid, NT, 0, a.C, xr, grow,
+                       [&](float x) { return empty ? 0.f : sc * (an_exp2(an_arg(x, m, hi, lo)) * mass); },
+                       [&](float q) { return empty ? 0.f : -sc * q; });
+}
+
+template <bool BF16, int E>
+__global__ __launch_bounds__(64 * AN_WAVES) void distill_wave_kernel(const DistillArgs a) {
+  __shared__ int s_idx[AN_WAVES][AN_TOP_MAX];
+  __shared__ float s_add[AN_WAVES][AN_TOP_MAX];
+  __shared__ unsigned s_mark[AN_WAVES][AN_WAVE_C / 32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long r = (long)blockIdx.x * AN_WAVES + wave;
+  if (r >= a.R) return;   // no barrier below: a wave keeps to its own row
+  const void* xr = an_row<BF16>(a.x, a.ld, r);
+  float v[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int c = lane + 64 * i;
+    v[i] = c < a.C ? an_at<BF16>(xr, c) : -INFINITY;
+  }
+  if (lane < AN_WAVE_C / 32) s_mark[wave][lane] = 0u;
+  __builtin_amdgcn_wave_barrier();
+  __threadfence_block();
+  float tv[2], tx[2];
+  bool live[2], beyond = false;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int k = lane + 64 * i;
+    int64_t j = -1;
+    tv[i] = tx[i] = 0.f;
+    if (k < a.K) {
+      j = a.indices[r * a.K + k];
+      beyond |= j >= a.C;
+      live[i] = j >= 0 && j < a.C;
+      if (live[i]) {
+        tv[i] = a.teacher[r * a.K + k];
+        tx[i] = an_at<BF16>(xr, j);
+        atomicOr(&s_mark[wave][j >> 5], 1u << (j & 31));
+      }
+      s_idx[wave][k] = live[i] ? (int)j : -1;
+    } else {
+      live[i] = false;
+    }
+  }
+  const bool bad = __ballot(beyond) != 0;
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < E; ++i) m = fmaxf(m, v[i]);
+  m = an_wave_row_max<E>(v, m);
+  __builtin_amdgcn_wave_barrier();
+  __threadfence_block();
+  double S = 0.0, O = 0.0;
+  int outside = 0;
+  float e32[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int c = lane + 64 * i;
+    const double e = an_exp(((double)v[i] - (double)m) * a.temp.inv_t);
+    e32[i] = (float)e;
+    S += e;
+    const bool in = (s_mark[wave][c >> 5] >> (c & 31)) & 1u;   // E <= 16: c < 1024
+    O += in ? 0.0 : e;
+    outside += c < a.C && !in ? 1 : 0;
+  }
+  S = an_wave_sum(S);
+  O = an_wave_sum(O);
+  const bool all = __ballot(outside != 0) == 0;
+  double q[2], loss;
+  const DistillStat st = an_distill_row(tv, tx, live, bad, m, S, O, all, a.tail, a.temp.inv_t, q, loss);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (lane + 64 * i < a.K) s_add[wave][lane + 64 * i] = (float)q[i];
+  if (lane == 0) {
+    a.row_loss[r] = (float)(a.t2 * loss);
+    if (a.stats != nullptr) a.stats[r] = st;
+  }
+  if (a.grad == nullptr) return;
+  const bool empty = an_no_gradient(st);
+  const double inv = empty ? 0.0 : 1.0 / st.S;
+  const float mass = (float)(st.mass * inv), slope = (float)(st.slope * inv) * a.scale;
+  unsigned char* grow = reinterpret_cast<unsigned char*>(a.grad) + r * a.ldg * (BF16 ? 2 : 4);
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int c = lane + 64 * i;
+    if (c < a.C) store1<BF16>(grow, (size_t)c, empty ? 0.f : e32[i] * slope);
+  }
+  __threadfence_block();
+  __builtin_amdgcn_wave_barrier();
+  const float sc = a.scale;
+  an_write_named<BF16>(s_idx[wave], s_add[wave], a.K, lane, 64, 0, a.C, xr, grow,
+                       [&](float x) { return empty ? 0.f : sc * ((float)an_exp(((double)x - (double)m) * a.temp.inv_t) * mass); },
+                       [&](float t) { return empty ? 0.f : -sc * t; });
+}
+
+// out[0] = scale * sum of x[0..n): one workgroup, every thread adds its own in order, waves in order
+__global__ __launch_bounds__(1024) void answer_sum_kernel(const float* x, long n, double scale, float* out) {
+  __shared__ double s_part[16];
+  double s = 0.0;
+  for (long i = threadIdx.x; i < n; i += 1024) s += (double)x[i];
+  s = an_wave_sum(s);
+  if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = s_part[0];
+    for (int w = 1; w < 16; ++w) s += s_part[w];
+    out[0] = (float)(scale * s);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Which kernel a row length takes
+// ---------------------------------------------------------------------------------------------
+// calls f(E) with the registers a lane needs for C classes, one wave per row
+template <class F>
+bool an_by_wave(int C, F f) {
+  if (C <= 64) f(std::integral_constant<int, 1>());
+  else if (C <= 128) f(std::integral_constant<int, 2>());
+  else if (C <= 256) f(std::integral_constant<int, 4>());
+  else if (C <= 512) f(std::integral_constant<int, 8>());
+  else f(std::integral_constant<int, 16>());
+  return true;
+}
+// calls f(NT, E) with the workgroup and pieces per thread that hold C classes wherever the row starts (a piece more
+// than it fills when aligned); E = 0: the row is read again for every use
+template <bool BF16, class F>
+void an_by_block(int C, F f) {
+  const int pieces = (C + Piece<BF16>::V - 1) / Piece<BF16>::V + 1;
+#define AN_FIT(NT, E) if (pieces <= NT * E) return f(std::integral_constant<int, NT>(), std::integral_constant<int, E>())
+  if constexpr (BF16) {
+    AN_FIT(256, 2); AN_FIT(256, 4); AN_FIT(512, 4); AN_FIT(512, 8); AN_FIT(1024, 7); AN_FIT(1024, 9);
+  } else {
+    AN_FIT(256, 4); AN_FIT(256, 8); AN_FIT(512, 8); AN_FIT(512, 16); AN_FIT(1024, 13); AN_FIT(1024, 17);
+  }
+#undef AN_FIT
+  return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 0>());
+}
+
+bool an_shape_ok(long ld, int R, int C, int K, double temperature) {
+  // (temperatures between 2^-20 and 2^20: their factors stay far inside f32)
+  return R > 0 && C > 0 && C < 0x7ffffff0 && ld >= 0 && K >= 0 && K <= AN_TOP_MAX && K <= C && temperature >= 9.5367431640625e-07 &&
+         temperature <= 1048576.0;
+}
+// The gradient's rows have to lie on their 16-byte grid as the logits' do.
+bool an_grad_layout_ok(const void* x, long ld, const void* g, long ldg, int C, int dtype) {
+  const long es = (long)vqaf_esize(dtype);
+  return ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 15u) == 0 && ((ld - ldg) * es) % 16 == 0 && ldg >= C;
+}
+bool an_element_aligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % vqaf_esize(dtype) == 0; }
+
+template <class OP>
+int an_launch_grad(const OP& op, const void* x, long ld, int R, int C, int dtype, void* grad, long ldg, hipStream_t st) {
+  if (C <= AN_WAVE_C) {
+    const dim3 grid((unsigned)((R + AN_WAVES - 1) / AN_WAVES));
+    an_by_wave(C, [&](auto e) {
+      constexpr int E = decltype(e)::value;
+      if (dtype == VQAF_BF16) hipLaunchKernelGGL((answer_grad_wave_kernel<true, E, OP>), grid, dim3(64 * AN_WAVES), 0, st, op, x, ld, (long)R, C, grad, ldg);
+      else hipLaunchKernelGGL((answer_grad_wave_kernel<false, E, OP>), grid, dim3(64 * AN_WAVES), 0, st, op, x, ld, (long)R, C, grad, ldg);
+    });
+  } else {
+    const int V = dtype == VQAF_BF16 ? 8 : 4;
+    const long segments = ((long)C + V - 1 + (V - 1)) / V / (AN_ST * AN_SP) + 1;
+    VQAF_REQUIRE(segments * R < 0x7fffffffL, VQAF_E_SHAPE);
+    const dim3 grid((unsigned)(segments * R));
+    if (dtype == VQAF_BF16) hipLaunchKernelGGL((answer_grad_block_kernel<true, OP>), grid, dim3(AN_ST), 0, st, op, x, ld, (long)R, C, (int)segments, grad, ldg);
+    else hipLaunchKernelGGL((answer_grad_block_kernel<false, OP>), grid, dim3(AN_ST), 0, st, op, x, ld, (long)R, C, (int)segments, grad, ldg);
+  }
+  VQAF_LAUNCH_CHECK();
+}
+
+template <bool BF16>
+void an_launch_logprobs(const LogprobArgs& a, hipStream_t st) {
+  if (a.C <= AN_WAVE_C) {
+    an_by_wave(a.C, [&](auto e) {
+      hipLaunchKernelGGL((logprob_wave_kernel<BF16, decltype(e)::value>), dim3((unsigned)((a.R + AN_WAVES - 1) / AN_WAVES)),
+                         dim3(64 * AN_WAVES), 0, st, a);
+    });
+  } else {
+    an_by_block<BF16>(a.C, [&](auto nt, auto e) {
+      hipLaunchKernelGGL((logprob_block_kernel<BF16, decltype(nt)::value, decltype(e)::value>), dim3((unsigned)a.R),
+                         dim3(decltype(nt)::value), 0, st, a);
+    });
+  }
+}
+
+template <bool BF16>
+int an_launch_distill(const DistillArgs& a, hipStream_t st) {
+  if (a.C <= AN_WAVE_C) {
+    an_by_wave(a.C, [&](auto e) {
+      hipLaunchKernelGGL((distill_wave_kernel<BF16, decltype(e)::value>), dim3((unsigned)((a.R + AN_WAVES - 1) / AN_WAVES)),
+                         dim3(64 * AN_WAVES), 0, st, a);
+    });
+  } else {
+    const size_t mark = a.tail ? ((size_t)a.C + 2 * Piece<BF16>::V + 31) / 32 * 4 : 0;
+    VQAF_REQUIRE(mark <= 49152, VQAF_E_SHAPE);   // 393 thousand classes with the remaining mass as an event
+    an_by_block<BF16>(a.C, [&](auto nt, auto e) {
+      constexpr int NT = decltype(nt)::value, E = decltype(e)::value;
+      if (a.tail) hipLaunchKernelGGL((distill_block_kernel<BF16, NT, E, true>), dim3((unsigned)a.R), dim3(NT), mark, st, a);
+      else hipLaunchKernelGGL((distill_block_kernel<BF16, NT, E, false>), dim3((unsigned)a.R), dim3(NT), 0, st, a);
+    });
+  }
+  VQAF_LAUNCH_CHECK();
+}
+
+}  // namespace
+
+extern "C" int vqaf_token_logprobs(const void* logits, long ld, const int64_t* targets, int R, int C, int T, int K, int dtype,
+                                   double temperature, float* logprobs, float* entropy, float* top_logprobs,
+                                   int64_t* top_indices, float* stats, vqaf_stream_t stream) {
+  VQAF_ENTRY();
+  VQAF_REQUIRE(logits != nullptr, VQAF_E_NULL);
+  VQAF_REQUIRE(an_shape_ok(ld, R, C, K, temperature) && T >= 0 && T <= AN_TOP_MAX, VQAF_E_SHAPE);
+  VQAF_REQUIRE(vqaf_dtype_ok(dtype), VQAF_E_DTYPE);
+  VQAF_REQUIRE(T == 0 || (targets != nullptr && logprobs != nullptr), VQAF_E_NULL);
+  VQAF_REQUIRE(K == 0 || (top_logprobs != nullptr && top_indices != nullptr), VQAF_E_NULL);
+  VQAF_REQUIRE(an_element_aligned(logits, dtype), VQAF_E_ALIGN);
+  LogprobArgs a;
+  a.x = logits; a.targets = targets; a.logprobs = logprobs; a.entropy = entropy;
+  a.top_logprobs = top_logprobs; a.top_indices = top_indices; a.stats = stats;
+  a.ld = ld; a.R = R; a.C = C; a.T = T; a.K = K;
+  a.temp = an_temp(temperature);
+  if (dtype == VQAF_BF16) an_launch_logprobs<true>(a, (hipStream_t)stream);
+  else an_launch_logprobs<false>(a, (hipStream_t)stream);
+  VQAF_LAUNCH_CHECK();
+}
+
+extern "C" int vqaf_token_logprobs_bwd(const void* logits, long ld, const int64_t* targets, const int64_t* top_indices, int R,
+                                       int C, int T, int K, int dtype, double temperature, const float* stats,
+                                       const float* entropy, const float* g_logprobs, const float* g_entropy,
+                                       const float* g_top, void* grad, long ld_grad, vqaf_stream_t stream) {
+  VQAF_ENTRY();
+  VQAF_REQUIRE(logits != nullptr && stats != nullptr && grad != nullptr, VQAF_E_NULL);
+  VQAF_REQUIRE(an_shape_ok(ld, R, C, K, temperature) && T >= 0 && T <= AN_TOP_MAX, VQAF_E_SHAPE);
+  VQAF_REQUIRE(vqaf_dtype_ok(dtype), VQAF_E_DTYPE);
+  VQAF_REQUIRE(g_logprobs == nullptr || T == 0 || targets != nullptr, VQAF_E_NULL);
+  VQAF_REQUIRE(g_top == nullptr || K == 0 || top_indices != nullptr, VQAF_E_NULL);
+  VQAF_REQUIRE(g_entropy == nullptr || entropy != nullptr, VQAF_E_NULL);
+  VQAF_REQUIRE(an_element_aligned(logits, dtype) && an_grad_layout_ok(logits, ld, grad, ld_grad, C, dtype), VQAF_E_ALIGN);
+  LogprobGrad op;
+  op.targets = targets; op.top_indices = top_indices; op.stats = stats; op.entropy = entropy;
+  op.g_lp = T > 0 ? g_logprobs : nullptr; op.g_ent = g_entropy; op.g_top = K > 0 ? g_top : nullptr;
+  op.T = T; op.K = K;
+  op.temp = an_temp(temperature);
+  return an_launch_grad(op, logits, ld, R, C, dtype, grad, ld_grad, (hipStream_t)stream);
+}
+
+extern "C" int vqaf_distill(const void* logits, long ld, const float* teacher, const int64_t* indices, int R, int C, int K,
+                            int dtype, double temperature, int tail, float* row_loss, double* stats, void* grad,
+                            long ld_grad, double scale, float* loss, vqaf_stream_t stream) {
+  VQAF_ENTRY();
+  VQAF_REQUIRE(logits && teacher && indices && row_loss, VQAF_E_NULL);
+  VQAF_REQUIRE(an_shape_ok(ld, R, C, 0, temperature) && K >= 1 && K <= AN_TOP_MAX, VQAF_E_SHAPE);
+  VQAF_REQUIRE(vqaf_dtype_ok(dtype), VQAF_E_DTYPE);
+  VQAF_REQUIRE(an_element_aligned(logits, dtype), VQAF_E_ALIGN);
+  VQAF_REQUIRE(grad == nullptr || an_grad_layout_ok(logits, ld, grad, ld_grad, C, dtype), VQAF_E_ALIGN);
+  DistillArgs a;
+  a.x = logits; a.teacher = teacher; a.indices = indices; a.row_loss = row_loss;
+  a.stats = reinterpret_cast<DistillStat*>(stats); a.grad = grad;
+  a.ld = ld; a.ldg = ld_grad; a.R = R; a.C = C; a.K = K; a.tail = tail != 0;
+  a.scale = (float)(temperature * scale);
+  a.t2 = temperature * temperature;
+  a.temp = an_temp(temperature);
+  const int rc = dtype == VQAF_BF16 ? an_launch_distill<true>(a, (hipStream_t)stream)
+                                    : an_launch_distill<false>(a, (hipStream_t)stream);
+  if (rc != VQAF_OK || loss == nullptr) return rc;
+  hipLaunchKernelGGL(answer_sum_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, row_loss, (long)R, scale, loss);
+  VQAF_LAUNCH_CHECK();
+}
+
+extern "C" int vqaf_distill_bwd(const void* logits, long ld, const float* teacher, const int64_t* indices, int R, int C, int K,
+                                int dtype, double temperature, const double* stats, const float* up, int up_step, int skip_unit,
+                                double scale, void* grad, long ld_grad, vqaf_stream_t stream) {
+  VQAF_ENTRY();
+  VQAF_REQUIRE(logits && teacher && indices && stats && up && grad, VQAF_E_NULL);
+  VQAF_REQUIRE(an_shape_ok(ld, R, C, 0, temperature) && K >= 1 && K <= AN_TOP_MAX && (up_step == 0 || up_step == 1), VQAF_E_SHAPE);
+  VQAF_REQUIRE(vqaf_dtype_ok(dtype), VQAF_E_DTYPE);
+  VQAF_REQUIRE(an_element_aligned(logits, dtype) && an_grad_layout_ok(logits, ld, grad, ld_grad, C, dtype), VQAF_E_ALIGN);
+  DistillGrad op;
+  op.teacher = teacher; op.indices = indices; op.stats = reinterpret_cast<const DistillStat*>(stats); op.up = up;
+  op.up_step = up_step; op.K = K; op.scale = (float)(temperature * scale);
+  op.skip_unit = skip_unit != 0 && up_step == 0;
+  op.temp = an_temp(temperature);
+  return an_launch_grad(op, logits, ld, R, C, dtype, grad, ld_grad, (hipStream_t)stream);
+}

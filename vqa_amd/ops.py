@@ -6,11 +6,12 @@ device memory, streams and autograd bookkeeping only; the arithmetic is in the k
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
-
+import contextlib
 import weakref
+from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import check, dtype_code, load, ptr, stream_ptr
@@ -810,6 +811,235 @@ def unit_gradient(loss: torch.Tensor) -> torch.Tensor:
         one = torch.ones((), dtype=loss.dtype, device=loss.device)
         _unit_grads[key] = one
     return one
+
+
+# --------------------------------------------------------------------------------------------
+# Answer scores and distillation
+# --------------------------------------------------------------------------------------------
+ANSWERS_MAX = 128  # given tokens, alternatives and teacher's answers per row
+
+
+class TokenLogprobs(NamedTuple):
+    """What `token_logprobs` returns; None where it was not asked for."""
+    logprobs: Optional[torch.Tensor]
+    entropy: Optional[torch.Tensor]
+    top_logprobs: Optional[torch.Tensor]
+    top_indices: Optional[torch.Tensor]
+
+
+def _on(device: torch.device):
+    """Makes `device` the current one for the launches inside (a launch goes to the current device, whatever its
+    stream)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _answer_rows(logits: torch.Tensor):
+    """(logits as (R,C) with unit inner stride, its row pitch)."""
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits need a dimension of classes, got shape {tuple(logits.shape)}")
+    require_gpu(logits)
+    dtype_code(logits)
+    C = logits.shape[-1]
+    x = logits if logits.dim() == 2 else logits.reshape(-1, C)
+    if C > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    return x, (x.stride(0) if x.shape[0] > 1 else C)
+
+
+def _grad_rows(x: torch.Tensor, ld: int) -> torch.Tensor:
+    """An (R,C) tensor of x's dtype whose rows lie on the 16-byte grid as x's do."""
+    R, C = x.shape
+    per = 16 // x.element_size()
+    off, ldg = (x.data_ptr() // x.element_size()) % per, C + (ld - C) % per
+    if off == 0 and ldg == C:
+        return torch.empty(R, C, dtype=x.dtype, device=x.device)
+    buf = torch.empty(off + R * ldg, dtype=x.dtype, device=x.device)
+    return buf.as_strided((R, C), (ldg, 1), off)
+
+
+def _temperature(t: float) -> float:
+    t = float(t)
+    if not 2.0 ** -20 <= t <= 2.0 ** 20:
+        raise ValueError(f"temperature has to be in [2^-20, 2^20], got {t}")
+    return t
+
+
+def _f32(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if g is None else g.to(torch.float32).contiguous()
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, ld, targets, top, temperature, entropy, stats):
+        R, C = x.shape
+        dev = x.device
+        T = 0 if targets is None else targets.shape[1]
+        lp = torch.empty(R, T, dtype=torch.float32, device=dev) if targets is not None else None
+        ent = torch.empty(R, dtype=torch.float32, device=dev) if entropy else None
+        tl = torch.empty(R, top, dtype=torch.float32, device=dev) if top else None
+        ti = torch.empty(R, top, dtype=torch.int64, device=dev) if top else None
+        st = torch.empty(R, 2, dtype=torch.float32, device=dev) if stats else None
+        with _on(dev):
+            check(load().vqaf_token_logprobs(x.data_ptr(), ld, ptr(targets), R, C, T, top, dtype_code(x), temperature,
+                                             ptr(lp), ptr(ent), ptr(tl), ptr(ti), ptr(st), stream_ptr(dev)),
+                  "vqaf_token_logprobs")
+        if stats:
+            ctx.save_for_backward(x, targets, ti, st, ent)
+            ctx.meta = (ld, T, top, temperature)
+            ctx.set_materialize_grads(False)
+            if ti is not None:
+                ctx.mark_non_differentiable(ti)
+        return lp, ent, tl, ti
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_lp, g_ent, g_top, _g_idx):
+        x, targets, ti, st, ent = ctx.saved_tensors
+        ld, T, top, temperature = ctx.meta
+        if g_lp is None and g_ent is None and g_top is None:
+            return (None,) * 7
+        R, C = x.shape
+        g_lp, g_ent, g_top = _f32(g_lp), _f32(g_ent), _f32(g_top)
+        grad = _grad_rows(x, ld)
+        with _on(x.device):
+            check(load().vqaf_token_logprobs_bwd(x.data_ptr(), ld, ptr(targets), ptr(ti), R, C, T, top, dtype_code(x),
+                                                 temperature, ptr(st), ptr(ent), ptr(g_lp), ptr(g_ent), ptr(g_top),
+                                                 grad.data_ptr(), grad.stride(0), stream_ptr(x.device)),
+                  "vqaf_token_logprobs_bwd")
+        return (grad,) + (None,) * 6
+
+
+def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0, temperature: float = 1.0,
+                   entropy: bool = True) -> TokenLogprobs:
+    """Log probabilities of given tokens under softmax(logits / temperature), the entropy of that distribution and its
+    `top` most probable tokens, from one read of the logits (vqaf_token_logprobs).
+
+    logits (..., C) f32 or bf16.  targets (...) or (..., T) int64, at most 128 for each row: a negative one is none
+    (log probability 0, no gradient), one past the classes gives NaN.  Results are f32 with the leading dimensions of
+    `logits`; alternatives come in falling order, ties by the lowest index.  The log probabilities and the entropy are
+    differentiable.  Rows of nothing but -inf have log probabilities -inf, entropy 0 and no gradient; a NaN or +inf
+    makes its row NaN."""
+    x, ld = _answer_rows(logits)
+    R, C = x.shape
+    lead = logits.shape[:-1]
+    temperature = _temperature(temperature)
+    top = int(top)
+    if not 0 <= top <= min(C, ANSWERS_MAX):
+        raise ValueError(f"top has to be in [0, {min(C, ANSWERS_MAX)}], got {top}")
+    tg, given = None, None
+    if targets is not None:
+        given = targets.shape
+        if given != lead and given[:-1] != lead:
+            raise ValueError(f"targets of shape {tuple(given)} do not fit logits of shape {tuple(logits.shape)}")
+        if targets.dtype.is_floating_point or targets.dtype.is_complex or targets.dtype == torch.bool:
+            raise TypeError(f"targets are token indices, got {targets.dtype}")
+        if targets.device != logits.device:
+            raise ValueError(f"targets are on {targets.device}, logits on {logits.device}")
+        T = 1 if given == lead else given[-1]
+        if T > ANSWERS_MAX:
+            raise ValueError(f"at most {ANSWERS_MAX} targets for each row, got {T}")
+        tg = targets.to(torch.int64).reshape(R, T).contiguous()
+    needs = torch.is_grad_enabled() and x.requires_grad
+    if R == 0:
+        z = x.sum(1, dtype=torch.float32)
+        lp = None if tg is None else (z[:, None].expand(0, tg.shape[1]) * 1.0)
+        ent, tl = (z if entropy else None), (z[:, None].expand(0, top) * 1.0 if top else None)
+        ti = torch.empty(0, top, dtype=torch.int64, device=x.device) if top else None
+    else:
+        lp, ent, tl, ti = _TokenLogprobs.apply(x, ld, tg, top, temperature, bool(entropy), needs)
+    if len(lead) == 1:
+        if lp is not None and given == lead:
+            lp = lp.view(given)
+        return TokenLogprobs(lp, ent, tl, ti)
+    return TokenLogprobs(None if lp is None else lp.view(given), None if ent is None else ent.view(lead),
+                         None if tl is None else tl.view(*lead, top), None if ti is None else ti.view(*lead, top))
+
+
+class _Distill(torch.autograd.Function):
+    """Row losses, or their sum / mean with the gradient for an incoming gradient of 1 formed in the same pass."""
+
+    @staticmethod
+    def forward(ctx, x, ld, teacher, indices, temperature, tail, scale, needs):
+        R, C = x.shape
+        K = teacher.shape[1]
+        dev = x.device
+        rows = torch.empty(R, dtype=torch.float32, device=dev)
+        stats = torch.empty(R, 5, dtype=torch.float64, device=dev) if needs else None
+        whole = scale is not None
+        grad = _grad_rows(x, ld) if needs and whole else None
+        loss = torch.empty((), dtype=torch.float32, device=dev) if whole else None
+        with _on(dev):
+            check(load().vqaf_distill(x.data_ptr(), ld, ptr(teacher), ptr(indices), R, C, K, dtype_code(x), temperature,
+                                      int(tail), ptr(rows), ptr(stats), None if grad is None else grad.data_ptr(),
+                                      0 if grad is None else grad.stride(0), scale if whole else 1.0, ptr(loss),
+                                      stream_ptr(dev)), "vqaf_distill")
+        if needs:
+            ctx.save_for_backward(x, teacher, indices, stats)
+            ctx.meta = (ld, K, temperature, scale if whole else 1.0, whole)
+            ctx.unit = grad
+        return loss if whole else rows
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, up):
+        x, teacher, indices, stats = ctx.saved_tensors
+        ld, K, temperature, scale, whole = ctx.meta
+        none = (None,) * 7
+        grad, ctx.unit = ctx.unit, None   # handed out once: a second backward forms its own
+        if grad is not None and up is _unit_grads.get((up.device, up.dtype)):
+            return (grad,) + none
+        ready = grad is not None
+        if not ready:
+            grad = _grad_rows(x, ld)
+        up = _f32(up)
+        with _on(x.device):
+            check(load().vqaf_distill_bwd(x.data_ptr(), ld, ptr(teacher), ptr(indices), x.shape[0], x.shape[1], K,
+                                          dtype_code(x), temperature, ptr(stats), ptr(up), 0 if whole else 1, int(ready),
+                                          scale, grad.data_ptr(), grad.stride(0), stream_ptr(x.device)),
+                  "vqaf_distill_bwd")
+        return (grad,) + none
+
+
+def distill_loss(logits: torch.Tensor, teacher: torch.Tensor, indices: torch.Tensor, temperature: float = 1.0,
+                 tail: bool = False, reduction: str = "mean") -> torch.Tensor:
+    """temperature^2 * KL(teacher || softmax(logits / temperature)) over a teacher's top answers (vqaf_distill).
+
+    logits (..., C) f32 or bf16; teacher (..., K) the teacher's log probabilities AT THIS TEMPERATURE of the answers
+    `indices` (..., K) int64, K <= 128 -- top_logprobs and top_indices of `token_logprobs(teacher_logits, top=K,
+    temperature=temperature)`.  tail=False divides them by their sum (any constant per row cancels); tail=True keeps
+    them and takes the mass that they leave as one more event, met by all other classes together.  A negative index is
+    no answer, and a row without answers has no loss and no gradient; an index past the classes makes its row NaN.
+    reduction: "mean" over the rows, "sum", or "none" (f32, the leading dimensions of `logits`).  The teacher's side is
+    constant.  `loss.backward(gradient=unit_gradient(loss))` hands on the gradient that the forward pass formed; any
+    other incoming gradient forms it again, rounded once."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction has to be mean, sum or none, got {reduction!r}")
+    x, ld = _answer_rows(logits)
+    R, C = x.shape
+    lead = logits.shape[:-1]
+    temperature = _temperature(temperature)
+    if teacher.shape != indices.shape or teacher.shape[:-1] != lead or teacher.dim() != logits.dim():
+        raise ValueError(f"teacher {tuple(teacher.shape)} and indices {tuple(indices.shape)} do not fit logits of shape "
+                         f"{tuple(logits.shape)}")
+    K = teacher.shape[-1]
+    if not 1 <= K <= ANSWERS_MAX:
+        raise ValueError(f"between 1 and {ANSWERS_MAX} answers for each row, got {K}")
+    if not teacher.dtype.is_floating_point:
+        raise TypeError(f"teacher holds log probabilities, got {teacher.dtype}")
+    if indices.dtype.is_floating_point or indices.dtype.is_complex or indices.dtype == torch.bool:
+        raise TypeError(f"indices are token indices, got {indices.dtype}")
+    if teacher.device != logits.device or indices.device != logits.device:
+        raise ValueError(f"logits are on {logits.device}, teacher on {teacher.device}, indices on {indices.device}")
+    if R == 0:
+        rows = x.sum(1, dtype=torch.float32)
+        return rows.view(lead) if reduction == "none" else rows.sum() if reduction == "sum" else rows.mean()
+    v = teacher.detach().to(torch.float32).reshape(R, K).contiguous()
+    idx = indices.to(torch.int64).reshape(R, K).contiguous()
+    scale = {"mean": 1.0 / R, "sum": 1.0, "none": None}[reduction]
+    out = _Distill.apply(x, ld, v, idx, temperature, bool(tail), scale, torch.is_grad_enabled() and x.requires_grad)
+    return out.view(lead) if scale is None and len(lead) != 1 else out
 
 
 def gemm_bf16_supported(lda: int, a_kmajor: bool, ldb: int, b_kmajor: bool, M: int, N: int, K: int) -> bool:
