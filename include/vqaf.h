@@ -844,6 +844,22 @@ int vqaf_wgrad_tn(const void* gy, long ldg, const void* x, long ldx, int M, int 
                   int gw_dtype, void* gb, int gb_dtype, void* workspace, size_t workspace_bytes,
                   vqaf_stream_t stream);
 
+/* Linear layers in eight-bit integers, a scale for each token and each output channel: the scoring passes of the
+ * encoders (no gradient).  vqaf_quantize_rows: scale (M) f32 = max(max|x_m| / 127, 2^-126), q (M, ldq) = x / scale
+ * rounded half to even as if the quotient were exact, zeros from K to ldq (ldq a multiple of 16, q 16-byte aligned);
+ * x (M,K) `dtype` with any row pitch and element alignment.  A row with NaN or an infinity has scale NaN, q zero.
+ * vqaf_int8_linear: y (M,N) `y_dtype` = (sum_k q_mk w_nk) scale_m w_scale_n + bias_n with the rows of x quantised so
+ * and the weights w (N,K) as vqaf_quantize_rows left them: rows of whole 16-byte pieces (ldw a multiple of 16 and at
+ * least K rounded up to it; what lies between is never counted).  The integer sum is exact (K <= 131072); scales, bias
+ * (N) `bias_dtype` or NULL and the rounding follow in f32.  workspace: vqaf_int8_linear_workspace_bytes(M, K) bytes of
+ * device memory, 16-byte aligned (0 for a few tokens: one launch then does it all). */
+int vqaf_quantize_rows(const void* x, long ldx, int M, int K, int dtype, int8_t* q, long ldq, float* scale,
+                       vqaf_stream_t stream);
+size_t vqaf_int8_linear_workspace_bytes(int M, int K);
+int vqaf_int8_linear(const void* x, long ldx, int x_dtype, const int8_t* w, long ldw, const float* w_scale,
+                     const void* bias, int bias_dtype, int M, int N, int K, void* y, long ldy, int y_dtype,
+                     void* workspace, size_t workspace_bytes, vqaf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -197,6 +197,10 @@ SIGNATURES = {
                                c_long, _P]),
     "vqaf_wgrad_tn_supported": (c_int, [c_long, c_long, c_long, c_int, c_int, c_int]),
     "vqaf_wgrad_tn_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "vqaf_quantize_rows": (c_int, [_P, c_long, c_int, c_int, c_int, _P, c_long, _P, _P]),
+    "vqaf_int8_linear_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "vqaf_int8_linear": (c_int, [_P, c_long, c_int, _P, c_long, _P, _P, c_int, c_int, c_int, c_int, _P, c_long, c_int, _P,
+                                 c_size_t, _P]),
     "vqaf_wgrad_tn": (c_int, [_P, c_long, _P, c_long, c_int, c_int, c_int, _P, c_long, c_int, _P, c_int, _P, c_size_t,
                               _P]),
 }

@@ -1151,6 +1151,97 @@ def wgrad_tn(gy2: torch.Tensor, x2: torch.Tensor, w_dtype: torch.dtype = torch.b
     return gw, gb
 
 
+# --------------------------------------------------------------------------------------------
+# Linear layers in eight-bit integers
+# --------------------------------------------------------------------------------------------
+INT8_MAX_K = 131072  # the integer sum stays inside 32 bits
+
+
+def _int8_rows(x: torch.Tensor, what: str):
+    require_gpu(x)
+    dtype_code(x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{what} needs a last dimension, got shape {tuple(x.shape)}")
+    if x.shape[-1] > INT8_MAX_K:
+        raise ValueError(f"{what}: at most {INT8_MAX_K} columns, got {x.shape[-1]}")
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if x2.shape[1] > 1 and x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    return x2, (x2.stride(0) if x2.shape[0] > 1 else x2.shape[1])
+
+
+@torch.no_grad()
+def quantize_rows(x: torch.Tensor):
+    """(q (..., K) int8, scale (...) f32) with q = x / scale rounded half to even and scale = max|row| / 127
+    (vqaf_quantize_rows): a Linear layer's weight (out, in), one scale for each output channel, as `int8_linear` takes
+    it.  q is laid out in rows of whole 128-byte pieces."""
+    x2, ld = _int8_rows(x, "quantize_rows")
+    M, K = x2.shape
+    pitch = (K + 127) // 128 * 128
+    q = torch.empty(M, pitch, dtype=torch.int8, device=x.device)
+    scale = torch.empty(M, dtype=torch.float32, device=x.device)
+    if M:
+        with _on(x.device):
+            check(load().vqaf_quantize_rows(x2.data_ptr(), ld, M, K, dtype_code(x2), q.data_ptr(), pitch, ptr(scale),
+                                            stream_ptr(x.device)), "vqaf_quantize_rows")
+    lead = x.shape[:-1]
+    return (q[:, :K] if len(lead) == 1 else q.view(*lead, pitch)[..., :K]), scale.view(lead)
+
+
+def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x (..., K) f32 or bf16 through a Linear layer held in eight-bit integers: weight (N,K) int8 and weight_scale (N)
+    f32 from `quantize_rows`, bias (N) f32 or bf16 or None; the tokens are quantised row by row on the way in
+    (vqaf_int8_linear).  Returns (..., N) in out_dtype (default: x's).  Weights in rows that are not whole 16-byte
+    pieces are copied into such rows first.  There is no gradient: an input that requires one is refused while
+    gradients are recorded."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight_scale, bias)):
+        raise RuntimeError("int8_linear has no gradient: call it under torch.no_grad(), or train the layer in bf16")
+    x2, ld = _int8_rows(x, "int8_linear")
+    if weight.dim() != 2 or weight.dtype != torch.int8:
+        raise TypeError(f"weight has to be (N,K) int8, got {tuple(weight.shape)} {weight.dtype}")
+    N, K = weight.shape
+    M = x2.shape[0]
+    if x2.shape[1] != K or N < 1:
+        raise ValueError(f"x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
+    if weight_scale.shape != (N,) or weight_scale.dtype != torch.float32:
+        raise ValueError(f"weight_scale has to be ({N},) float32, got {tuple(weight_scale.shape)} {weight_scale.dtype}")
+    if bias is not None and bias.shape != (N,):
+        raise ValueError(f"bias has to be ({N},), got {tuple(bias.shape)}")
+    for t in (weight, weight_scale, bias):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"x is on {x.device}, a parameter on {t.device}")
+    dt = out_dtype or x.dtype
+    code = _lib.BF16 if dt == torch.bfloat16 else _lib.F32
+    if dt not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"out_dtype has to be float32 or bfloat16, got {dt}")
+    if bias is not None:
+        dtype_code(bias)
+        bias = bias.contiguous()
+    ldw = weight.stride(0) if N > 1 else (K + 15) // 16 * 16
+    fits = weight.stride(1) == 1 or K == 1
+    if N == 1 and fits:   # one row: its pitch says nothing, its last piece has to be there
+        fits = weight.storage_offset() + ldw <= weight.untyped_storage().nbytes()
+    elif fits:
+        fits = ldw % 16 == 0 and ldw >= K and weight.storage_offset() + (N - 1) * ldw + (K + 15) // 16 * 16 <= \
+            weight.untyped_storage().nbytes()
+    if not fits or weight.data_ptr() % 16:
+        whole = torch.zeros(N, (K + 15) // 16 * 16, dtype=torch.int8, device=x.device)
+        whole[:, :K] = weight
+        weight, ldw = whole, whole.shape[1]
+    y = torch.empty(M, N, dtype=dt, device=x.device)
+    if M:
+        lib = load()
+        need = lib.vqaf_int8_linear_workspace_bytes(M, K)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        with _on(x.device):
+            check(lib.vqaf_int8_linear(x2.data_ptr(), ld, dtype_code(x2), weight.data_ptr(), ldw,
+                                       ptr(weight_scale.contiguous()), ptr(bias),
+                                       dtype_code(bias) if bias is not None else 0, M, N, K, y.data_ptr(), N, code, ptr(ws),
+                                       need, stream_ptr(x.device)), "vqaf_int8_linear")
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+
+
 def keep_count(n_tokens: int, prune_ratio: float) -> int:
     """k = max(1, int(N * (1 - prune_ratio))) in Python double arithmetic (utils/fusion.py:41)."""
     return max(1, int(n_tokens * (1 - prune_ratio)))
