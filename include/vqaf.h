@@ -746,7 +746,7 @@ int vqaf_token_logprobs_bwd(const void* logits, long ld, const int64_t* targets,
  * the same read of the logits.  loss, if non-NULL, receives scale * sum of rows, added in a fixed order.  stats (R,5)
  * f64, or NULL, receives what vqaf_distill_bwd needs: the gradient for an incoming gradient `up` in device memory, one
  * for each row (up_step 1) or a scalar (0), times scale.  skip_unit (scalar only): leave grad as it is where up[0] is
- * exactly 1, for a caller who has the forward's gradient in it.  K in [1, 128].  With tail at most 393000 classes. */
+ * exactly 1, for a caller who has the forward's gradient in it.  K in [1, 128], at most 393000 classes. */
 int vqaf_distill(const void* logits, long ld, const float* teacher, const int64_t* indices, int R, int C, int K,
                  int dtype, double temperature, int tail, float* row_loss, double* stats, void* grad, long ld_grad,
                  double scale, float* loss, vqaf_stream_t stream);

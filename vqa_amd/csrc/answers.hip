@@ -130,6 +130,7 @@ __device__ __forceinline__ double an_exp(double t) {
 struct AnTemp {
   float hi, lo;
   double inv_t;
+  double delta;   // hi = log2(e) / T * (1 + delta)
 };
 inline AnTemp an_temp(double temperature) {
   AnTemp t;
@@ -137,6 +138,7 @@ inline AnTemp an_temp(double temperature) {
   const double c = AN_LOG2E * t.inv_t;
   t.hi = (float)c;
   t.lo = (float)(c - (double)t.hi);
+  t.delta = (double)t.hi / c - 1.0;
   return t;
 }
 // (x - m) log2(e) / T.  x = -inf gives -inf (the second term, of either sign, stays finite); NaN comes through the first.
@@ -166,13 +168,12 @@ __device__ __forceinline__ void an_unpack(const u32x4 r, float (&v)[Piece<BF16>:
   }
 }
 
-// Geometry of one row: its first element lies `shift` elements into piece 0.  `lo` and `hi` bound the memory of the
-// whole matrix: a piece that reaches outside it (at the very first or last row only) is read element by element.
+// Geometry of one row: its first element lies `shift` elements into piece 0.  A piece that reaches outside the memory of
+// the whole matrix (at the very first or last row only) is read element by element.
 struct Span {
   const unsigned char* first;   // address of piece 0
-  const unsigned char* lo;
-  const unsigned char* hi;
   int shift, pieces, C;
+  int skip_lo, skip_hi;         // 1: piece 0 / the last piece reaches outside the matrix
 };
 template <bool BF16>
 __device__ __forceinline__ Span an_span(const void* base, long ld, long row, long rows, int C) {
@@ -182,11 +183,26 @@ __device__ __forceinline__ Span an_span(const void* base, long ld, long row, lon
   const unsigned char* r = b + row * ld * ES;
   s.shift = (int)((reinterpret_cast<uintptr_t>(r) & 15u) / ES);
   s.first = r - s.shift * ES;
-  s.lo = b;
-  s.hi = b + ((rows - 1) * ld + C) * ES;
   s.pieces = (s.shift + C + Piece<BF16>::V - 1) / Piece<BF16>::V;
   s.C = C;
+  s.skip_lo = s.first < b ? 1 : 0;
+  s.skip_hi = s.first + (long)s.pieces * 16 > b + ((rows - 1) * ld + C) * ES ? 1 : 0;
   return s;
+}
+// The largest of two bf16 pairs as signed 16-bit integers: their order is that of the values as long as one of them is
+// not negative (a negative result says that none was; NaN with a positive sign comes out above infinity).
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ unsigned an_pkmax(unsigned a, unsigned b) {
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(s16x2, a), __builtin_bit_cast(s16x2, b)));
+}
+// ... and where all are negative: the smallest as unsigned ones is the value nearest to zero
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ unsigned an_pkmin(unsigned a, unsigned b) {
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+__device__ __forceinline__ int an_pkmax1(unsigned a) {
+  const int lo = (int)(short)a, hi = (int)a >> 16;
+  return lo > hi ? lo : hi;
 }
 // Elements of piece c outside the row become -inf.  `el` = column of the piece's first element.
 template <bool BF16>
@@ -231,16 +247,17 @@ struct RowPieces {
   Span s;
   u32x4 raw[E > 0 ? E : 1];
 
-  // one piece; pieces past the row read piece 1, which lies inside it (rows here have more than 1024 classes)
+  // One piece.  Pieces past the row, and those that reach outside the matrix, read piece 1 instead, which lies inside
+  // the row (rows here have more than 1024 classes).
   __device__ __forceinline__ u32x4 fetch(int c) const {
-    const unsigned char* p = s.first + (long)c * 16;
-    const bool safe = c < s.pieces && p >= s.lo && p + 16 <= s.hi;
-    return *reinterpret_cast<const u32x4*>(safe ? p : s.first + 16);
+    const bool safe = c >= s.skip_lo && c < s.pieces - s.skip_hi;
+    return *reinterpret_cast<const u32x4*>(s.first + (size_t)(safe ? (unsigned)c * 16u : 16u));
   }
   __device__ __forceinline__ u32x4 finish(u32x4 r, int c) const {
-    const unsigned char* p = s.first + (long)c * 16;
     const int el = c * V - s.shift;
-    if (c < s.pieces && (p < s.lo || p + 16 > s.hi)) r = an_load_edge<BF16>(s, el);
+    if (s.skip_lo + s.skip_hi != 0) {   // uniform
+      if ((c == 0 && s.skip_lo) || (c == s.pieces - 1 && s.skip_hi)) r = an_load_edge<BF16>(s, el);
+    }
     return an_mask<BF16>(r, el, s.C);
   }
   __device__ __forceinline__ void load() {
@@ -249,6 +266,76 @@ struct RowPieces {
       for (int i = 0; i < E; ++i) raw[i] = fetch((int)threadIdx.x + i * NT);
 #pragma unroll
       for (int i = 0; i < E; ++i) raw[i] = finish(raw[i], (int)threadIdx.x + i * NT);
+    }
+  }
+  // The thread's largest value; NaN counts as the largest or not at all.
+  __device__ __forceinline__ float max() const {
+    if constexpr (BF16) {
+      unsigned k = 0x80008000u;   // the lowest pair
+      walk_raw([&](const u32x4 r, int, int) { k = an_pkmax(k, an_pkmax(an_pkmax(r.x, r.y), an_pkmax(r.z, r.w))); });
+      const int b = an_pkmax1(k);
+      if (b >= 0) return __uint_as_float((unsigned)b << 16);
+      k = 0xff80ff80u;            // -inf
+      walk_raw([&](const u32x4 r, int, int) { k = an_pkmin(k, an_pkmin(an_pkmin(r.x, r.y), an_pkmin(r.z, r.w))); });
+      return __uint_as_float(min(k & 0xffffu, k >> 16) << 16);
+    } else {
+      float m = -INFINITY;
+      walk([&](const float (&v)[V], int, int) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = fmaxf(m, v[j]);
+      });
+      return m;
+    }
+  }
+  // whether a piece may hold a value of at least thr (it does, unless bf16 and thr <= 0)
+  static __device__ __forceinline__ bool reaches(const u32x4 r, float thr) {
+    if constexpr (BF16) {
+      const int b = an_pkmax1(an_pkmax(an_pkmax(r.x, r.y), an_pkmax(r.z, r.w)));
+      return !(thr > 0.f) || (b >= 0 && __uint_as_float((unsigned)b << 16) >= thr);
+    } else {
+      return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w))) >= thr;
+    }
+  }
+  // f(v, el) for the pieces that may hold a value of at least thr: few, so they are read again one by one (they are in
+  // the caches) rather than looked through in registers, which would unroll f once for each of them
+  template <class F>
+  __device__ __forceinline__ void walk_reaching(float thr, F f) const {
+    static_assert(E <= 64, "one bit for each piece");
+    u64 hit = 0;
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) hit |= reaches(raw[i], thr) ? 1ull << i : 0ull;
+    }
+    int c = threadIdx.x;
+    while (E > 0 ? hit != 0 : c < s.pieces) {
+      if (E > 0) {
+        c = (int)threadIdx.x + (__ffsll((long long)hit) - 1) * NT;
+        hit &= hit - 1;
+      }
+      const u32x4 r = c < s.pieces ? finish(fetch(c), c) : u32x4{0, 0, 0, 0};
+      if (c < s.pieces && (E > 0 || reaches(r, thr))) {
+        float v[V];
+        an_unpack<BF16>(r, v);
+        f(v, c * V - s.shift);
+      }
+      if (E == 0) c += NT;
+    }
+  }
+  // Between two walks: the compiler sees the pieces as new, so that it unpacks them again (an instruction each) instead
+  // of keeping the unpacked row, twice its size, alive from one walk to the next.
+  __device__ __forceinline__ void renew() {
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) asm volatile("" : "+v"(raw[i]));
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void walk_raw(F f) const {
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) f(raw[i], (int)threadIdx.x + i * NT, ((int)threadIdx.x + i * NT) * V - s.shift);
+    } else {
+      for (int c = threadIdx.x; c < s.pieces; c += NT) f(finish(fetch(c), c), c, c * V - s.shift);
     }
   }
   // f(v, c, el): the V values of piece c, the first of them in column el; columns outside [0, C) hold -inf
@@ -260,6 +347,7 @@ struct RowPieces {
         float v[V];
         an_unpack<BF16>(raw[i], v);
         f(v, (int)threadIdx.x + i * NT, ((int)threadIdx.x + i * NT) * V - s.shift);
+        __builtin_amdgcn_sched_barrier(0);   // one piece's temporaries at a time: other waves fill the gaps
       }
     } else {
       for (int c = threadIdx.x; c < s.pieces; c += NT) {
@@ -271,13 +359,16 @@ struct RowPieces {
   }
 };
 
-// whether the row holds a NaN (every thread of the workgroup calls)
-template <int NT, class ROW>
-__device__ __forceinline__ bool an_block_nan(const ROW& row) {
+// whether the row holds a NaN (every thread of the workgroup calls; the row is read again)
+template <bool BF16, int NT>
+__device__ __forceinline__ bool an_block_nan(const Span& span) {
+  constexpr int V = Piece<BF16>::V;
+  RowPieces<BF16, NT, 0> row;
+  row.s = span;
   int nan = 0;
-  row.walk([&](const float (&v)[ROW::V], int, int) {
+  row.walk([&](const float (&v)[V], int, int) {
 #pragma unroll
-    for (int j = 0; j < ROW::V; ++j) nan |= v[j] != v[j] ? 1 : 0;
+    for (int j = 0; j < V; ++j) nan |= v[j] != v[j] ? 1 : 0;
   });
   return __syncthreads_or(nan) != 0;
 }
@@ -423,8 +514,8 @@ __device__ __forceinline__ float an_threshold(const float* tmax, int threads_wit
   return an_unkey(lo);
 }
 
-template <bool BF16, int NT, int E>
-__global__ __launch_bounds__(NT) void logprob_block_kernel(const LogprobArgs a) {
+template <bool BF16, int NT, int E, int W>
+__global__ __launch_bounds__(NT, W) void logprob_block_kernel(const LogprobArgs a) {
   constexpr int V = Piece<BF16>::V, NW = NT / 64;
   __shared__ TopShared<NT> sh;
   __shared__ float s_max[NW];
@@ -435,11 +526,8 @@ __global__ __launch_bounds__(NT) void logprob_block_kernel(const LogprobArgs a) 
   row.s = an_span<BF16>(a.x, a.ld, r, a.R, a.C);
   row.load();
 
-  float m = -INFINITY;
-  row.walk([&](const float (&v)[V], int, int) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) m = fmaxf(m, v[j]);
-  });
+  float m = row.max();
+  row.renew();
   if (a.K > 0) {
     sh.tmax[tid] = m;
     if (tid == 0) sh.n = 0;
@@ -451,26 +539,27 @@ __global__ __launch_bounds__(NT) void logprob_block_kernel(const LogprobArgs a) 
   m = s_max[0];
 #pragma unroll
   for (int i = 1; i < NW; ++i) m = fmaxf(m, s_max[i]);
-  if (m == -INFINITY && an_block_nan<NT>(row)) m = NAN;   // (the maximum leaves NaN out)
+  if (m == -INFINITY && an_block_nan<BF16, NT>(row.s)) m = NAN;   // (the maximum may leave NaN out)
 
-  double S = 0.0, W = 0.0;
-  const float hi = a.temp.hi, lo = a.temp.lo;
+  // one factor only: what its rounding shifts is taken out of log S below, to first order
+  double S = 0.0, Wt = 0.0;
+  const float hi = a.temp.hi;
   row.walk([&](const float (&v)[V], int, int) {
     float e[V], w[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float t = an_arg(v[j], m, hi, lo);
+      const float t = (v[j] - m) * hi;
       e[j] = an_exp2(t);
       w[j] = e[j] * an_floor(t);
     }
     S += (double)an_tree<V>(e);
-    W += (double)an_tree<V>(w);
+    Wt += (double)an_tree<V>(w);
   });
   S = an_wave_sum(S);
-  W = an_wave_sum(W);
+  Wt = an_wave_sum(Wt);
   if (lane == 0) {
     s_sum[0][wave] = S;
-    s_sum[1][wave] = W;
+    s_sum[1][wave] = Wt;
   }
   if (a.K > 0 && wave == 0) {
     const float t = an_threshold<NT>(sh.tmax, row.s.pieces < NT ? row.s.pieces : NT, a.K);
@@ -478,21 +567,22 @@ __global__ __launch_bounds__(NT) void logprob_block_kernel(const LogprobArgs a) 
   }
   __syncthreads();
   S = s_sum[0][0];
-  W = s_sum[1][0];
+  Wt = s_sum[1][0];
 #pragma unroll
   for (int i = 1; i < NW; ++i) {
     S += s_sum[0][i];
-    W += s_sum[1][i];
+    Wt += s_sum[1][i];
   }
   const bool empty = m == -INFINITY;
   const bool broken = !empty && !(S == S);   // a NaN or +inf in the row
-  const double log_s = empty ? -INFINITY : log(S);
+  const double mean_t = AN_LN2 * (Wt / S);
+  const double log_s = empty ? -INFINITY : log(S) - a.temp.delta * mean_t;
   const void* xr = an_row<BF16>(a.x, a.ld, r);
   if (tid == 0) {
-    if (a.entropy != nullptr) a.entropy[r] = empty ? 0.f : (float)(log_s - AN_LN2 * (W / S));
+    if (a.entropy != nullptr) a.entropy[r] = empty ? 0.f : (float)(log_s - mean_t * (1.0 - a.temp.delta));
     if (a.stats != nullptr) {
       a.stats[2 * r] = m;
-      a.stats[2 * r + 1] = empty ? 1.f : (float)S;
+      a.stats[2 * r + 1] = empty ? 1.f : (float)(S * (1.0 - a.temp.delta * mean_t));
     }
   }
   for (int i = tid; i < a.T; i += NT) {
@@ -505,11 +595,12 @@ __global__ __launch_bounds__(NT) void logprob_block_kernel(const LogprobArgs a) 
   if (a.K == 0) return;
 
   // candidates: what reaches the threshold
+  row.renew();
   bool counted = broken;
   if (!broken) {
     const float thr = sh.thr;
     if (sh.tmax[tid] >= thr) {
-      row.walk([&](const float (&v)[V], int, int el) {
+      row.walk_reaching(thr, [&](const float (&v)[V], int el) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           if (v[j] >= thr && el + j >= 0 && el + j < a.C) {
@@ -572,12 +663,49 @@ __device__ __forceinline__ float an_wave_row_max(const float (&v)[E], float m) {
   return m;
 }
 
-// K rounds of "the largest left, the lowest index of it": cheaper than a threshold while K is small
-constexpr int AN_ROUNDS = 12;
+constexpr int AN_WCAP = 256;   // candidates a wave lists
+
+// Exactly the K best of a row of keys (0: none), by bisection over the keys and then in the order of the index, into
+// cand[0..K).  From `low`, which at least K keys reach.
+template <int E>
+__device__ __forceinline__ void an_wave_select(const unsigned (&key)[E], unsigned low, int K, u64* cand) {
+  const int lane = threadIdx.x & 63;
+  unsigned best = key[0];
+#pragma unroll
+  for (int i = 1; i < E; ++i) best = key[i] > best ? key[i] : best;
+  unsigned up = an_wave_umax(best);
+  while (low < up) {
+    const unsigned mid = low + ((up - low) >> 1) + 1;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) c += __popcll(__ballot(key[i] >= mid));
+    if (c >= K) {
+      low = mid;
+      if (c == K) break;
+    } else {
+      up = mid - 1;
+    }
+  }
+  int n = 0, above = 0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) above += __popcll(__ballot(key[i] > low));
+  int ties = K - above;   // of those equal to it, the first (all of them where the count was exact)
+  const u64 below_lane = (1ull << lane) - 1ull;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const u64 eq = __ballot(key[i] == low);
+    const bool take = key[i] > low || (key[i] == low && __popcll(eq & below_lane) < ties);
+    const u64 who = __ballot(take);
+    if (take) cand[n + __popcll(who & below_lane)] = an_pack(key[i], lane + 64 * i);
+    n += __popcll(who);
+    ties -= __popcll(eq);
+    ties = ties < 0 ? 0 : ties;
+  }
+}
 
 template <bool BF16, int E>
 __global__ __launch_bounds__(64 * AN_WAVES) void logprob_wave_kernel(const LogprobArgs a) {
-  __shared__ u64 s_cand[AN_WAVES][AN_TOP_MAX];
+  __shared__ u64 s_cand[AN_WAVES][AN_WCAP];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long r = (long)blockIdx.x * AN_WAVES + wave;
   if (r >= a.R) return;   // no barrier below: a wave keeps to its own row
@@ -590,27 +718,34 @@ __global__ __launch_bounds__(64 * AN_WAVES) void logprob_wave_kernel(const Logpr
   }
   int64_t t = -1;
   if (lane < a.T) t = a.targets[r * a.T + lane];   // the first 64; more are read below
-  float m = -INFINITY;
+  float best = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < E; ++i) m = fmaxf(m, v[i]);
-  m = an_wave_row_max<E>(v, m);
+  for (int i = 0; i < E; ++i) best = fmaxf(best, v[i]);
+  const float m = an_wave_row_max<E>(v, best);
   const bool empty = m == -INFINITY;
-  double S = 0.0, W = 0.0;
+  double S = 0.0, Wt = 0.0;
+  const float hi = a.temp.hi;
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const double d = ((double)v[i] - (double)m) * a.temp.inv_t;
-    const double e = an_exp(d);
-    S += e;
-    W += e * (d < -4096.0 ? -4096.0 : d);
+  for (int i0 = 0; i0 < E; i0 += 8) {   // eight at a time in f32, as in the longer rows
+    float es = 0.f, ws = 0.f;
+#pragma unroll
+    for (int i = i0; i < E && i < i0 + 8; ++i) {
+      const float u = (v[i] - m) * hi, e = an_exp2(u);
+      es += e;
+      ws = fmaf(e, an_floor(u), ws);
+    }
+    S += (double)es;
+    Wt += (double)ws;
   }
   S = an_wave_sum(S);
-  W = an_wave_sum(W);
-  const double log_s = empty ? -INFINITY : log(S);
+  Wt = an_wave_sum(Wt);
+  const double mean_t = AN_LN2 * (Wt / S);
+  const double log_s = empty ? -INFINITY : log(S) - a.temp.delta * mean_t;
   if (lane == 0) {
-    if (a.entropy != nullptr) a.entropy[r] = empty ? 0.f : (float)(log_s - W / S);
+    if (a.entropy != nullptr) a.entropy[r] = empty ? 0.f : (float)(log_s - mean_t * (1.0 - a.temp.delta));
     if (a.stats != nullptr) {
       a.stats[2 * r] = m;
-      a.stats[2 * r + 1] = empty ? 1.f : (float)S;
+      a.stats[2 * r + 1] = empty ? 1.f : (float)(S * (1.0 - a.temp.delta * mean_t));
     }
   }
   for (int i = lane; i < a.T; i += 64) {
@@ -622,73 +757,56 @@ __global__ __launch_bounds__(64 * AN_WAVES) void logprob_wave_kernel(const Logpr
   }
   if (a.K == 0) return;
 
-  unsigned key[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) key[i] = lane + 64 * i < a.C ? an_key(v[i]) : 0u;
-  if (a.K <= AN_ROUNDS) {
-    for (int k = 0; k < a.K; ++k) {
-      unsigned best = key[0];
-#pragma unroll
-      for (int i = 1; i < E; ++i) best = key[i] > best ? key[i] : best;
-      best = an_wave_umax(best);
-      int at = -1;
-#pragma unroll
-      for (int i = E - 1; i >= 0; --i) {
-        const u64 who = __ballot(key[i] == best);
-        if (who != 0) at = i * 64 + __ffsll((long long)who) - 1;
-      }
-      // (K <= C, so a live element is left: best > 0)
-#pragma unroll
-      for (int i = 0; i < E; ++i) key[i] = at == lane + 64 * i ? 0u : key[i];
-      if (lane == 0) {
-        a.top_indices[r * a.K + k] = at;
-        a.top_logprobs[r * a.K + k] = an_logprob(an_unkey(best), m, log_s, a.temp.inv_t);
+  // What the K-th largest of the lanes' maxima reaches is a short list that holds the K best.  Long ties, NaN and
+  // longer lists go by the keys of all elements.
+  u64* cand = s_cand[wave];
+  const bool broken = !empty && !(S == S);
+  int n = AN_WCAP + 1;
+  if (a.K <= 64 && !broken) {
+    const unsigned mine = lane < a.C ? an_key(best) : 0u;   // (lanes past a short row have none)
+    unsigned up = an_wave_umax(mine), low = an_wave_umin(mine);
+    if (low < AN_KEY_MINF) low = AN_KEY_MINF;
+    while (low < up) {
+      const unsigned mid = low + ((up - low) >> 1) + 1;
+      const int c = __popcll(__ballot(mine >= mid));
+      if (c >= a.K) {
+        low = mid;
+        if (c == a.K) break;
+      } else {
+        up = mid - 1;
       }
     }
-    return;
-  }
-  // the K-th key by bisection, from the smallest of the lanes' maxima where that is sure to be reached K times
-  unsigned best = key[0];
+    const float thr = an_unkey(low);
+    n = 0;
+    const u64 below_lane = (1ull << lane) - 1ull;
 #pragma unroll
-  for (int i = 1; i < E; ++i) best = key[i] > best ? key[i] : best;
-  unsigned up = an_wave_umax(best), low = an_wave_umin(best);
-  if (a.K > 64 || low < AN_KEY_MINF) low = AN_KEY_MINF;
-  while (low < up) {
-    const unsigned mid = low + ((up - low) >> 1) + 1;
-    int c = 0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) c += __popcll(__ballot(key[i] >= mid));
-    if (c >= a.K) {
-      low = mid;
-      if (c == a.K) break;
-    } else {
-      up = mid - 1;
+    for (int i = 0; i < E; ++i) {
+      const bool take = v[i] >= thr && lane + 64 * i < a.C;
+      const u64 who = __ballot(take);
+      if (who != 0) {
+        const int at = n + __popcll(who & below_lane);
+        if (take && at < AN_WCAP) cand[at] = an_pack(an_key(v[i]), lane + 64 * i);
+        n += __popcll(who);
+      }
     }
   }
-  // all elements above it, then the first of those equal to it: exactly K, in shared memory
-  int n = 0, above = 0;
+  if (n > AN_WCAP) {
+    unsigned key[E];
 #pragma unroll
-  for (int i = 0; i < E; ++i) above += __popcll(__ballot(key[i] > low));
-  int ties = a.K - above;
-  const u64 below_lane = (1ull << lane) - 1ull;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const u64 eq = __ballot(key[i] == low);
-    const bool take = key[i] > low || (key[i] == low && __popcll(eq & below_lane) < ties);
-    const u64 who = __ballot(take);
-    if (take) s_cand[wave][n + __popcll(who & below_lane)] = an_pack(key[i], lane + 64 * i);
-    n += __popcll(who);
-    ties -= __popcll(eq);
-    ties = ties < 0 ? 0 : ties;
+    for (int i = 0; i < E; ++i) key[i] = lane + 64 * i < a.C ? an_key(v[i]) : 0u;
+    an_wave_select<E>(key, AN_KEY_MINF, a.K, cand);
+    n = a.K;
   }
   __builtin_amdgcn_wave_barrier();
   __threadfence_block();
-  for (int i = lane; i < a.K; i += 64) {
-    const u64 mine = s_cand[wave][i];
+  for (int i = lane; i < n; i += 64) {
+    const u64 mine = cand[i];
     int before = 0;
-    for (int j = 0; j < a.K; ++j) before += s_cand[wave][j] > mine ? 1 : 0;
-    a.top_indices[r * a.K + before] = an_index(mine);
-    a.top_logprobs[r * a.K + before] = an_logprob(an_unkey((unsigned)(mine >> 32)), m, log_s, a.temp.inv_t);
+    for (int j = 0; j < n; ++j) before += cand[j] > mine ? 1 : 0;
+    if (before < a.K) {
+      a.top_indices[r * a.K + before] = an_index(mine);
+      a.top_logprobs[r * a.K + before] = an_logprob(an_unkey((unsigned)(mine >> 32)), m, log_s, a.temp.inv_t);
+    }
   }
 }
 
@@ -837,19 +955,23 @@ __device__ __forceinline__ void an_store(unsigned char* grow, int el, int C, con
   }
 }
 
-// Mentions in shared memory, `count` threads with number `id` share them: writes the entries in [from, to).
+// Mentions in shared memory, `count` threads with number `id` share them: writes the entries in [from, to).  `repeats`:
+// an entry may be named more than once.
 template <bool BF16, class F, class G>
-__device__ __forceinline__ void an_write_named(const int* idx, const float* add, int ns, int id, int count, int from, int to,
-                                               const void* xr, unsigned char* grow, F base, G term) {
+__device__ __forceinline__ void an_write_named(const int* idx, const float* add, int ns, bool repeats, int id, int count,
+                                               int from, int to, const void* xr, unsigned char* grow, F base, G term) {
   for (int s = id; s < ns; s += count) {
     const int j = idx[s];
     if (j < from || j >= to) continue;
     bool first = true;
-    float t = 0.f;
-    for (int o = 0; o < ns; ++o) {
-      const bool same = idx[o] == j;
-      if (same && o < s) first = false;
-      if (same) t += add[o];
+    float t = add[s];
+    if (repeats) {
+      t = 0.f;
+      for (int o = 0; o < ns; ++o) {
+        const bool same = idx[o] == j;
+        if (same && o < s) first = false;
+        if (same) t += add[o];
+      }
     }
     if (first) store1<BF16>(grow, (size_t)j, base(an_at<BF16>(xr, j)) + term(t));
   }
@@ -890,7 +1012,7 @@ __global__ __launch_bounds__(AN_ST) void answer_grad_block_kernel(const OP op, c
   }
   __syncthreads();
   const int from = c0 * V - row.s.shift;
-  an_write_named<BF16>(s_idx, s_add, ns, tid, AN_ST, from < 0 ? 0 : from, min(C, from + AN_ST * AN_SP * V),
+  an_write_named<BF16>(s_idx, s_add, ns, ns > 1, tid, AN_ST, from < 0 ? 0 : from, min(C, from + AN_ST * AN_SP * V),
                        an_row<BF16>(x, ld, r), grow, [&](float v) { return OP::base(w, v); },
                        [&](float t) { return OP::term(w, t); });
 }
@@ -921,7 +1043,7 @@ __global__ __launch_bounds__(64 * AN_WAVES) void answer_grad_wave_kernel(const O
   }
   __threadfence_block();
   __builtin_amdgcn_wave_barrier();
-  an_write_named<BF16>(s_idx[wave], s_add[wave], ns, lane, 64, 0, C, xr, grow, [&](float u) { return OP::base(w, u); },
+  an_write_named<BF16>(s_idx[wave], s_add[wave], ns, ns > 1, lane, 64, 0, C, xr, grow, [&](float u) { return OP::base(w, u); },
                        [&](float t) { return OP::term(w, t); });
 }
 
@@ -942,56 +1064,78 @@ struct DistillArgs {
   AnTemp temp;
 };
 
-// One wave: the row's loss and statistics.  lane holds the teacher's answers lane and lane + 64: value v, student logit
-// x, `live` where there is one.  s_all: sum of e over the row, s_out: over the classes outside the list (tail only),
-// `all`: the list covers every class.  q[] receives the teacher's probabilities.
-__device__ __forceinline__ DistillStat an_distill_row(const float (&v)[2], const float (&x)[2], const bool (&live)[2], bool bad,
-                                                      float m, double s_all, double s_out, bool all, int tail, double inv_t,
-                                                      double (&q)[2], double& loss) {
+// A row's list of answers in shared memory: the teacher's log probability, the student's logit, the class (-1: none),
+// whether an earlier entry names it too, and, in the end, the teacher's probability.
+struct DistillList {
+  float v[AN_TOP_MAX], x[AN_TOP_MAX], q[AN_TOP_MAX];
+  int idx[AN_TOP_MAX], again[AN_TOP_MAX];
+};
+
+// One wave: the row's statistics and loss from the sum of e over the classes outside the list (s_out) or, without a tail,
+// over all of them (s_all).  `all`: the list covers every class; `bad`: an answer lies past the classes.
+// Short loops on purpose: the pieces of the row are alive around this.
+__device__ __forceinline__ DistillStat an_distill_row(DistillList& list, int K, bool bad, float m, double s_all, double s_out,
+                                                      bool all, bool tail, double inv_t, double& loss) {
+  const int lane = threadIdx.x & 63;
+  const bool empty = m == -INFINITY;
   DistillStat st;
   st.m = m;
   st.S = s_all;
-  const bool empty = m == -INFINITY;
-  const double log_s = log(s_all);
   st.log_q = 0.0;
   bool some = true;
-  if (!tail) {
-    float vm = fmaxf(live[0] ? v[0] : -INFINITY, live[1] ? v[1] : -INFINITY);
+  if (tail) {
+    double own = 0.0;
+#pragma unroll 1
+    for (int k = lane; k < K; k += 64)
+      if (list.idx[k] >= 0 && !list.again[k]) own += an_exp(((double)list.x[k] - (double)m) * inv_t);
+    st.S = s_out + an_wave_sum(own);
+  } else {
+    float vm = -INFINITY;
+    bool nan = false;
+#pragma unroll 1
+    for (int k = lane; k < K; k += 64) {
+      if (list.idx[k] < 0) continue;
+      vm = fmaxf(vm, list.v[k]);
+      nan |= list.v[k] != list.v[k];
+    }
     vm = an_wave_max(vm);
     // (a NaN among the values is left out of the maximum and comes back through the sum)
-    const bool nan = __ballot((live[0] && v[0] != v[0]) || (live[1] && v[1] != v[1])) != 0;
-    some = vm != -INFINITY || nan;
+    some = vm != -INFINITY || __ballot(nan) != 0;
     if (some) {
       double sum = 0.0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) sum += live[i] ? an_exp((double)v[i] - (double)vm) : 0.0;
+#pragma unroll 1
+      for (int k = lane; k < K; k += 64) sum += list.idx[k] >= 0 ? an_exp((double)list.v[k] - (double)vm) : 0.0;
       st.log_q = (double)vm + log(an_wave_sum(sum));
     }
   }
+  const double log_s = log(st.S);
   double mass = 0.0, l = 0.0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const double lq = (double)v[i] - st.log_q;
-    q[i] = live[i] && some ? an_exp(lq) : 0.0;
-    mass += q[i];
-    const double lp = empty ? -INFINITY : ((double)x[i] - (double)m) * inv_t - log_s;
-    if (q[i] != 0.0) l += q[i] * (lq - lp);   // (NaN goes in)
+  bool any = false;
+#pragma unroll 1
+  for (int k = lane; k < K; k += 64) {
+    const bool live = list.idx[k] >= 0;
+    const double lq = (double)list.v[k] - st.log_q;
+    const double q = live && some ? an_exp(lq) : 0.0;
+    const double lp = empty ? -INFINITY : ((double)list.x[k] - (double)m) * inv_t - log_s;
+    any |= live;
+    mass += q;
+    if (q != 0.0) l += q * (lq - lp);   // (NaN goes in)
+    list.q[k] = (float)q;
   }
   mass = an_wave_sum(mass);
   l = an_wave_sum(l);
-  double rest = 0.0, slope_cut = 0.0;
+  double cut = 0.0;
   if (tail) {
-    const bool any = __ballot(live[0] || live[1]) != 0;
-    rest = all || !any ? 0.0 : 1.0 - mass;   // (a row without answers teaches nothing)
+    double rest = all || __ballot(any) == 0 ? 0.0 : 1.0 - mass;   // (a row without answers teaches nothing)
     if (!(rest > (double)AN_NO_REST)) rest = 0.0;
     mass += rest;
     if (rest > 0.0) {
       if (empty) {
         l += INFINITY;
       } else {
-        const double P = s_out / s_all;
+        const double P = s_out / st.S;
         l += rest * (log(rest) - log(P));
-        slope_cut = P > 0.0 ? rest / P : (P == 0.0 ? mass : P);
+        cut = P > 0.0 ? rest / P : (P == 0.0 ? mass : P);
       }
     }
   } else if (some) {
@@ -999,110 +1143,127 @@ __device__ __forceinline__ DistillStat an_distill_row(const float (&v)[2], const
   }
   if (bad) l = mass = NAN;
   st.mass = mass;
-  st.slope = mass - slope_cut;
+  st.slope = mass - cut;
   loss = l;
   return st;
 }
 
-template <int NT, bool BF16>
+template <int NT>
 struct DistillShared {
-  float v[AN_TOP_MAX], x[AN_TOP_MAX], add[AN_TOP_MAX];
-  int idx[AN_TOP_MAX];
+  DistillList list;
   float s_max[NT / 64];
-  double s_sum[2][NT / 64];
-  int bad;
+  double s_sum[NT / 64];
+  int bad, repeats;
   DistillStat st;
 };
 
-// MARK: the classes of the list are marked in a bitmap (in units of pieces) so that the others can be summed apart:
-// 1 - sum p would lose what is left of it where the student agrees with its teacher.
-template <bool BF16, int NT, int E, bool TAIL>
-__global__ __launch_bounds__(NT) void distill_block_kernel(const DistillArgs a) {
+// The elements of a piece whose bits are set become -inf.
+template <bool BF16>
+__device__ __forceinline__ u32x4 an_drop(u32x4 r, unsigned bits) {
+  unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int j = 0; j < Piece<BF16>::V; ++j) {
+    const bool out = (bits >> j) & 1u;
+    if constexpr (BF16) {
+      const unsigned keep = (j & 1) ? 0x0000ffffu : 0xffff0000u, put = (j & 1) ? 0xff800000u : 0x0000ff80u;
+      w[j >> 1] = out ? ((w[j >> 1] & keep) | put) : w[j >> 1];
+    } else {
+      w[j] = out ? 0xff800000u : w[j];
+    }
+  }
+  return u32x4{w[0], w[1], w[2], w[3]};
+}
+
+// One workgroup per row.  The classes of the list are marked in a bitmap (in units of pieces).  TAIL: their elements are
+// taken out of the registers before the exponentials, so that the rest is summed by itself (1 - sum p would lose what is
+// left of it where the student agrees with its teacher), and their own terms are added by the list.
+// HOLD: the exponentials stay in registers for the gradient (f32: in the place of the logits; bf16: in twice the
+// registers, where that still leaves two workgroups to a CU); otherwise they are formed again.
+template <bool BF16, int NT, int E, bool TAIL, bool HOLD, int W>
+__global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs a) {
   constexpr int V = Piece<BF16>::V, NW = NT / 64;
-  __shared__ DistillShared<NT, BF16> sh;
-  extern __shared__ unsigned s_mark[];   // TAIL: one bit per element of the pieces
+  __shared__ DistillShared<NT> sh;
+  extern __shared__ unsigned s_mark[];   // one bit per element of the pieces
   const long r = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   RowPieces<BF16, NT, E> row;
   row.s = an_span<BF16>(a.x, a.ld, r, a.R, a.C);
   row.load();
   const void* xr = an_row<BF16>(a.x, a.ld, r);
-  if (TAIL)
-    for (int i = tid; i < (row.s.pieces * V + 31) / 32; i += NT) s_mark[i] = 0u;
-  if (tid == 0) sh.bad = 0;
+  for (int i = tid; i < (row.s.pieces * V + 31) / 32; i += NT) s_mark[i] = 0u;
+  if (tid == 0) sh.bad = sh.repeats = 0;
   __syncthreads();
   if (tid < a.K) {
     const int64_t j = a.indices[r * a.K + tid];
     const bool live = j >= 0 && j < a.C;
-    sh.idx[tid] = live ? (int)j : -1;
-    sh.v[tid] = a.teacher[r * a.K + tid];
-    sh.x[tid] = live ? an_at<BF16>(xr, j) : 0.f;
+    int again = 0;
+    sh.list.idx[tid] = live ? (int)j : -1;
+    sh.list.v[tid] = a.teacher[r * a.K + tid];
+    sh.list.x[tid] = live ? an_at<BF16>(xr, j) : 0.f;
     if (j >= a.C) sh.bad = 1;
-    if (TAIL && live) {
+    if (live) {
       const int b = (int)j + row.s.shift;
-      atomicOr(&s_mark[b >> 5], 1u << (b & 31));
+      again = (atomicOr(&s_mark[b >> 5], 1u << (b & 31)) >> (b & 31)) & 1u;
+      if (again) sh.repeats = 1;
     }
+    sh.list.again[tid] = again;
   }
-  float m = -INFINITY;
-  row.walk([&](const float (&v)[V], int, int) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) m = fmaxf(m, v[j]);
-  });
-  m = an_wave_max(m);
+  float m = an_wave_max(row.max());
+  row.renew();
   if (lane == 0) sh.s_max[wave] = m;
   __syncthreads();
   m = sh.s_max[0];
 #pragma unroll
   for (int i = 1; i < NW; ++i) m = fmaxf(m, sh.s_max[i]);
-  if (m == -INFINITY && an_block_nan<NT>(row)) m = NAN;
+  if (m == -INFINITY && an_block_nan<BF16, NT>(row.s)) m = NAN;
 
-  double S = 0.0, O = 0.0;
+  double S = 0.0;   // TAIL: over the classes outside the list
   const float hi = a.temp.hi, lo = a.temp.lo;
-  row.walk([&](const float (&v)[V], int c, int) {
-    float e[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) e[j] = an_exp2(an_arg(v[j], m, hi, lo));
-    S += (double)an_tree<V>(e);
+  const auto marks = [&](int c) { return c < row.s.pieces ? s_mark[(c * V) >> 5] >> ((c * V) & 31) : 0u; };
+  float held[HOLD ? E : 1][V];
+  int at = tid;
+  asm volatile("" : "+v"(at));   // the pieces' columns are computed again, not kept from the load
+  if constexpr (E > 0) {
     if constexpr (TAIL) {
-      // the piece's bits: a byte (bf16) or a nibble (f32); pieces past the row have none and hold zeros
-      unsigned b = 0;
-      if (c < row.s.pieces) b = s_mark[(c * V) >> 5] >> ((c * V) & 31);
+      constexpr unsigned all = (1u << V) - 1u;
 #pragma unroll
-      for (int j = 0; j < V; ++j) e[j] = (b >> j) & 1u ? 0.f : e[j];
-      O += (double)an_tree<V>(e);
+      for (int i = 0; i < E; ++i) {
+        const unsigned b = marks(at + i * NT) & all;
+        if (b != 0) row.raw[i] = an_drop<BF16>(row.raw[i], b);
+      }
     }
-  });
-  S = an_wave_sum(S);
-  if (TAIL) O = an_wave_sum(O);
-  if (lane == 0) {
-    sh.s_sum[0][wave] = S;
-    if (TAIL) sh.s_sum[1][wave] = O;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      float e[V];
+      an_unpack<BF16>(row.raw[i], e);
+#pragma unroll
+      for (int j = 0; j < V; ++j) e[j] = an_exp2(an_arg(e[j], m, hi, lo));
+      S += (double)an_tree<V>(e);
+      if constexpr (HOLD) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) held[i][j] = e[j];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  } else {
+    row.walk_raw([&](const u32x4 p, int c, int) {
+      float e[V];
+      an_unpack<BF16>(TAIL ? an_drop<BF16>(p, marks(c)) : p, e);
+#pragma unroll
+      for (int j = 0; j < V; ++j) e[j] = an_exp2(an_arg(e[j], m, hi, lo));
+      S += (double)an_tree<V>(e);
+    });
   }
+  S = an_wave_sum(S);
+  if (lane == 0) sh.s_sum[wave] = S;
   __syncthreads();
   if (wave == 0) {
-    S = O = 0.0;
+    S = 0.0;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      S += sh.s_sum[0][i];
-      if (TAIL) O += sh.s_sum[1][i];
-    }
-    float v[2], x[2];
-    bool live[2];
-    double q[2], loss;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int k = lane + 64 * i;
-      live[i] = k < a.K && sh.idx[k < a.K ? k : 0] >= 0;
-      v[i] = live[i] ? sh.v[k] : 0.f;
-      x[i] = live[i] ? sh.x[k] : 0.f;
-    }
+    for (int i = 0; i < NW; ++i) S += sh.s_sum[i];
+    double loss;
     // (more than 1024 classes and at most 128 answers: never all of them)
-    const DistillStat st = an_distill_row(v, x, live, sh.bad != 0, m, S, O, false, TAIL ? 1 : 0, a.temp.inv_t, q, loss);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int k = lane + 64 * i;
-      if (k < a.K) sh.add[k] = (float)q[i];
-    }
+    const DistillStat st = an_distill_row(sh.list, a.K, sh.bad != 0, m, S, S, false, TAIL, a.temp.inv_t, loss);
     if (lane == 0) {
       sh.st = st;
       a.row_loss[r] = (float)(a.t2 * loss);
@@ -1112,32 +1273,48 @@ __global__ __launch_bounds__(NT) void distill_block_kernel(const DistillArgs a) 
   if (a.grad == nullptr) return;   // uniform
   __syncthreads();
   const DistillStat st = sh.st;
-  const bool empty = an_no_gradient(st);
-  const double inv = empty ? 0.0 : 1.0 / st.S;
+  const bool none = an_no_gradient(st);
+  const double inv = none ? 0.0 : 1.0 / st.S;
   const float mass = (float)(st.mass * inv), slope = (float)(st.slope * inv) * a.scale;
   unsigned char* grow = reinterpret_cast<unsigned char*>(a.grad) + r * a.ldg * (BF16 ? 2 : 4);
-  row.walk([&](const float (&v)[V], int c, int el) {
-    if (c >= row.s.pieces) return;
-    float g[V];
+  asm volatile("" : "+v"(at));
+  if constexpr (HOLD) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) g[j] = empty ? 0.f : an_exp2(an_arg(v[j], m, hi, lo)) * slope;
-    an_store<BF16>(grow, el, a.C, g);
-  });
+    for (int i = 0; i < E; ++i) {
+      const int c = at + i * NT;
+      float g[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) g[j] = none ? 0.f : held[i][j] * slope;
+      if (c < row.s.pieces) an_store<BF16>(grow, c * V - row.s.shift, a.C, g);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  } else {
+    row.renew();
+    row.walk([&](const float (&v)[V], int c, int) {
+      const int here = c - tid + at;
+      if (here >= row.s.pieces) return;
+      float g[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) g[j] = none ? 0.f : an_exp2(an_arg(v[j], m, hi, lo)) * slope;
+      an_store<BF16>(grow, here * V - row.s.shift, a.C, g);
+    });
+  }
   __syncthreads();
   const float sc = a.scale;
-  an_write_named<BF16>(sh.idx, sh.add, a.K, tid, NT, 0, a.C, xr, grow,
-                       [&](float x) { return empty ? 0.f : sc * (an_exp2(an_arg(x, m, hi, lo)) * mass); },
-                       [&](float q) { return empty ? 0.f : -sc * q; });
+  an_write_named<BF16>(sh.list.idx, sh.list.q, a.K, sh.repeats != 0, tid, NT, 0, a.C, xr, grow,
+                       [&](float x) { return none ? 0.f : sc * (an_exp2(an_arg(x, m, hi, lo)) * mass); },
+                       [&](float q) { return none ? 0.f : -sc * q; });
 }
 
 template <bool BF16, int E>
 __global__ __launch_bounds__(64 * AN_WAVES) void distill_wave_kernel(const DistillArgs a) {
-  __shared__ int s_idx[AN_WAVES][AN_TOP_MAX];
-  __shared__ float s_add[AN_WAVES][AN_TOP_MAX];
+  __shared__ DistillList s_list[AN_WAVES];
   __shared__ unsigned s_mark[AN_WAVES][AN_WAVE_C / 32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long r = (long)blockIdx.x * AN_WAVES + wave;
   if (r >= a.R) return;   // no barrier below: a wave keeps to its own row
+  DistillList& list = s_list[wave];
+  unsigned* mark = s_mark[wave];
   const void* xr = an_row<BF16>(a.x, a.ld, r);
   float v[E];
 #pragma unroll
@@ -1145,38 +1322,30 @@ __global__ __launch_bounds__(64 * AN_WAVES) void distill_wave_kernel(const Disti
     const int c = lane + 64 * i;
     v[i] = c < a.C ? an_at<BF16>(xr, c) : -INFINITY;
   }
-  if (lane < AN_WAVE_C / 32) s_mark[wave][lane] = 0u;
+  if (lane < AN_WAVE_C / 32) mark[lane] = 0u;
   __builtin_amdgcn_wave_barrier();
   __threadfence_block();
-  float tv[2], tx[2];
-  bool live[2], beyond = false;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int k = lane + 64 * i;
-    int64_t j = -1;
-    tv[i] = tx[i] = 0.f;
-    if (k < a.K) {
-      j = a.indices[r * a.K + k];
-      beyond |= j >= a.C;
-      live[i] = j >= 0 && j < a.C;
-      if (live[i]) {
-        tv[i] = a.teacher[r * a.K + k];
-        tx[i] = an_at<BF16>(xr, j);
-        atomicOr(&s_mark[wave][j >> 5], 1u << (j & 31));
-      }
-      s_idx[wave][k] = live[i] ? (int)j : -1;
-    } else {
-      live[i] = false;
-    }
+  bool beyond = false, named_again = false;
+  for (int k = lane; k < a.K; k += 64) {
+    const int64_t j = a.indices[r * a.K + k];
+    const bool live = j >= 0 && j < a.C;
+    int again = 0;
+    beyond |= j >= a.C;
+    list.idx[k] = live ? (int)j : -1;
+    list.v[k] = a.teacher[r * a.K + k];
+    list.x[k] = live ? an_at<BF16>(xr, j) : 0.f;
+    if (live) again = (atomicOr(&mark[j >> 5], 1u << (j & 31)) >> (j & 31)) & 1u;
+    named_again |= again != 0;
+    list.again[k] = again;
   }
-  const bool bad = __ballot(beyond) != 0;
+  const bool bad = __ballot(beyond) != 0, repeats = __ballot(named_again) != 0;
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < E; ++i) m = fmaxf(m, v[i]);
   m = an_wave_row_max<E>(v, m);
   __builtin_amdgcn_wave_barrier();
   __threadfence_block();
-  double S = 0.0, O = 0.0;
+  double S = 0.0;   // tail: over the classes outside the list
   int outside = 0;
   float e32[E];
 #pragma unroll
@@ -1184,39 +1353,34 @@ __global__ __launch_bounds__(64 * AN_WAVES) void distill_wave_kernel(const Disti
     const int c = lane + 64 * i;
     const double e = an_exp(((double)v[i] - (double)m) * a.temp.inv_t);
     e32[i] = (float)e;
-    S += e;
-    const bool in = (s_mark[wave][c >> 5] >> (c & 31)) & 1u;   // E <= 16: c < 1024
-    O += in ? 0.0 : e;
+    const bool in = (mark[c >> 5] >> (c & 31)) & 1u;   // E <= 16: c < 1024
+    S += a.tail && in ? 0.0 : e;
     outside += c < a.C && !in ? 1 : 0;
   }
   S = an_wave_sum(S);
-  O = an_wave_sum(O);
   const bool all = __ballot(outside != 0) == 0;
-  double q[2], loss;
-  const DistillStat st = an_distill_row(tv, tx, live, bad, m, S, O, all, a.tail, a.temp.inv_t, q, loss);
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (lane + 64 * i < a.K) s_add[wave][lane + 64 * i] = (float)q[i];
+  double loss;
+  const DistillStat st = an_distill_row(list, a.K, bad, m, S, S, all, a.tail != 0, a.temp.inv_t, loss);
   if (lane == 0) {
     a.row_loss[r] = (float)(a.t2 * loss);
     if (a.stats != nullptr) a.stats[r] = st;
   }
   if (a.grad == nullptr) return;
-  const bool empty = an_no_gradient(st);
-  const double inv = empty ? 0.0 : 1.0 / st.S;
+  const bool none = an_no_gradient(st);
+  const double inv = none ? 0.0 : 1.0 / st.S;
   const float mass = (float)(st.mass * inv), slope = (float)(st.slope * inv) * a.scale;
   unsigned char* grow = reinterpret_cast<unsigned char*>(a.grad) + r * a.ldg * (BF16 ? 2 : 4);
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const int c = lane + 64 * i;
-    if (c < a.C) store1<BF16>(grow, (size_t)c, empty ? 0.f : e32[i] * slope);
+    if (c < a.C) store1<BF16>(grow, (size_t)c, none ? 0.f : e32[i] * slope);
   }
   __threadfence_block();
   __builtin_amdgcn_wave_barrier();
   const float sc = a.scale;
-  an_write_named<BF16>(s_idx[wave], s_add[wave], a.K, lane, 64, 0, a.C, xr, grow,
-                       [&](float x) { return empty ? 0.f : sc * ((float)an_exp(((double)x - (double)m) * a.temp.inv_t) * mass); },
-                       [&](float t) { return empty ? 0.f : -sc * t; });
+  an_write_named<BF16>(list.idx, list.q, a.K, repeats, lane, 64, 0, a.C, xr, grow,
+                       [&](float x) { return none ? 0.f : sc * ((float)an_exp(((double)x - (double)m) * a.temp.inv_t) * mass); },
+                       [&](float t) { return none ? 0.f : -sc * t; });
 }
 
 // out[0] = scale * sum of x[0..n): one workgroup, every thread adds its own in order, waves in order
@@ -1254,12 +1418,18 @@ void an_by_block(int C, F f) {
   const int pieces = (C + Piece<BF16>::V - 1) / Piece<BF16>::V + 1;
 #define AN_FIT(NT, E) if (pieces <= NT * E) return f(std::integral_constant<int, NT>(), std::integral_constant<int, E>())
   if constexpr (BF16) {
-    AN_FIT(256, 2); AN_FIT(256, 4); AN_FIT(512, 4); AN_FIT(512, 8); AN_FIT(1024, 7); AN_FIT(1024, 9);
+    AN_FIT(256, 2); AN_FIT(256, 4); AN_FIT(256, 8); AN_FIT(256, 12); AN_FIT(256, 16); AN_FIT(256, 20); AN_FIT(256, 25); AN_FIT(256, 33);
   } else {
-    AN_FIT(256, 4); AN_FIT(256, 8); AN_FIT(512, 8); AN_FIT(512, 16); AN_FIT(1024, 13); AN_FIT(1024, 17);
+    AN_FIT(256, 4); AN_FIT(256, 8); AN_FIT(256, 16); AN_FIT(256, 24); AN_FIT(256, 32); AN_FIT(256, 40); AN_FIT(256, 50); AN_FIT(512, 33);
   }
 #undef AN_FIT
   return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 0>());
+}
+
+// waves per SIMD to compile for: the pieces in registers and about 40 more
+constexpr int an_waves(int e) {
+  const int regs = 4 * e + 40, w = 512 / ((regs + 7) / 8 * 8);
+  return w < 1 ? 1 : w > 8 ? 8 : w;
 }
 
 bool an_shape_ok(long ld, int R, int C, int K, double temperature) {
@@ -1303,7 +1473,7 @@ void an_launch_logprobs(const LogprobArgs& a, hipStream_t st) {
     });
   } else {
     an_by_block<BF16>(a.C, [&](auto nt, auto e) {
-      hipLaunchKernelGGL((logprob_block_kernel<BF16, decltype(nt)::value, decltype(e)::value>), dim3((unsigned)a.R),
+      hipLaunchKernelGGL((logprob_block_kernel<BF16, decltype(nt)::value, decltype(e)::value, an_waves(decltype(e)::value)>), dim3((unsigned)a.R),
                          dim3(decltype(nt)::value), 0, st, a);
     });
   }
@@ -1317,12 +1487,14 @@ int an_launch_distill(const DistillArgs& a, hipStream_t st) {
                          dim3(64 * AN_WAVES), 0, st, a);
     });
   } else {
-    const size_t mark = a.tail ? ((size_t)a.C + 2 * Piece<BF16>::V + 31) / 32 * 4 : 0;
-    VQAF_REQUIRE(mark <= 49152, VQAF_E_SHAPE);   // 393 thousand classes with the remaining mass as an event
+    const size_t mark = ((size_t)a.C + 2 * Piece<BF16>::V + 31) / 32 * 4;
+    VQAF_REQUIRE(mark <= 49152, VQAF_E_SHAPE);   // 393 thousand classes
     an_by_block<BF16>(a.C, [&](auto nt, auto e) {
       constexpr int NT = decltype(nt)::value, E = decltype(e)::value;
-      if (a.tail) hipLaunchKernelGGL((distill_block_kernel<BF16, NT, E, true>), dim3((unsigned)a.R), dim3(NT), mark, st, a);
-      else hipLaunchKernelGGL((distill_block_kernel<BF16, NT, E, false>), dim3((unsigned)a.R), dim3(NT), 0, st, a);
+      constexpr bool HOLD = E > 0 && (!BF16 || E <= 4);
+      constexpr int W = an_waves(BF16 && HOLD ? 2 * E + 2 : E + 2);
+      if (a.tail) hipLaunchKernelGGL((distill_block_kernel<BF16, NT, E, true, HOLD, W>), dim3((unsigned)a.R), dim3(NT), mark, st, a);
+      else hipLaunchKernelGGL((distill_block_kernel<BF16, NT, E, false, HOLD, W>), dim3((unsigned)a.R), dim3(NT), mark, st, a);
     });
   }
   VQAF_LAUNCH_CHECK();

@@ -827,6 +827,11 @@ class TokenLogprobs(NamedTuple):
     top_indices: Optional[torch.Tensor]
 
 
+def _raw_stream(device: torch.device) -> int:
+    """The current stream of `device` as the C ABI takes it (stream_ptr without building a stream object)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
+
+
 def _on(device: torch.device):
     """Makes `device` the current one for the launches inside (a launch goes to the current device, whatever its
     stream)."""
@@ -870,27 +875,32 @@ def _f32(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return None if g is None else g.to(torch.float32).contiguous()
 
 
+def _logprobs_forward(x, ld, targets, top, temperature, entropy, stats):
+    """One launch; (logprobs, entropy, top_logprobs, top_indices, stats), None where not asked for."""
+    R, C = x.shape
+    dev = x.device
+    T = 0 if targets is None else targets.shape[1]
+    lp = torch.empty(R, T, dtype=torch.float32, device=dev) if targets is not None else None
+    ent = torch.empty(R, dtype=torch.float32, device=dev) if entropy else None
+    tl = torch.empty(R, top, dtype=torch.float32, device=dev) if top else None
+    ti = torch.empty(R, top, dtype=torch.int64, device=dev) if top else None
+    st = torch.empty(R, 2, dtype=torch.float32, device=dev) if stats else None
+    with _on(dev):
+        check(load().vqaf_token_logprobs(x.data_ptr(), ld, ptr(targets), R, C, T, top, dtype_code(x), temperature,
+                                         ptr(lp), ptr(ent), ptr(tl), ptr(ti), ptr(st), _raw_stream(dev)),
+              "vqaf_token_logprobs")
+    return lp, ent, tl, ti, st
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, ld, targets, top, temperature, entropy, stats):
-        R, C = x.shape
-        dev = x.device
-        T = 0 if targets is None else targets.shape[1]
-        lp = torch.empty(R, T, dtype=torch.float32, device=dev) if targets is not None else None
-        ent = torch.empty(R, dtype=torch.float32, device=dev) if entropy else None
-        tl = torch.empty(R, top, dtype=torch.float32, device=dev) if top else None
-        ti = torch.empty(R, top, dtype=torch.int64, device=dev) if top else None
-        st = torch.empty(R, 2, dtype=torch.float32, device=dev) if stats else None
-        with _on(dev):
-            check(load().vqaf_token_logprobs(x.data_ptr(), ld, ptr(targets), R, C, T, top, dtype_code(x), temperature,
-                                             ptr(lp), ptr(ent), ptr(tl), ptr(ti), ptr(st), stream_ptr(dev)),
-                  "vqaf_token_logprobs")
-        if stats:
-            ctx.save_for_backward(x, targets, ti, st, ent)
-            ctx.meta = (ld, T, top, temperature)
-            ctx.set_materialize_grads(False)
-            if ti is not None:
-                ctx.mark_non_differentiable(ti)
+    def forward(ctx, x, ld, targets, top, temperature, entropy):
+        lp, ent, tl, ti, st = _logprobs_forward(x, ld, targets, top, temperature, entropy, True)
+        ctx.save_for_backward(x, targets, ti, st, ent)
+        ctx.meta = (ld, 0 if targets is None else targets.shape[1], top, temperature)
+        ctx.set_materialize_grads(False)
+        if ti is not None:
+            ctx.mark_non_differentiable(ti)
         return lp, ent, tl, ti
 
     @staticmethod
@@ -899,16 +909,16 @@ class _TokenLogprobs(torch.autograd.Function):
         x, targets, ti, st, ent = ctx.saved_tensors
         ld, T, top, temperature = ctx.meta
         if g_lp is None and g_ent is None and g_top is None:
-            return (None,) * 7
+            return (None,) * 6
         R, C = x.shape
         g_lp, g_ent, g_top = _f32(g_lp), _f32(g_ent), _f32(g_top)
         grad = _grad_rows(x, ld)
         with _on(x.device):
             check(load().vqaf_token_logprobs_bwd(x.data_ptr(), ld, ptr(targets), ptr(ti), R, C, T, top, dtype_code(x),
                                                  temperature, ptr(st), ptr(ent), ptr(g_lp), ptr(g_ent), ptr(g_top),
-                                                 grad.data_ptr(), grad.stride(0), stream_ptr(x.device)),
+                                                 grad.data_ptr(), grad.stride(0), _raw_stream(x.device)),
                   "vqaf_token_logprobs_bwd")
-        return (grad,) + (None,) * 6
+        return (grad,) + (None,) * 5
 
 
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0, temperature: float = 1.0,
@@ -941,65 +951,67 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
         if T > ANSWERS_MAX:
             raise ValueError(f"at most {ANSWERS_MAX} targets for each row, got {T}")
         tg = targets.to(torch.int64).reshape(R, T).contiguous()
-    needs = torch.is_grad_enabled() and x.requires_grad
     if R == 0:
         z = x.sum(1, dtype=torch.float32)
         lp = None if tg is None else (z[:, None].expand(0, tg.shape[1]) * 1.0)
         ent, tl = (z if entropy else None), (z[:, None].expand(0, top) * 1.0 if top else None)
         ti = torch.empty(0, top, dtype=torch.int64, device=x.device) if top else None
+    elif x.requires_grad and torch.is_grad_enabled():
+        lp, ent, tl, ti = _TokenLogprobs.apply(x, ld, tg, top, temperature, bool(entropy))
     else:
-        lp, ent, tl, ti = _TokenLogprobs.apply(x, ld, tg, top, temperature, bool(entropy), needs)
+        lp, ent, tl, ti, _ = _logprobs_forward(x, ld, tg, top, temperature, entropy, False)
     if len(lead) == 1:
-        if lp is not None and given == lead:
-            lp = lp.view(given)
-        return TokenLogprobs(lp, ent, tl, ti)
+        return TokenLogprobs(lp.view(given) if lp is not None and given == lead else lp, ent, tl, ti)
     return TokenLogprobs(None if lp is None else lp.view(given), None if ent is None else ent.view(lead),
                          None if tl is None else tl.view(*lead, top), None if ti is None else ti.view(*lead, top))
+
+
+def _distill_forward(x, ld, teacher, indices, temperature, tail, scale, needs):
+    """(row losses, or their sum times `scale`; statistics; gradient of that sum).  The last two are None unless a
+    backward needs them, the gradient also where there is no sum."""
+    R, C = x.shape
+    dev = x.device
+    rows = torch.empty(R, dtype=torch.float32, device=dev)
+    stats = torch.empty(R, 5, dtype=torch.float64, device=dev) if needs else None
+    whole = scale is not None
+    grad = _grad_rows(x, ld) if needs and whole else None
+    loss = torch.empty((), dtype=torch.float32, device=dev) if whole else None
+    with _on(dev):
+        check(load().vqaf_distill(x.data_ptr(), ld, teacher.data_ptr(), indices.data_ptr(), R, C, teacher.shape[1],
+                                  dtype_code(x), temperature, tail, rows.data_ptr(), ptr(stats),
+                                  None if grad is None else grad.data_ptr(), 0 if grad is None else grad.stride(0),
+                                  scale if whole else 1.0, ptr(loss), _raw_stream(dev)), "vqaf_distill")
+    return (loss if whole else rows), stats, grad
 
 
 class _Distill(torch.autograd.Function):
     """Row losses, or their sum / mean with the gradient for an incoming gradient of 1 formed in the same pass."""
 
     @staticmethod
-    def forward(ctx, x, ld, teacher, indices, temperature, tail, scale, needs):
-        R, C = x.shape
-        K = teacher.shape[1]
-        dev = x.device
-        rows = torch.empty(R, dtype=torch.float32, device=dev)
-        stats = torch.empty(R, 5, dtype=torch.float64, device=dev) if needs else None
-        whole = scale is not None
-        grad = _grad_rows(x, ld) if needs and whole else None
-        loss = torch.empty((), dtype=torch.float32, device=dev) if whole else None
-        with _on(dev):
-            check(load().vqaf_distill(x.data_ptr(), ld, ptr(teacher), ptr(indices), R, C, K, dtype_code(x), temperature,
-                                      int(tail), ptr(rows), ptr(stats), None if grad is None else grad.data_ptr(),
-                                      0 if grad is None else grad.stride(0), scale if whole else 1.0, ptr(loss),
-                                      stream_ptr(dev)), "vqaf_distill")
-        if needs:
-            ctx.save_for_backward(x, teacher, indices, stats)
-            ctx.meta = (ld, K, temperature, scale if whole else 1.0, whole)
-            ctx.unit = grad
-        return loss if whole else rows
+    def forward(ctx, x, ld, teacher, indices, temperature, tail, scale):
+        out, stats, ctx.unit = _distill_forward(x, ld, teacher, indices, temperature, tail, scale, True)
+        ctx.save_for_backward(x, teacher, indices, stats)
+        ctx.meta = (ld, temperature, scale)
+        return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, up):
-        x, teacher, indices, stats = ctx.saved_tensors
-        ld, K, temperature, scale, whole = ctx.meta
-        none = (None,) * 7
         grad, ctx.unit = ctx.unit, None   # handed out once: a second backward forms its own
-        if grad is not None and up is _unit_grads.get((up.device, up.dtype)):
-            return (grad,) + none
         ready = grad is not None
-        if not ready:
-            grad = _grad_rows(x, ld)
-        up = _f32(up)
-        with _on(x.device):
-            check(load().vqaf_distill_bwd(x.data_ptr(), ld, ptr(teacher), ptr(indices), x.shape[0], x.shape[1], K,
-                                          dtype_code(x), temperature, ptr(stats), ptr(up), 0 if whole else 1, int(ready),
-                                          scale, grad.data_ptr(), grad.stride(0), stream_ptr(x.device)),
-                  "vqaf_distill_bwd")
-        return (grad,) + none
+        x, teacher, indices, stats = ctx.saved_tensors   # (also tells of logits changed in place since)
+        if not ready or up is not _unit_grads.get((up.device, up.dtype)):
+            ld, temperature, scale = ctx.meta
+            if not ready:
+                grad = _grad_rows(x, ld)
+            up = _f32(up)
+            with _on(x.device):
+                check(load().vqaf_distill_bwd(x.data_ptr(), ld, teacher.data_ptr(), indices.data_ptr(), x.shape[0],
+                                              x.shape[1], teacher.shape[1], dtype_code(x), temperature, stats.data_ptr(),
+                                              up.data_ptr(), int(scale is None), int(ready),
+                                              1.0 if scale is None else scale, grad.data_ptr(), grad.stride(0),
+                                              _raw_stream(x.device)), "vqaf_distill_bwd")
+        return grad, None, None, None, None, None, None
 
 
 def distill_loss(logits: torch.Tensor, teacher: torch.Tensor, indices: torch.Tensor, temperature: float = 1.0,
@@ -1037,8 +1049,11 @@ def distill_loss(logits: torch.Tensor, teacher: torch.Tensor, indices: torch.Ten
         return rows.view(lead) if reduction == "none" else rows.sum() if reduction == "sum" else rows.mean()
     v = teacher.detach().to(torch.float32).reshape(R, K).contiguous()
     idx = indices.to(torch.int64).reshape(R, K).contiguous()
-    scale = {"mean": 1.0 / R, "sum": 1.0, "none": None}[reduction]
-    out = _Distill.apply(x, ld, v, idx, temperature, bool(tail), scale, torch.is_grad_enabled() and x.requires_grad)
+    scale = 1.0 / R if reduction == "mean" else 1.0 if reduction == "sum" else None
+    if x.requires_grad and torch.is_grad_enabled():
+        out = _Distill.apply(x, ld, v, idx, temperature, int(bool(tail)), scale)
+    else:
+        out = _distill_forward(x, ld, v, idx, temperature, int(bool(tail)), scale, False)[0]
     return out.view(lead) if scale is None and len(lead) != 1 else out
 
 
@@ -1183,7 +1198,7 @@ def quantize_rows(x: torch.Tensor):
     if M:
         with _on(x.device):
             check(load().vqaf_quantize_rows(x2.data_ptr(), ld, M, K, dtype_code(x2), q.data_ptr(), pitch, ptr(scale),
-                                            stream_ptr(x.device)), "vqaf_quantize_rows")
+                                            _raw_stream(x.device)), "vqaf_quantize_rows")
     lead = x.shape[:-1]
     return (q[:, :K] if len(lead) == 1 else q.view(*lead, pitch)[..., :K]), scale.view(lead)
 
@@ -1195,7 +1210,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     (vqaf_int8_linear).  Returns (..., N) in out_dtype (default: x's).  Weights in rows that are not whole 16-byte
     pieces are copied into such rows first.  There is no gradient: an input that requires one is refused while
     gradients are recorded."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight_scale, bias)):
+    if (x.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad)) and \
+            torch.is_grad_enabled():
         raise RuntimeError("int8_linear has no gradient: call it under torch.no_grad(), or train the layer in bf16")
     x2, ld = _int8_rows(x, "int8_linear")
     if weight.dim() != 2 or weight.dtype != torch.int8:
@@ -1208,9 +1224,9 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         raise ValueError(f"weight_scale has to be ({N},) float32, got {tuple(weight_scale.shape)} {weight_scale.dtype}")
     if bias is not None and bias.shape != (N,):
         raise ValueError(f"bias has to be ({N},), got {tuple(bias.shape)}")
-    for t in (weight, weight_scale, bias):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"x is on {x.device}, a parameter on {t.device}")
+    if weight.device != x.device or weight_scale.device != x.device or (bias is not None and bias.device != x.device):
+        raise ValueError(f"x is on {x.device}, weight on {weight.device}, weight_scale on {weight_scale.device}"
+                         + ("" if bias is None else f", bias on {bias.device}"))
     dt = out_dtype or x.dtype
     code = _lib.BF16 if dt == torch.bfloat16 else _lib.F32
     if dt not in (torch.float32, torch.bfloat16):
@@ -1238,7 +1254,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
             check(lib.vqaf_int8_linear(x2.data_ptr(), ld, dtype_code(x2), weight.data_ptr(), ldw,
                                        ptr(weight_scale.contiguous()), ptr(bias),
                                        dtype_code(bias) if bias is not None else 0, M, N, K, y.data_ptr(), N, code, ptr(ws),
-                                       need, stream_ptr(x.device)), "vqaf_int8_linear")
+                                       need, _raw_stream(x.device)), "vqaf_int8_linear")
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
