@@ -5,8 +5,10 @@ count roundings for arithmetic in units u = 2^-24 (half an f32 step, relative):
 
   exponent   t = (x - m) log2(e) / T: the difference (1 u |t|), the product (1 u |t|): an error of 2 |t| u in t is one of
              2 ln2 |t| u < 2 |t| u in e = 2^t; the hardware exponential adds one step, 2 u
-  sums       three levels of f32 additions (3 u), the rest in f64; so S is off by at most (2 E|t| + 6) u, relative, with
-             E|t| the mean of |t| under p
+  sums       up to eight f32 additions in a row for S (8 u), the rest in f64; so S is off by at most (2 E|t| + 10) u,
+             relative, with E|t| the mean of |t| under p; sum e t: a product, up to 16 additions in a row and six levels
+             over a wave
+  logarithm  of the sum as f32: one step of the result, 2 u |log S|
   products   u each
 """
 from __future__ import annotations
@@ -46,8 +48,9 @@ def distribution(logits: torch.Tensor, temperature: float):
 
 
 def sum_bound(p, t):
-    """Relative bound of S, an absolute one of log S."""
-    return (2 * (p * t).sum(1) + 6) * U
+    """Relative bound of S, an absolute one of log S (the logarithm's own step included)."""
+    log_s = -torch.log(p.amax(1).clamp_min(1e-300))   # the largest term of S is 1
+    return (2 * (p * t).sum(1) + 10 + 2 * log_s) * U
 
 
 def entropy(lp, p):
@@ -55,8 +58,9 @@ def entropy(lp, p):
 
 
 def entropy_bound(h, p, t):
-    """H = log S - ln2 W / S, W = sum e t: each term e t is off by (2 |t| + 7) u relative, three levels of sums add 3 u."""
-    w = (p * t * (2 * t + 10)).sum(1) * math.log(2.0) * U
+    """H = log S - ln2 W / S, W = sum e t: each term e t is off by (2 |t| + 2 + 2) u relative, the sums add 22 u, the
+    quotient and its factor 4 u."""
+    w = (p * t * (2 * t + 30)).sum(1) * math.log(2.0) * U
     return sum_bound(p, t) * (1 + math.log(2.0) * (p * t).sum(1)) + w + 2 * U * h.abs() + 4 * U
 
 

@@ -1,0 +1,475 @@
+// The distillation loss against a teacher's top answers, with its gradient: a student trained on what a model answers
+// with in place of hard labels (utils/src.py:96).  For the answers i_k with the teacher's probabilities q_k and the rest
+// r that no answer of the list holds, z = x / T, e_j = exp(z_j - max z), S = sum_j e_j, p_j = e_j / S:
+//   L = T^2 [ sum_k q_k (log q_k - log p_{i_k}) + r (log r - log P) ],     P = sum of p_j outside the list
+//   dL / dx_j = T [ p_j (sum q + r) - sum_{k: i_k = j} q_k ] on the list,  T p_j [ sum q + r - r / P ] elsewhere.
+// Rows are held and walked as in answers.hip; the gradient for an incoming gradient of 1 leaves from the same read.
+
+#include "answers.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------
+// Distillation loss, with the gradient of the sum (or mean) in the same pass
+// ---------------------------------------------------------------------------------------------
+// (R,5) f64: m, S, mass = sum q + r, slope = mass - r / P, log Q (q_k = exp(v_k - log Q))
+struct DistillStat {
+  double m, S, mass, slope, log_q;
+};
+
+// a row that is all masked, or that no answer teaches (whatever its logits hold)
+__device__ __forceinline__ bool an_no_gradient(const DistillStat& s) {
+  return s.m == -INFINITY || (s.mass == 0.0 && s.slope == 0.0);
+}
+
+struct DistillGrad {
+  const float* teacher;
+  const int64_t* indices;
+  const DistillStat* stats;
+  const float* up;     // gradient of the loss, one per row (up_step 1) or one (0)
+  int up_step, K, skip_unit;   // skip_unit: nothing is left to do where up[0] is 1 (the gradient is there already)
+  float scale;         // T * (1 for a sum, 1 / R for a mean)
+  AnTemp temp;
+  struct Row {
+    float m, mass, slope, hi, lo, g;
+    double log_q;
+    bool empty;
+  };
+  __device__ __forceinline__ bool done() const { return skip_unit && up[0] == 1.0f; }
+  __device__ __forceinline__ int named() const { return K; }
+  __device__ __forceinline__ void mention(long r, int s, int C, int& idx, float& add) const {
+    const int64_t j = indices[r * K + s];
+    idx = j >= 0 && j < C ? (int)j : -1;
+    add = (float)an_exp((double)teacher[r * K + s] - stats[r].log_q);
+  }
+  __device__ __forceinline__ Row row(long r, int, int) const {
+    Row w;
+    const DistillStat s = stats[r];
+    w.m = (float)s.m;
+    w.empty = an_no_gradient(s);
+    const double inv = w.empty ? 0.0 : 1.0 / s.S;
+    w.mass = (float)(s.mass * inv);
+    w.slope = (float)(s.slope * inv);
+    w.hi = temp.hi;
+    w.lo = temp.lo;
+    w.g = scale * up[r * up_step];
+    return w;
+  }
+  static __device__ __forceinline__ float dense(const Row& w, float x) {
+    return w.empty ? 0.f : w.g * (an_exp2(an_arg(x, w.m, w.hi, w.lo)) * w.slope);
+  }
+  static __device__ __forceinline__ float base(const Row& w, float x) {
+    return w.empty ? 0.f : w.g * (an_exp2(an_arg(x, w.m, w.hi, w.lo)) * w.mass);
+  }
+  static __device__ __forceinline__ float term(const Row& w, float q) { return w.empty ? 0.f : -w.g * q; }
+};
+
+struct DistillArgs {
+  const void* x;
+  const float* teacher;
+  const int64_t* indices;
+  float* row_loss;
+  DistillStat* stats;   // or NULL
+  void* grad;           // or NULL
+  long ld, ldg, R;
+  int C, K, tail;
+  float scale;          // of the gradient: T * (1 or 1 / R)
+  double t2;            // T^2
+  AnTemp temp;
+};
+
+// A row's list of answers in shared memory: the teacher's log probability, the student's logit, the class (-1: none),
+// whether an earlier entry names it too, and, in the end, the teacher's probability.
+struct DistillList {
+  float v[AN_TOP_MAX], x[AN_TOP_MAX], q[AN_TOP_MAX];
+  int idx[AN_TOP_MAX], again[AN_TOP_MAX];
+};
+
+// One wave: the row's statistics and loss from the sum of e over the classes outside the list (s_out) or, without a tail,
+// over all of them (s_all).  `all`: the list covers every class; `bad`: an answer lies past the classes.
+// Short loops on purpose: the pieces of the row are alive around this.
+__device__ __forceinline__ DistillStat an_distill_row(DistillList& list, int K, bool bad, float m, double s_all, double s_out,
+                                                      bool all, bool tail, double inv_t, double& loss) {
+  const int lane = threadIdx.x & 63;
+  const bool empty = m == -INFINITY;
+  DistillStat st;
+  st.m = m;
+  st.S = s_all;
+  st.log_q = 0.0;
+  bool some = true;
+  if (tail) {
+    double own = 0.0;
+#pragma unroll 1
+    for (int k = lane; k < K; k += 64)
+      if (list.idx[k] >= 0 && !list.again[k]) own += an_exp(((double)list.x[k] - (double)m) * inv_t);
+    st.S = s_out + an_wave_sum(own);
+  } else {
+    float vm = -INFINITY;
+    bool nan = false;
+#pragma unroll 1
+    for (int k = lane; k < K; k += 64) {
+      if (list.idx[k] < 0) continue;
+      vm = fmaxf(vm, list.v[k]);
+      nan |= list.v[k] != list.v[k];
+    }
+    vm = an_wave_max(vm);
+    // (a NaN among the values is left out of the maximum and comes back through the sum)
+    some = vm != -INFINITY || __ballot(nan) != 0;
+    if (some) {
+      double sum = 0.0;
+#pragma unroll 1
+      for (int k = lane; k < K; k += 64) sum += list.idx[k] >= 0 ? an_exp((double)list.v[k] - (double)vm) : 0.0;
+      st.log_q = (double)vm + log(an_wave_sum(sum));
+    }
+  }
+  const double log_s = log(st.S);
+  double mass = 0.0, l = 0.0;
+  bool any = false;
+#pragma unroll 1
+  for (int k = lane; k < K; k += 64) {
+    const bool live = list.idx[k] >= 0;
+    const double lq = (double)list.v[k] - st.log_q;
+    const double q = live && some ? an_exp(lq) : 0.0;
+    const double lp = empty ? -INFINITY : ((double)list.x[k] - (double)m) * inv_t - log_s;
+    any |= live;
+    mass += q;
+    if (q != 0.0) l += q * (lq - lp);   // (NaN goes in)
+    list.q[k] = (float)q;
+  }
+  mass = an_wave_sum(mass);
+  l = an_wave_sum(l);
+  double cut = 0.0;
+  if (tail) {
+    double rest = all || __ballot(any) == 0 ? 0.0 : 1.0 - mass;   // (a row without answers teaches nothing)
+    if (!(rest > (double)AN_NO_REST)) rest = 0.0;
+    mass += rest;
+    if (rest > 0.0) {
+      if (empty) {
+        l += INFINITY;
+      } else {
+        const double P = s_out / st.S;
+        l += rest * (log(rest) - log(P));
+        cut = P > 0.0 ? rest / P : (P == 0.0 ? mass : P);
+      }
+    }
+  } else if (some) {
+    mass = mass / mass;   // 1, or NaN
+  }
+  if (bad) l = mass = NAN;
+  st.mass = mass;
+  st.slope = mass - cut;
+  loss = l;
+  return st;
+}
+
+template <int NT>
+struct DistillShared {
+  DistillList list;
+  float s_max[NT / 64];
+  double s_sum[NT / 64];
+  int bad, repeats;
+  DistillStat st;
+};
+
+// The elements of a piece whose bits are set become -inf.
+template <bool BF16>
+__device__ __forceinline__ u32x4 an_drop(u32x4 r, unsigned bits) {
+  unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int j = 0; j < Piece<BF16>::V; ++j) {
+    const bool out = (bits >> j) & 1u;
+    if constexpr (BF16) {
+      const unsigned keep = (j & 1) ? 0x0000ffffu : 0xffff0000u, put = (j & 1) ? 0xff800000u : 0x0000ff80u;
+      w[j >> 1] = out ? ((w[j >> 1] & keep) | put) : w[j >> 1];
+    } else {
+      w[j] = out ? 0xff800000u : w[j];
+    }
+  }
+  return u32x4{w[0], w[1], w[2], w[3]};
+}
+
+// One workgroup per row.  The classes of the list are marked in a bitmap (in units of pieces).  TAIL: their elements are
+// taken out of the registers before the exponentials, so that the rest is summed by itself (1 - sum p would lose what is
+// left of it where the student agrees with its teacher), and their own terms are added by the list.
+// HOLD: the exponentials stay in registers for the gradient (f32: in the place of the logits; bf16: in twice the
+// registers, where that still leaves two workgroups to a CU); otherwise they are formed again.
+template <bool BF16, int NT, int E, bool TAIL, bool HOLD, int W>
+__global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs a) {
+  constexpr int V = Piece<BF16>::V, NW = NT / 64;
+  __shared__ DistillShared<NT> sh;
+  extern __shared__ unsigned s_mark[];   // one bit per element of the pieces
+  const long r = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  RowPieces<BF16, NT, E> row;
+  row.s = an_span<BF16>(a.x, a.ld, r, a.R, a.C);
+  row.load();
+  const void* xr = an_row<BF16>(a.x, a.ld, r);
+  for (int i = tid; i < (row.s.pieces * V + 31) / 32; i += NT) s_mark[i] = 0u;
+  if (tid == 0) sh.bad = sh.repeats = 0;
+  __syncthreads();
+  if (tid < a.K) {
+    const int64_t j = a.indices[r * a.K + tid];
+    const bool live = j >= 0 && j < a.C;
+    int again = 0;
+    sh.list.idx[tid] = live ? (int)j : -1;
+    sh.list.v[tid] = a.teacher[r * a.K + tid];
+    sh.list.x[tid] = live ? an_at<BF16>(xr, j) : 0.f;
+    if (j >= a.C) sh.bad = 1;
+    if (live) {
+      const int b = (int)j + row.s.shift;
+      again = (atomicOr(&s_mark[b >> 5], 1u << (b & 31)) >> (b & 31)) & 1u;
+      if (again) sh.repeats = 1;
+    }
+    sh.list.again[tid] = again;
+  }
+  float m = an_wave_max(row.max());
+  row.renew();
+  if (lane == 0) sh.s_max[wave] = m;
+  __syncthreads();
+  m = sh.s_max[0];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) m = fmaxf(m, sh.s_max[i]);
+  if (m == -INFINITY && an_block_nan<BF16, NT>(row.s)) m = NAN;
+
+  double S = 0.0;   // TAIL: over the classes outside the list
+  const float hi = a.temp.hi, lo = a.temp.lo;
+  const auto marks = [&](int c) { return c < row.s.pieces ? s_mark[(c * V) >> 5] >> ((c * V) & 31) : 0u; };
+  float held[HOLD ? E : 1][V];
+  int at = tid;
+  asm volatile("" : "+v"(at));   // the pieces' columns are computed again, not kept from the load
+  if constexpr (E > 0) {
+    if constexpr (TAIL) {
+      constexpr unsigned all = (1u << V) - 1u;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const unsigned b = marks(at + i * NT) & all;
+        if (b != 0) row.raw[i] = an_drop<BF16>(row.raw[i], b);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      float e[V];
+      an_unpack<BF16>(row.raw[i], e);
+#pragma unroll
+      for (int j = 0; j < V; ++j) e[j] = an_exp2(an_arg(e[j], m, hi, lo));
+      S += (double)an_tree<V>(e);
+      if constexpr (HOLD) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) held[i][j] = e[j];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  } else {
+    row.walk_raw([&](const u32x4 p, int c, int) {
+      float e[V];
+      an_unpack<BF16>(TAIL ? an_drop<BF16>(p, marks(c)) : p, e);
+#pragma unroll
+      for (int j = 0; j < V; ++j) e[j] = an_exp2(an_arg(e[j], m, hi, lo));
+      S += (double)an_tree<V>(e);
+    });
+  }
+  S = an_wave_sum(S);
+  if (lane == 0) sh.s_sum[wave] = S;
+  __syncthreads();
+  if (wave == 0) {
+    S = 0.0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) S += sh.s_sum[i];
+    double loss;
+    // (more than 1024 classes and at most 128 answers: never all of them)
+    const DistillStat st = an_distill_row(sh.list, a.K, sh.bad != 0, m, S, S, false, TAIL, a.temp.inv_t, loss);
+    if (lane == 0) {
+      sh.st = st;
+      a.row_loss[r] = (float)(a.t2 * loss);
+      if (a.stats != nullptr) a.stats[r] = st;
+    }
+  }
+  if (a.grad == nullptr) return;   // uniform
+  __syncthreads();
+  const DistillStat st = sh.st;
+  const bool none = an_no_gradient(st);
+  const double inv = none ? 0.0 : 1.0 / st.S;
+  const float mass = (float)(st.mass * inv), slope = (float)(st.slope * inv) * a.scale;
+  unsigned char* grow = reinterpret_cast<unsigned char*>(a.grad) + r * a.ldg * (BF16 ? 2 : 4);
+  asm volatile("" : "+v"(at));
+  if constexpr (HOLD) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int c = at + i * NT;
+      float g[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) g[j] = none ? 0.f : held[i][j] * slope;
+      if (c < row.s.pieces) an_store<BF16>(grow, c * V - row.s.shift, a.C, g);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  } else {
+    row.renew();
+    row.walk([&](const float (&v)[V], int c, int) {
+      const int here = c - tid + at;
+      if (here >= row.s.pieces) return;
+      float g[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) g[j] = none ? 0.f : an_exp2(an_arg(v[j], m, hi, lo)) * slope;
+      an_store<BF16>(grow, here * V - row.s.shift, a.C, g);
+    });
+  }
+  __syncthreads();
+  const float sc = a.scale;
+  an_write_named<BF16>(sh.list.idx, sh.list.q, a.K, sh.repeats != 0, tid, NT, 0, a.C, xr, grow,
+                       [&](float x) { return none ? 0.f : sc * (an_exp2(an_arg(x, m, hi, lo)) * mass); },
+                       [&](float q) { return none ? 0.f : -sc * q; });
+}
+
+template <bool BF16, int E>
+__global__ __launch_bounds__(64 * AN_WAVES) void distill_wave_kernel(const DistillArgs a) {
+  __shared__ DistillList s_list[AN_WAVES];
+  __shared__ unsigned s_mark[AN_WAVES][AN_WAVE_C / 32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long r = (long)blockIdx.x * AN_WAVES + wave;
+  if (r >= a.R) return;   // no barrier below: a wave keeps to its own row
+  DistillList& list = s_list[wave];
+  unsigned* mark = s_mark[wave];
+  const void* xr = an_row<BF16>(a.x, a.ld, r);
+  float v[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int c = lane + 64 * i;
+    v[i] = c < a.C ? an_at<BF16>(xr, c) : -INFINITY;
+  }
+  if (lane < AN_WAVE_C / 32) mark[lane] = 0u;
+  __builtin_amdgcn_wave_barrier();
+  __threadfence_block();
+  bool beyond = false, named_again = false;
+  for (int k = lane; k < a.K; k += 64) {
+    const int64_t j = a.indices[r * a.K + k];
+    const bool live = j >= 0 && j < a.C;
+    int again = 0;
+    beyond |= j >= a.C;
+    list.idx[k] = live ? (int)j : -1;
+    list.v[k] = a.teacher[r * a.K + k];
+    list.x[k] = live ? an_at<BF16>(xr, j) : 0.f;
+    if (live) again = (atomicOr(&mark[j >> 5], 1u << (j & 31)) >> (j & 31)) & 1u;
+    named_again |= again != 0;
+    list.again[k] = again;
+  }
+  const bool bad = __ballot(beyond) != 0, repeats = __ballot(named_again) != 0;
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < E; ++i) m = fmaxf(m, v[i]);
+  m = an_wave_row_max<E>(v, m);
+  __builtin_amdgcn_wave_barrier();
+  __threadfence_block();
+  double S = 0.0;   // tail: over the classes outside the list
+  int outside = 0;
+  float e32[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int c = lane + 64 * i;
+    const double e = an_exp(((double)v[i] - (double)m) * a.temp.inv_t);
+    e32[i] = (float)e;
+    const bool in = (mark[c >> 5] >> (c & 31)) & 1u;   // E <= 16: c < 1024
+    S += a.tail && in ? 0.0 : e;
+    outside += c < a.C && !in ? 1 : 0;
+  }
+  S = an_wave_sum(S);
+  const bool all = __ballot(outside != 0) == 0;
+  double loss;
+  const DistillStat st = an_distill_row(list, a.K, bad, m, S, S, all, a.tail != 0, a.temp.inv_t, loss);
+  if (lane == 0) {
+    a.row_loss[r] = (float)(a.t2 * loss);
+    if (a.stats != nullptr) a.stats[r] = st;
+  }
+  if (a.grad == nullptr) return;
+  const bool none = an_no_gradient(st);
+  const double inv = none ? 0.0 : 1.0 / st.S;
+  const float mass = (float)(st.mass * inv), slope = (float)(st.slope * inv) * a.scale;
+  unsigned char* grow = reinterpret_cast<unsigned char*>(a.grad) + r * a.ldg * (BF16 ? 2 : 4);
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int c = lane + 64 * i;
+    if (c < a.C) store1<BF16>(grow, (size_t)c, none ? 0.f : e32[i] * slope);
+  }
+  __threadfence_block();
+  __builtin_amdgcn_wave_barrier();
+  const float sc = a.scale;
+  an_write_named<BF16>(list.idx, list.q, a.K, repeats, lane, 64, 0, a.C, xr, grow,
+                       [&](float x) { return none ? 0.f : sc * ((float)an_exp(((double)x - (double)m) * a.temp.inv_t) * mass); },
+                       [&](float t) { return none ? 0.f : -sc * t; });
+}
+
+// out[0] = scale * sum of x[0..n): one workgroup, every thread adds its own in order, waves in order
+__global__ __launch_bounds__(1024) void answer_sum_kernel(const float* x, long n, double scale, float* out) {
+  __shared__ double s_part[16];
+  double s = 0.0;
+  for (long i = threadIdx.x; i < n; i += 1024) s += (double)x[i];
+  s = an_wave_sum(s);
+  if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = s_part[0];
+    for (int w = 1; w < 16; ++w) s += s_part[w];
+    out[0] = (float)(scale * s);
+  }
+}
+
+template <bool BF16>
+int an_launch_distill(const DistillArgs& a, hipStream_t st) {
+  if (a.C <= AN_WAVE_C) {
+    an_by_wave(a.C, [&](auto e) {
+      hipLaunchKernelGGL((distill_wave_kernel<BF16, decltype(e)::value>), dim3((unsigned)((a.R + AN_WAVES - 1) / AN_WAVES)),
+                         dim3(64 * AN_WAVES), 0, st, a);
+    });
+  } else {
+    const size_t mark = ((size_t)a.C + 2 * Piece<BF16>::V + 31) / 32 * 4;
+    VQAF_REQUIRE(mark <= 49152, VQAF_E_SHAPE);   // 393 thousand classes
+    an_by_block<BF16>(a.C, [&](auto nt, auto e) {
+      constexpr int NT = decltype(nt)::value, E = decltype(e)::value;
+      constexpr bool HOLD = E > 0 && (!BF16 || E <= 4);
+      constexpr int W = an_waves(BF16 && HOLD ? 2 * E + 2 : E + 2);
+      if (a.tail) hipLaunchKernelGGL((distill_block_kernel<BF16, NT, E, true, HOLD, W>), dim3((unsigned)a.R), dim3(NT), mark, st, a);
+      else hipLaunchKernelGGL((distill_block_kernel<BF16, NT, E, false, HOLD, W>), dim3((unsigned)a.R), dim3(NT), mark, st, a);
+    });
+  }
+  VQAF_LAUNCH_CHECK();
+}
+
+}  // namespace
+
+extern "C" int vqaf_distill(const void* logits, long ld, const float* teacher, const int64_t* indices, int R, int C, int K,
+                            int dtype, double temperature, int tail, float* row_loss, double* stats, void* grad,
+                            long ld_grad, double scale, float* loss, vqaf_stream_t stream) {
+  VQAF_ENTRY();
+  VQAF_REQUIRE(logits && teacher && indices && row_loss, VQAF_E_NULL);
+  VQAF_REQUIRE(an_shape_ok(ld, R, C, 0, temperature) && K >= 1 && K <= AN_TOP_MAX, VQAF_E_SHAPE);
+  VQAF_REQUIRE(vqaf_dtype_ok(dtype), VQAF_E_DTYPE);
+  VQAF_REQUIRE(an_element_aligned(logits, dtype), VQAF_E_ALIGN);
+  VQAF_REQUIRE(grad == nullptr || an_grad_layout_ok(logits, ld, grad, ld_grad, C, dtype), VQAF_E_ALIGN);
+  DistillArgs a;
+  a.x = logits; a.teacher = teacher; a.indices = indices; a.row_loss = row_loss;
+  a.stats = reinterpret_cast<DistillStat*>(stats); a.grad = grad;
+  a.ld = ld; a.ldg = ld_grad; a.R = R; a.C = C; a.K = K; a.tail = tail != 0;
+  a.scale = (float)(temperature * scale);
+  a.t2 = temperature * temperature;
+  a.temp = an_temp(temperature);
+  const int rc = dtype == VQAF_BF16 ? an_launch_distill<true>(a, (hipStream_t)stream)
+                                    : an_launch_distill<false>(a, (hipStream_t)stream);
+  if (rc != VQAF_OK || loss == nullptr) return rc;
+  hipLaunchKernelGGL(answer_sum_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, row_loss, (long)R, scale, loss);
+  VQAF_LAUNCH_CHECK();
+}
+
+extern "C" int vqaf_distill_bwd(const void* logits, long ld, const float* teacher, const int64_t* indices, int R, int C, int K,
+                                int dtype, double temperature, const double* stats, const float* up, int up_step, int skip_unit,
+                                double scale, void* grad, long ld_grad, vqaf_stream_t stream) {
+  VQAF_ENTRY();
+  VQAF_REQUIRE(logits && teacher && indices && stats && up && grad, VQAF_E_NULL);
+  VQAF_REQUIRE(an_shape_ok(ld, R, C, 0, temperature) && K >= 1 && K <= AN_TOP_MAX && (up_step == 0 || up_step == 1), VQAF_E_SHAPE);
+  VQAF_REQUIRE(vqaf_dtype_ok(dtype), VQAF_E_DTYPE);
+  VQAF_REQUIRE(an_element_aligned(logits, dtype) && an_grad_layout_ok(logits, ld, grad, ld_grad, C, dtype), VQAF_E_ALIGN);
+  DistillGrad op;
+  op.teacher = teacher; op.indices = indices; op.stats = reinterpret_cast<const DistillStat*>(stats); op.up = up;
+  op.up_step = up_step; op.K = K; op.scale = (float)(temperature * scale);
+  op.skip_unit = skip_unit != 0 && up_step == 0;
+  op.temp = an_temp(temperature);
+  return an_launch_grad(op, logits, ld, R, C, dtype, grad, ld_grad, (hipStream_t)stream);
+}
