@@ -320,7 +320,7 @@ __device__ __forceinline__ void an_wave_select(const unsigned (&key)[E], unsigne
 }
 
 template <bool BF16, int E>
-__global__ __launch_bounds__(64 * AN_WAVES) void logprob_wave_kernel(const LogprobArgs a) {
+__global__ __launch_bounds__(64 * AN_WAVES, E <= 8 ? 8 : 5) void logprob_wave_kernel(const LogprobArgs a) {
   __shared__ __attribute__((aligned(16))) u64 s_cand[AN_WAVES][AN_WCAP + 16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long r = (long)blockIdx.x * AN_WAVES + wave;
@@ -339,6 +339,7 @@ __global__ __launch_bounds__(64 * AN_WAVES) void logprob_wave_kernel(const Logpr
   for (int i = 0; i < E; ++i) best = fmaxf(best, v[i]);
   const float m = an_wave_row_max<E>(v, best);
   const bool empty = m == -INFINITY;
+  float xt = t >= 0 && t < a.C ? an_at<BF16>(xr, t) : 0.f;   // on its way under the exponentials
   double S = 0.0;
   float Wt = 0.f;
   const float hi = a.temp.hi;
@@ -367,45 +368,80 @@ __global__ __launch_bounds__(64 * AN_WAVES) void logprob_wave_kernel(const Logpr
     }
   }
   for (int i = lane; i < a.T; i += 64) {
-    if (i >= 64) t = a.targets[r * a.T + i];
-    float lp = 0.f;
-    if (t >= a.C) lp = NAN;
-    else if (t >= 0) lp = an_logprob(an_at<BF16>(xr, t), m, log_s, a.temp.inv_t);
-    a.logprobs[r * a.T + i] = lp;
+    if (i >= 64) {
+      t = a.targets[r * a.T + i];
+      xt = t >= 0 && t < a.C ? an_at<BF16>(xr, t) : 0.f;
+    }
+    a.logprobs[r * a.T + i] = t < 0 ? 0.f : t >= a.C ? NAN : an_logprob(xt, m, log_s, a.temp.inv_t);   // (negative: none)
   }
   if (a.K == 0) return;
 
-  // What the K-th largest of the lanes' maxima reaches is a short list that holds the K best.  Long ties, NaN and
-  // longer lists go by the keys of all elements.
+  // What the K-th largest of the lanes' maxima reaches is a list that holds the K best, short while K is; where it is too
+  // long the bisection goes on over all elements.  Long ties and NaN go by the keys alone.
   u64* cand = s_cand[wave];
   const bool broken = !empty && !(S == S);
   int n = AN_WCAP + 1;
-  if (a.K <= 64 && !broken) {
+  if (!broken) {
     const unsigned mine = lane < a.C ? an_key(best) : 0u;   // (lanes past a short row have none)
-    unsigned up = an_wave_umax(mine), low = an_wave_umin(mine);
-    if (low < AN_KEY_MINF) low = AN_KEY_MINF;
-    while (low < up) {
-      const unsigned mid = low + ((up - low) >> 1) + 1;
-      const int c = __popcll(__ballot(mine >= mid));
-      if (c >= a.K) {
-        low = mid;
-        if (c == a.K) break;
-      } else {
-        up = mid - 1;
+    const unsigned most = an_wave_umax(mine);
+    unsigned up = most, low = AN_KEY_MINF;
+    if (a.K <= 8) {   // so few are found faster one by one: a reduction each, against some fifteen steps
+      unsigned left = mine;
+      low = most;
+      for (int k = 1; k < a.K; ++k) {
+        const u64 who = __ballot(left == low);
+        left = lane == __ffsll((long long)who) - 1 ? 0u : left;
+        low = an_wave_umax(left);
+      }
+      if (low < AN_KEY_MINF) low = AN_KEY_MINF;   // fewer lanes than answers: a short row, all of it
+    } else if (a.K <= 64) {
+      low = an_wave_umin(mine);
+      if (low < AN_KEY_MINF) low = AN_KEY_MINF;
+      while (low < up) {
+        const unsigned mid = low + ((up - low) >> 1) + 1;
+        const int c = __popcll(__ballot(mine >= mid));
+        if (c >= a.K) {
+          low = mid;
+          if (c == a.K) break;
+        } else {
+          up = mid - 1;
+        }
       }
     }
-    const float thr = an_unkey(low);
-    n = 0;
-    const u64 below_lane = (1ull << lane) - 1ull;
+    // what reaches thr into the list, as far as it goes; how many do
+    const auto collect = [&](float thr) {
+      const u64 below_lane = (1ull << lane) - 1ull;
+      int c = 0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const bool take = v[i] >= thr && lane + 64 * i < a.C;
-      const u64 who = __ballot(take);
-      if (who != 0) {
-        const int at = n + __popcll(who & below_lane);
-        if (take && at < AN_WCAP) cand[at] = an_pack(an_key(v[i]), lane + 64 * i);
-        n += __popcll(who);
+      for (int i = 0; i < E; ++i) {
+        const bool take = v[i] >= thr && lane + 64 * i < a.C;
+        const u64 who = __ballot(take);
+        if (who != 0) {
+          const int at = c + __popcll(who & below_lane);
+          if (take && at < AN_WCAP) cand[at] = an_pack(an_key(v[i]), lane + 64 * i);
+          c += __popcll(who);
+        }
       }
+      return c;
+    };
+    n = collect(an_unkey(low));
+    const int enough = a.K + (a.K >> 2) + 32;
+    if (n > enough && low < most) {   // (ranking the list costs its length squared)
+      up = most;
+      while (n > enough && low < up) {
+        const unsigned mid = low + ((up - low) >> 1) + 1;
+        const float thr = an_unkey(mid);
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) c += __popcll(__ballot(v[i] >= thr && lane + 64 * i < a.C));
+        if (c >= a.K) {
+          low = mid;
+          n = c;
+        } else {
+          up = mid - 1;
+        }
+      }
+      n = collect(an_unkey(low));
     }
   }
   if (n > AN_WCAP) {
