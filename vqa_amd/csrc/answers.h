@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "wave.h"
 
 namespace {
 
@@ -32,61 +33,6 @@ __device__ __forceinline__ float an_unkey(unsigned k) {
 constexpr unsigned AN_KEY_MINF = 0x007fffffu;   // an_key(-inf): the lowest key of any value
 __device__ __forceinline__ u64 an_pack(unsigned key, int idx) { return ((u64)key << 32) | (unsigned)~idx; }
 __device__ __forceinline__ int an_index(u64 c) { return (int)~(unsigned)c; }
-
-// ---------------------------------------------------------------------------------------------
-// Wave reductions through DPP; the result is in every lane (read from lane 63).
-// ---------------------------------------------------------------------------------------------
-template <int CTRL, int ROWS>
-__device__ __forceinline__ unsigned an_dpp(unsigned idle, unsigned x) {
-  return (unsigned)__builtin_amdgcn_update_dpp((int)idle, (int)x, CTRL, ROWS, 0xf, false);
-}
-template <class F>
-__device__ __forceinline__ unsigned an_wave_u32(unsigned x, unsigned idle, F f) {
-  x = f(x, an_dpp<0x111, 0xf>(idle, x));
-  x = f(x, an_dpp<0x112, 0xf>(idle, x));
-  x = f(x, an_dpp<0x114, 0xf>(idle, x));
-  x = f(x, an_dpp<0x118, 0xf>(idle, x));
-  x = f(x, an_dpp<0x142, 0xa>(idle, x));
-  x = f(x, an_dpp<0x143, 0xc>(idle, x));
-  return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
-}
-__device__ __forceinline__ float an_wave_max(float v) {
-  return __uint_as_float(an_wave_u32(__float_as_uint(v), 0xff800000u, [](unsigned a, unsigned b) {
-    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
-  }));
-}
-__device__ __forceinline__ float an_wave_fsum(float v) {
-  return __uint_as_float(an_wave_u32(__float_as_uint(v), 0u, [](unsigned a, unsigned b) {
-    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
-  }));
-}
-__device__ __forceinline__ unsigned an_wave_umax(unsigned v) {
-  return an_wave_u32(v, 0u, [](unsigned a, unsigned b) { return a > b ? a : b; });
-}
-__device__ __forceinline__ unsigned an_wave_umin(unsigned v) {
-  return an_wave_u32(v, 0xffffffffu, [](unsigned a, unsigned b) { return a < b ? a : b; });
-}
-__device__ __forceinline__ unsigned an_wave_uadd(unsigned v) {
-  return an_wave_u32(v, 0u, [](unsigned a, unsigned b) { return a + b; });
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double an_dadd(double x) {
-  const u64 u = __builtin_bit_cast(u64, x);
-  const u64 o = ((u64)an_dpp<CTRL, ROWS>(0u, (unsigned)(u >> 32)) << 32) | an_dpp<CTRL, ROWS>(0u, (unsigned)u);
-  return x + __builtin_bit_cast(double, o);   // idle lanes contribute +0
-}
-__device__ __forceinline__ double an_wave_sum(double x) {
-  x = an_dadd<0x111, 0xf>(x);
-  x = an_dadd<0x112, 0xf>(x);
-  x = an_dadd<0x114, 0xf>(x);
-  x = an_dadd<0x118, 0xf>(x);
-  x = an_dadd<0x142, 0xa>(x);
-  x = an_dadd<0x143, 0xc>(x);
-  const u64 u = __builtin_bit_cast(u64, x);
-  const u64 r = ((u64)(unsigned)__builtin_amdgcn_readlane((int)(u >> 32), 63) << 32) |
-                (unsigned)__builtin_amdgcn_readlane((int)(unsigned)u, 63);
-  return __builtin_bit_cast(double, r);
-}
 
 // exp(t) for t <= 0 to about 2^-40: t = k ln 2 + f with |f| <= ln 2 / 2, Taylor's polynomial of degree 10 in f
 // (the first term left out is f^11 / 11! < 2^-41).  NaN stays NaN; below -700 the result is zero.
@@ -381,7 +327,7 @@ constexpr int AN_WAVES = 4;   // rows per workgroup
 // maximum over the wave; NaN for a row that holds nothing else but -inf (the maximum leaves NaN out)
 template <int E>
 __device__ __forceinline__ float an_wave_row_max(const float (&v)[E], float m) {
-  m = an_wave_max(m);
+  m = dpp_wave_max(m);
   if (m == -INFINITY) {
     bool nan = false;
 #pragma unroll

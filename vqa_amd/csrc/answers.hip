@@ -80,7 +80,7 @@ __device__ __forceinline__ int an_block_count(const ROW& row, int* cnt, F f) {
 #pragma unroll
     for (int j = 0; j < V; ++j) n += (el + j >= 0 && el + j < row.s.C && f(v[j], el + j)) ? 1u : 0u;
   });
-  n = an_wave_uadd(n);
+  n = dpp_wave_uadd(n);
   if ((threadIdx.x & 63) == 0) atomicAdd(&cnt[0], (int)n);
   __syncthreads();
   return cnt[0];
@@ -142,8 +142,8 @@ __device__ __forceinline__ float an_threshold(const float* tmax, int threads_wit
   unsigned best = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) best = k[i] > best ? k[i] : best;
-  hi = an_wave_umax(best);
-  lo = an_wave_umin(best);                      // 64 maxima reach it if every lane has one
+  hi = dpp_wave_umax(best);
+  lo = dpp_wave_umin(best);                      // 64 maxima reach it if every lane has one
   if (K > 64 || lo < AN_KEY_MINF) lo = AN_KEY_MINF;
   const int most = K + (K >> 1) + 16;
   // invariant: at least K maxima are >= lo; fewer than K are >= hi + 1
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(NT, W) void logprob_block_kernel(const LogprobArgs 
     sh.tmax[tid] = m;
     if (tid == 0) sh.n = 0;
   }
-  m = an_wave_max(m);
+  m = dpp_wave_max(m);
   if (lane == 0) s_max[wave] = m;
   __syncthreads();
   m = s_max[0];
@@ -203,8 +203,8 @@ __global__ __launch_bounds__(NT, W) void logprob_block_kernel(const LogprobArgs 
     S += (double)an_tree<V>(e);
     Wt += (double)an_tree<V>(w);
   });
-  S = an_wave_sum(S);
-  Wt = an_wave_sum(Wt);
+  S = dpp_wave_sum(S);
+  Wt = dpp_wave_sum(Wt);
   if (lane == 0) {
     s_sum[0][wave] = S;
     s_sum[1][wave] = Wt;
@@ -289,7 +289,7 @@ __device__ __forceinline__ void an_wave_select(const unsigned (&key)[E], unsigne
   unsigned best = key[0];
 #pragma unroll
   for (int i = 1; i < E; ++i) best = key[i] > best ? key[i] : best;
-  unsigned up = an_wave_umax(best);
+  unsigned up = dpp_wave_umax(best);
   while (low < up) {
     const unsigned mid = low + ((up - low) >> 1) + 1;
     int c = 0;
@@ -355,8 +355,8 @@ __global__ __launch_bounds__(64 * AN_WAVES, E <= 8 ? 8 : 5) void logprob_wave_ke
     S += (double)es;
     Wt += ws;
   }
-  S = an_wave_sum(S);
-  const float w = an_wave_fsum(Wt), s32 = (float)S;
+  S = dpp_wave_sum(S);
+  const float w = dpp_wave_sum(Wt), s32 = (float)S;
   // log S: the f32 logarithm of the rounded sum and the rounding's share
   const float mean_t = (float)AN_LN2 * (w / s32);
   const double log_s = empty ? -INFINITY : (double)logf(s32) + (S - (double)s32) / s32 - a.temp.delta * mean_t;
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(64 * AN_WAVES, E <= 8 ? 8 : 5) void logprob_wave_ke
   int n = AN_WCAP + 1;
   if (!broken) {
     const unsigned mine = lane < a.C ? an_key(best) : 0u;   // (lanes past a short row have none)
-    const unsigned most = an_wave_umax(mine);
+    const unsigned most = dpp_wave_umax(mine);
     unsigned up = most, low = AN_KEY_MINF;
     if (a.K <= 8) {   // so few are found faster one by one: a reduction each, against some fifteen steps
       unsigned left = mine;
@@ -391,11 +391,11 @@ __global__ __launch_bounds__(64 * AN_WAVES, E <= 8 ? 8 : 5) void logprob_wave_ke
       for (int k = 1; k < a.K; ++k) {
         const u64 who = __ballot(left == low);
         left = lane == __ffsll((long long)who) - 1 ? 0u : left;
-        low = an_wave_umax(left);
+        low = dpp_wave_umax(left);
       }
       if (low < AN_KEY_MINF) low = AN_KEY_MINF;   // fewer lanes than answers: a short row, all of it
     } else if (a.K <= 64) {
-      low = an_wave_umin(mine);
+      low = dpp_wave_umin(mine);
       if (low < AN_KEY_MINF) low = AN_KEY_MINF;
       while (low < up) {
         const unsigned mid = low + ((up - low) >> 1) + 1;
@@ -512,7 +512,7 @@ struct LogprobGrad {
       mention(r, s, C, j, g);
       sum += (double)g;
     }
-    w.A = (float)an_wave_sum(sum);
+    w.A = (float)dpp_wave_sum(sum);
     w.hi = temp.hi;
     w.lo = temp.lo;
     w.inv_t = (float)temp.inv_t;

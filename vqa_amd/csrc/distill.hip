@@ -102,7 +102,7 @@ __device__ __forceinline__ DistillStat an_distill_row(DistillList& list, int K, 
 #pragma unroll 1
     for (int k = lane; k < K; k += 64)
       if (list.idx[k] >= 0 && !list.again[k]) own += an_exp(((double)list.x[k] - (double)m) * inv_t);
-    st.S = s_out + an_wave_sum(own);
+    st.S = s_out + dpp_wave_sum(own);
   } else {
     float vm = -INFINITY;
     bool nan = false;
@@ -112,14 +112,14 @@ __device__ __forceinline__ DistillStat an_distill_row(DistillList& list, int K, 
       vm = fmaxf(vm, list.v[k]);
       nan |= list.v[k] != list.v[k];
     }
-    vm = an_wave_max(vm);
+    vm = dpp_wave_max(vm);
     // (a NaN among the values is left out of the maximum and comes back through the sum)
     some = vm != -INFINITY || __ballot(nan) != 0;
     if (some) {
       double sum = 0.0;
 #pragma unroll 1
       for (int k = lane; k < K; k += 64) sum += list.idx[k] >= 0 ? an_exp((double)list.v[k] - (double)vm) : 0.0;
-      st.log_q = (double)vm + log(an_wave_sum(sum));
+      st.log_q = (double)vm + log(dpp_wave_sum(sum));
     }
   }
   const double log_s = log(st.S);
@@ -136,8 +136,8 @@ __device__ __forceinline__ DistillStat an_distill_row(DistillList& list, int K, 
     if (q != 0.0) l += q * (lq - lp);   // (NaN goes in)
     list.q[k] = (float)q;
   }
-  mass = an_wave_sum(mass);
-  l = an_wave_sum(l);
+  mass = dpp_wave_sum(mass);
+  l = dpp_wave_sum(l);
   double cut = 0.0;
   if (tail) {
     double rest = all || __ballot(any) == 0 ? 0.0 : 1.0 - mass;   // (a row without answers teaches nothing)
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs 
     }
     sh.list.again[tid] = again;
   }
-  float m = an_wave_max(row.max());
+  float m = dpp_wave_max(row.max());
   row.renew();
   if (lane == 0) sh.s_max[wave] = m;
   __syncthreads();
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs 
       S += (double)an_tree<V>(e);
     });
   }
-  S = an_wave_sum(S);
+  S = dpp_wave_sum(S);
   if (lane == 0) sh.s_sum[wave] = S;
   __syncthreads();
   if (wave == 0) {
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(64 * AN_WAVES) void distill_wave_kernel(const Disti
     S += a.tail && in ? 0.0 : e;
     outside += c < a.C && !in ? 1 : 0;
   }
-  S = an_wave_sum(S);
+  S = dpp_wave_sum(S);
   const bool all = __ballot(outside != 0) == 0;
   double loss;
   const DistillStat st = an_distill_row(list, a.K, bad, m, S, S, all, a.tail != 0, a.temp.inv_t, loss);
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(1024) void answer_sum_kernel(const float* x, long n
   __shared__ double s_part[16];
   double s = 0.0;
   for (long i = threadIdx.x; i < n; i += 1024) s += (double)x[i];
-  s = an_wave_sum(s);
+  s = dpp_wave_sum(s);
   if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) {

@@ -14,7 +14,10 @@
 // workgroup takes 16 output channels, its waves cut the contraction among themselves and read the weights straight into
 // MFMA operands.  Up to a few tokens the workgroups also quantise the rows themselves and one launch does it all.
 
+#include <mutex>
+
 #include "common.h"
+#include "wave.h"
 
 namespace {
 
@@ -22,10 +25,10 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int I8_MAX_K = 131072;
-constexpr int I8_BK = 128;   // bytes (values) of a row in one k-step
+constexpr int I8_ROW = 128;   // rows of quantised tokens are whole multiples of this many bytes
 
 // ---------------------------------------------------------------------------------------------
-// One value.  s is at least 2^-126 and |x| <= 127.00001 s.
+// One value.  s is at least 2^-126 and |x| <= 127.00001 s, so the result stays in [-127, 127].
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ int i8_round(float x, float s, float inv) {
   float q = rintf(x * inv);
@@ -33,7 +36,7 @@ __device__ __forceinline__ int i8_round(float x, float s, float inv) {
   const bool odd = ((int)q) & 1;
   if (up > 0.f || (up == 0.f && odd)) q += 1.f;
   else if (down < 0.f || (down == 0.f && odd)) q -= 1.f;
-  return (int)fminf(fmaxf(q, -127.f), 127.f);
+  return (int)q;
 }
 __device__ __forceinline__ float i8_scale(float amax) { return fmaxf(__fdiv_rn(amax, 127.f), 1.17549435e-38f); }
 __device__ __forceinline__ unsigned i8_pack(int a, int b, int c, int d) {
@@ -58,20 +61,30 @@ __device__ __forceinline__ void i8_load8(const void* row, int k, int K, float (&
     for (int j = 0; j < 8; ++j) v[j] = k + j < K ? load1<BF16>(row, (size_t)(k + j)) : 0.f;
   }
 }
-// maximum of |v| that carries NaN and infinity as NaN: `bad` collects them
-__device__ __forceinline__ void i8_amax8(const float (&v)[8], float& amax, bool& bad) {
+// Maximum of |v| as bits: NaN lies above infinity, infinity above every number.
+__device__ __forceinline__ unsigned i8_amax8(const float (&v)[8], unsigned amax) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float a = fabsf(v[j]);
-    bad |= !(a < INFINITY);
-    amax = fmaxf(amax, a);
-  }
+  for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
+  return amax;
 }
+__device__ __forceinline__ bool i8_bad(unsigned amax) { return amax >= 0x7f800000u; }
+// x * inv is off by less than 2^-15 steps, so only a remainder that close to half a step leaves a doubt
 __device__ __forceinline__ u32x2 i8_quant8(const float (&v)[8], float s, float inv, bool bad) {
   int q[8];
+  bool doubt = false;
+  const float near = 0.49996f * s;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = bad ? 0 : i8_round(v[j], s, inv);
-  return u32x2{i8_pack(q[0], q[1], q[2], q[3]), i8_pack(q[4], q[5], q[6], q[7])};
+  for (int j = 0; j < 8; ++j) {
+    const float f = rintf(v[j] * inv);
+    doubt |= fabsf(fmaf(-f, s, v[j])) > near;
+    q[j] = (int)f;
+  }
+  if (doubt) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = i8_round(v[j], s, inv);
+  }
+  const u32x2 r = u32x2{i8_pack(q[0], q[1], q[2], q[3]), i8_pack(q[4], q[5], q[6], q[7])};
+  return bad ? u32x2{0, 0} : r;
 }
 
 // One wave per row: E x 512 columns in registers, or (E = 0) the row read twice.  Writes zeros up to the row's pitch.
@@ -82,17 +95,16 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantArgs a) {
   if (m >= a.M) return;
   const void* row = reinterpret_cast<const unsigned char*>(a.x) + m * a.ldx * (BF16 ? 2 : 4);
   int8_t* out = a.q + m * a.ldq;
-  float amax = 0.f;
-  bool bad = false;
+  unsigned top = 0;
   if constexpr (E > 0) {
     float v[E][8];
 #pragma unroll
     for (int i = 0; i < E; ++i) i8_load8<BF16, VEC>(row, i * 512 + lane * 8, a.K, v[i]);
 #pragma unroll
-    for (int i = 0; i < E; ++i) i8_amax8(v[i], amax, bad);
-    amax = wave_max(amax);
-    bad = __ballot(bad) != 0;
-    const float s = i8_scale(amax), inv = 1.0f / s;
+    for (int i = 0; i < E; ++i) top = i8_amax8(v[i], top);
+    top = dpp_wave_umax(top);
+    const bool bad = i8_bad(top);
+    const float s = i8_scale(__uint_as_float(top)), inv = 1.0f / s;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const int k = i * 512 + lane * 8;
@@ -103,11 +115,11 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantArgs a) {
     for (int k = lane * 8; k < a.K; k += 512) {
       float v[8];
       i8_load8<BF16, VEC>(row, k, a.K, v);
-      i8_amax8(v, amax, bad);
+      top = i8_amax8(v, top);
     }
-    amax = wave_max(amax);
-    bad = __ballot(bad) != 0;
-    const float s = i8_scale(amax), inv = 1.0f / s;
+    top = dpp_wave_umax(top);
+    const bool bad = i8_bad(top);
+    const float s = i8_scale(__uint_as_float(top)), inv = 1.0f / s;
     for (int k = lane * 8; k < a.ldq; k += 512) {
       float v[8];
       i8_load8<BF16, VEC>(row, k, a.K, v);
@@ -118,10 +130,10 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many tokens: 64 TM x 64 TN output tiles, four waves of 32 TM x 32 TN
+// Many tokens
 // ---------------------------------------------------------------------------------------------
 struct Int8Args {
-  const int8_t* q;        // (M, ldq) with zeros from K to ldq, a multiple of I8_BK
+  const int8_t* q;        // (M, ldq) with zeros from K to ldq, a multiple of I8_ROW
   const int8_t* w;        // (N, ldw), K values in whole 16-byte pieces
   const float* x_scale;
   const float* w_scale;
@@ -136,118 +148,48 @@ __device__ __forceinline__ void i8_glds16(const void* src, void* lds_dst) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
                                    (__attribute__((address_space(3))) void*)lds_dst, 16, 0, 0);
 }
-// piece c (16 values) of row r of a [rows][128] image lies at position c ^ i8_swz(r): the rows that one group of
-// ds_read_b128 lanes touches then fall on distinct 16-byte slots of the bank row
-__device__ __forceinline__ int i8_swz(int r) { return (r >> 1) & 7; }
-
 __device__ __forceinline__ float i8_bias(const Int8Args& g, int n) {
   if (g.bias == nullptr) return 0.f;
   return g.bias_bf16 ? bf16_to_f32(reinterpret_cast<const bf16_t*>(g.bias)[n]) : reinterpret_cast<const float*>(g.bias)[n];
 }
 
+// A wave's 32 TM tokens x 32 TN channels from (m0, n0) on: scales, bias, rounding, and out through an image of 32 tokens
+// in shared memory, so that stores are whole 16-byte pieces of rows.
+// acc[i][j][e]: token 32 i + (lane & 31), channel 32 j + (e & 3) + 8 (e >> 2) + 4 (lane >> 5)
 template <bool OUT_BF16, int TM, int TN>
-__global__ __launch_bounds__(256) void int8_tile_kernel(const Int8Args g) {
-  constexpr int BM = 64 * TM, BN = 64 * TN, XB = BM * I8_BK, WB = BN * I8_BK;
+__device__ __forceinline__ void i8_write_tile(const Int8Args& g, i32x16 (&acc)[TM][TN], unsigned char* img, int m0, int n0,
+                                              int lane) {
   constexpr int ES = OUT_BF16 ? 2 : 4;
-  constexpr int PITCH = 32 * TN * ES + (OUT_BF16 ? 8 : 16);   // of a wave's image of 32 tokens x 32 TN channels
-  constexpr int IMG = 4 * 32 * PITCH;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[XB + WB > IMG ? XB + WB : IMG];
-  // each XCD gets a contiguous run of tiles, columns fastest (workgroup ids go round-robin over the 8 XCDs)
-  const int nt = g.tiles_m * g.tiles_n;
-  const int xcd = blockIdx.x & 7, share = nt >> 3, more = nt & 7;
-  const int lin = (xcd < more ? xcd * (share + 1) : more * (share + 1) + (xcd - more) * share) + (blockIdx.x >> 3);
-  const int tile_m = lin / g.tiles_n, tile_n = lin - tile_m * g.tiles_n;
-  const int m0 = tile_m * BM, n0 = tile_n * BN;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave >> 1, wn = wave & 1, half = lane >> 5;
-
-  // LDS-DMA sources: piece j * 256 + tid -> (row piece / 8, position piece % 8)
-  constexpr int XJ = 2 * TM, WJ = 2 * TN;
-  const int8_t* xs[XJ];
-  const int8_t* ws[WJ];
-  int wk[WJ];
+  constexpr int PITCH = 32 * TN * ES + (OUT_BF16 ? 8 : 16);
+  const int half = lane >> 5;
+  float sx[TM];
 #pragma unroll
-  for (int j = 0; j < XJ; ++j) {
-    const int p = j * 256 + tid, row = p >> 3, c = (p & 7) ^ i8_swz(row);
-    xs[j] = g.q + (long)min(m0 + row, g.M - 1) * g.ldq + c * 16;   // rows past the edge repeat the last one;
-  }
+  for (int i = 0; i < TM; ++i) sx[i] = g.x_scale[min(m0 + i * 32 + (lane & 31), g.M - 1)];
 #pragma unroll
-  for (int j = 0; j < WJ; ++j) {
-    const int p = j * 256 + tid, row = p >> 3, c = (p & 7) ^ i8_swz(row);
-    ws[j] = g.w + (long)min(n0 + row, g.N - 1) * g.ldw + c * 16;   // their outputs are not stored
-    wk[j] = c * 16;
-  }
-  unsigned char* const dma_x = lds + wave * 1024;
-  unsigned char* const dma_w = lds + XB + wave * 1024;
-
-  int xr[TM], wr[TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) xr[i] = wm * 32 * TM + i * 32 + (lane & 31);
-#pragma unroll
-  for (int j = 0; j < TN; ++j) wr[j] = wn * 32 * TN + j * 32 + (lane & 31);
-
-  i32x16 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
-
-  const int T = (int)(g.ldq / I8_BK);
-  for (int t = 0; t < T; ++t) {
-    const int k0 = t * I8_BK;
-#pragma unroll
-    for (int j = 0; j < XJ; ++j) i8_glds16(xs[j] + k0, dma_x + j * 4096);
-#pragma unroll
-    for (int j = 0; j < WJ; ++j) {
-      // pieces past the weights' row (the tokens' integers are zero there) come from the block of zeros
-      const void* src = k0 + wk[j] < g.K ? (const void*)(ws[j] + k0) : (const void*)g.zeros;
-      i8_glds16(src, dma_w + j * 4096);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      i32x4 xf[TM], wf[TN];
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-        xf[i] = *reinterpret_cast<const i32x4*>(lds + xr[i] * I8_BK + (((2 * ks + half) ^ i8_swz(xr[i])) << 4));
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-        wf[j] = *reinterpret_cast<const i32x4*>(lds + XB + wr[j] * I8_BK + (((2 * ks + half) ^ i8_swz(wr[j])) << 4));
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[j], xf[i], acc[i][j], 0, 0, 0);
-    }
-    __syncthreads();
-  }
-
-  // acc[i][j][e]: token wm 32 TM + 32 i + (lane & 31), channel wn 32 TN + 32 j + (e & 3) + 8 (e >> 2) + 4 half
-  unsigned char* const img = lds + wave * (32 * PITCH);
-  float sw[TN][16], bv[TN][16];
-#pragma unroll
-  for (int j = 0; j < TN; ++j)
+  for (int j = 0; j < TN; ++j) {   // in place: the sums become the outputs' bits
+    float sw[16], bv[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int n = min(n0 + (wn * TN + j) * 32 + (e & 3) + 8 * (e >> 2) + 4 * half, g.N - 1);
-      sw[j][e] = g.w_scale[n];
-      bv[j][e] = i8_bias(g, n);
+      const int n = min(n0 + j * 32 + (e & 3) + 8 * (e >> 2) + 4 * half, g.N - 1);
+      sw[e] = g.w_scale[n];
+      bv[e] = i8_bias(g, n);
     }
 #pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        acc[i][j][e] = __float_as_int(fmaf((float)acc[i][j][e] * sx[i], sw[e], bv[e]));
+    __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const float sx = g.x_scale[min(m0 + xr[i], g.M - 1)];
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] = fmaf((float)acc[i][j][4 * r + e] * sx, sw[j][4 * r + e], bv[j][4 * r + e]);
+        for (int e = 0; e < 4; ++e) v[e] = __int_as_float(acc[i][j][4 * r + e]);
         unsigned char* at = img + (lane & 31) * PITCH + (j * 32 + 8 * r + 4 * half) * ES;
         if constexpr (OUT_BF16) *reinterpret_cast<u32x2*>(at) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
         else *reinterpret_cast<f32x4*>(at) = f32x4{v[0], v[1], v[2], v[3]};
@@ -257,7 +199,7 @@ __global__ __launch_bounds__(256) void int8_tile_kernel(const Int8Args g) {
 #pragma unroll
     for (int it = 0; it < 32 / ROWS; ++it) {
       const int ml = it * ROWS + lane / CH, c = lane % CH;
-      const int m = m0 + (wm * TM + i) * 32 + ml, n = n0 + wn * 32 * TN + c * PER;
+      const int m = m0 + i * 32 + ml, n = n0 + c * PER;
       const unsigned char* at = img + ml * PITCH + c * 16;
       const u32x2 lo = *reinterpret_cast<const u32x2*>(at), hi = *reinterpret_cast<const u32x2*>(at + 8);
       if (m < g.M && n < g.N) {
@@ -279,6 +221,141 @@ __global__ __launch_bounds__(256) void int8_tile_kernel(const Int8Args g) {
   }
 }
 
+// The product: output tiles of 32 TM WM tokens x 32 TN WN channels, a workgroup of WM x WN waves of 32 TM x 32 TN each.
+// k-steps of 64 values go through a ring of STAGES stages in shared memory, all but one of them in flight, one barrier a
+// step.  The fragment reads are inline assembly: for a read it can see, the compiler waits until every LDS-DMA has landed
+// and would drain the ring.  Each block of reads waits for itself; the other waves of the SIMD multiply meanwhile.
+constexpr int I8_BK = 64;
+
+// piece c (16 values) of row r of a [rows][64] image lies at position c ^ i8_swz(r): sixteen rows on sixteen slots
+__device__ __forceinline__ int i8_swz(int r) { return (r >> 2) & 3; }
+
+// one k32 step of a wave: TM token and TN channel fragments (blocks of 32 rows are 2048 bytes apart and swizzled alike)
+template <int TM, int TN>
+__device__ __forceinline__ void i8_step(unsigned xa, unsigned wa, i32x16 (&acc)[TM][TN]) {
+  i32x4 x[TM], w[TN];
+  if constexpr (TM == 4 && TN == 2) {
+    asm volatile("ds_read_b128 %4, %7\n\t"
+                 "ds_read_b128 %0, %6\n\t"
+                 "ds_read_b128 %5, %7 offset:2048\n\t"
+                 "ds_read_b128 %1, %6 offset:2048\n\t"
+                 "ds_read_b128 %2, %6 offset:4096\n\t"
+                 "ds_read_b128 %3, %6 offset:6144\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(w[0]), "=&v"(w[1])
+                 : "v"(xa), "v"(wa)
+                 : "memory");
+  } else if constexpr (TM == 2 && TN == 2) {
+    asm volatile("ds_read_b128 %2, %5\n\t"
+                 "ds_read_b128 %0, %4\n\t"
+                 "ds_read_b128 %3, %5 offset:2048\n\t"
+                 "ds_read_b128 %1, %4 offset:2048\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(w[0]), "=&v"(w[1])
+                 : "v"(xa), "v"(wa)
+                 : "memory");
+  } else {
+    static_assert(TM == 1 && TN == 1, "shapes with a block of reads");
+    asm volatile("ds_read_b128 %1, %3\n\t"
+                 "ds_read_b128 %0, %2\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(w[0])
+                 : "v"(xa), "v"(wa)
+                 : "memory");
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[j], x[i], acc[i][j], 0, 0, 0);
+}
+
+template <bool OUT_BF16, int TM, int TN, int WM, int WN, int STAGES, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void int8_tile_kernel(const Int8Args g) {
+  constexpr int THREADS = 64 * WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN;
+  constexpr int XB = BM * I8_BK, STAGE = (BM + BN) * I8_BK;
+  constexpr int XJ = BM * 4 / THREADS, WJ = BN * 4 / THREADS, D = XJ + WJ;   // LDS-DMA instructions a thread and stage
+  constexpr int IMG = 32 * (32 * TN * (OUT_BF16 ? 2 : 4) + (OUT_BF16 ? 8 : 16));
+  static_assert(XJ * THREADS == BM * 4 && WJ * THREADS == BN * 4, "whole rounds of LDS-DMA");
+  static_assert(WM * WN * IMG <= STAGES * STAGE, "the output images fit the ring");
+  extern __shared__ __attribute__((aligned(16))) unsigned char i8_lds[];   // STAGES * STAGE
+  // each XCD gets a contiguous run of tiles (workgroup ids go round-robin over the 8 XCDs), in groups of four tile rows
+  // with the columns slower within a group: what an XCD works on at a time shares operand rows both ways
+  const int nt = g.tiles_m * g.tiles_n;
+  const int xcd = blockIdx.x & 7, share = nt >> 3, more = nt & 7;
+  const int lin = (xcd < more ? xcd * (share + 1) : more * (share + 1) + (xcd - more) * share) + (blockIdx.x >> 3);
+  const int group = lin / (4 * g.tiles_n), first = group * 4, rows = min(4, g.tiles_m - first);
+  const int in = lin - group * 4 * g.tiles_n, tile_n = in / rows, tile_m = first + in - tile_n * rows;
+  const int m0 = tile_m * BM, n0 = tile_n * BN;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN, half = lane >> 5;
+
+  // LDS-DMA sources: piece j * THREADS + tid -> (row piece / 4, position piece % 4)
+  const int8_t* xs[XJ];
+  const int8_t* ws[WJ];
+  int wk[WJ];
+#pragma unroll
+  for (int j = 0; j < XJ; ++j) {
+    const int p = j * THREADS + tid, row = p >> 2, c = (p & 3) ^ i8_swz(row);
+    xs[j] = g.q + (long)min(m0 + row, g.M - 1) * g.ldq + c * 16;   // rows past the edge repeat the last one;
+  }
+#pragma unroll
+  for (int j = 0; j < WJ; ++j) {
+    const int p = j * THREADS + tid, row = p >> 2, c = (p & 3) ^ i8_swz(row);
+    ws[j] = g.w + (long)min(n0 + row, g.N - 1) * g.ldw + c * 16;   // their outputs are not stored
+    wk[j] = c * 16;
+  }
+  auto issue = [&](int t, int slot) {
+    unsigned char* st = i8_lds + slot * STAGE + wave * 1024;
+    const int k0 = t * I8_BK;
+#pragma unroll
+    for (int j = 0; j < XJ; ++j) i8_glds16(xs[j] + k0, st + j * (THREADS * 16));
+#pragma unroll
+    for (int j = 0; j < WJ; ++j)   // pieces past the weights' row (the tokens are zero there) come from the block of zeros
+      i8_glds16(k0 + wk[j] < g.K ? (const void*)(ws[j] + k0) : (const void*)g.zeros, st + XB + j * (THREADS * 16));
+  };
+
+  const unsigned base = (unsigned)reinterpret_cast<size_t>((__attribute__((address_space(3))) unsigned char*)i8_lds);
+  unsigned xa[2], wa[2];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks) {
+    const int r = lane & 31;
+    const unsigned at = base + (unsigned)(r * I8_BK + (((2 * ks + half) ^ i8_swz(r)) << 4));
+    xa[ks] = at + wm * (32 * TM * I8_BK);
+    wa[ks] = at + XB + wn * (32 * TN * I8_BK);
+  }
+
+  i32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+
+  const int T = (int)(g.ldq / I8_BK);
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < T) issue(s, s);
+  int slot = 0;
+  for (int t = 0; t < T; ++t) {
+    // stage t has landed when the instructions of the stages behind it are all that is left
+    const int behind = min(T - 1 - t, STAGES - 2);
+    if (behind == STAGES - 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * D) : "memory");
+    else if (behind >= 2 && STAGES > 4) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * D) : "memory");
+    else if (behind >= 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(D) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();   // everyone's has, and everyone is done with stage t - 1
+    if (t + STAGES - 1 < T) issue(t + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
+    const unsigned st = (unsigned)(slot * STAGE);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) i8_step<TM, TN>(xa[ks] + st, wa[ks] + st, acc);
+    slot = slot == STAGES - 1 ? 0 : slot + 1;
+  }
+  __syncthreads();   // the ring becomes the waves' output images
+  i8_write_tile<OUT_BF16, TM, TN>(g, acc, i8_lds + wave * IMG, m0 + wm * 32 * TM, n0 + wn * 32 * TN, lane);
+}
+
 // ---------------------------------------------------------------------------------------------
 // Few tokens: 16 output channels per workgroup, the contraction cut among its four waves
 // ---------------------------------------------------------------------------------------------
@@ -289,8 +366,7 @@ constexpr int I8_SELF_K = 8192;     // and the columns up to which they do
 template <bool X_BF16, bool OUT_BF16, int MT, bool SELF>
 __global__ __launch_bounds__(256) void int8_few_kernel(const Int8Args g, const void* x, long ldx, int x_vec) {
   __shared__ __attribute__((aligned(16))) i32x4 s_part[4][MT][64];
-  __shared__ float s_red[4];
-  __shared__ int s_bad[4];
+  __shared__ unsigned s_top[4];
   __shared__ float s_scale[I8_SELF];
   extern __shared__ __attribute__((aligned(16))) unsigned char s_q[];   // SELF: (M, kp)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -304,25 +380,20 @@ __global__ __launch_bounds__(256) void int8_few_kernel(const Int8Args g, const v
   if constexpr (SELF) {
     for (int m = 0; m < g.M; ++m) {
       const void* row = reinterpret_cast<const unsigned char*>(x) + m * ldx * (X_BF16 ? 2 : 4);
-      float amax = 0.f;
-      bool bad = false;
+      unsigned top = 0;
       for (int k = tid * 8; k < g.K; k += 2048) {
         float v[8];
         if (x_vec) i8_load8<X_BF16, true>(row, k, g.K, v);
         else i8_load8<X_BF16, false>(row, k, g.K, v);
-        i8_amax8(v, amax, bad);
+        top = i8_amax8(v, top);
       }
-      amax = wave_max(amax);
-      bad = __ballot(bad) != 0;
+      top = dpp_wave_umax(top);
       __syncthreads();
-      if (lane == 0) {
-        s_red[wave] = amax;
-        s_bad[wave] = bad;
-      }
+      if (lane == 0) s_top[wave] = top;
       __syncthreads();
-      amax = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-      bad = (s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3]) != 0;
-      const float s = i8_scale(amax), inv = 1.0f / s;
+      top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+      const bool bad = i8_bad(top);
+      const float s = i8_scale(__uint_as_float(top)), inv = 1.0f / s;
       for (int k = tid * 8; k < kp; k += 2048) {
         float v[8];
         if (x_vec) i8_load8<X_BF16, true>(row, k, g.K, v);
@@ -337,20 +408,35 @@ __global__ __launch_bounds__(256) void int8_few_kernel(const Int8Args g, const v
   i32x4 acc[MT];
 #pragma unroll
   for (int b = 0; b < MT; ++b) acc[b] = i32x4{0, 0, 0, 0};
-  for (int s = s0; s < s1; ++s) {
-    const int k = s * 64 + kl;
-    // (weights past K meet zeros; the piece that holds column K - 1 is whole, the next ones are not read)
-    const i32x4 wf = k < g.K ? *reinterpret_cast<const i32x4*>(wrow + k) : i32x4{0, 0, 0, 0};
+  // the operands of four steps are requested together: the loop is all latency
+  constexpr int U = 4;
+  const int k_last = (g.K - 1) & ~15;
+  for (int s = s0; s < s1; s += U) {
+    i32x4 wf[U], xf[U][MT];
 #pragma unroll
-    for (int b = 0; b < MT; ++b) {
-      const int m = b * 16 + (lane & 15);
-      i32x4 xf = i32x4{0, 0, 0, 0};
-      if constexpr (SELF) {
-        if (m < g.M) xf = *reinterpret_cast<const i32x4*>(s_q + m * kp + k);
-      } else {
-        xf = *reinterpret_cast<const i32x4*>(g.q + (long)min(m, g.M - 1) * g.ldq + k);
+    for (int u = 0; u < U; ++u) {
+      // (weights past K meet zeros; the piece that holds column K - 1 is whole, the next ones are not read)
+      const int k = (s + u) * 64 + kl;
+      wf[u] = *reinterpret_cast<const i32x4*>(wrow + min(k, k_last));
+      if constexpr (!SELF) {
+#pragma unroll
+        for (int b = 0; b < MT; ++b)
+          xf[u][b] = *reinterpret_cast<const i32x4*>(g.q + (long)min(b * 16 + (lane & 15), g.M - 1) * g.ldq + min(k, kp - 16));
       }
-      acc[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf, xf, acc[b], 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (s + u) * 64 + kl;
+      if (k >= g.K || s + u >= s1) wf[u] = i32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int b = 0; b < MT; ++b) {
+        if constexpr (SELF) {
+          const int m = lane & 15;
+          xf[u][b] = i32x4{0, 0, 0, 0};
+          if (m < g.M && k < kp) xf[u][b] = *reinterpret_cast<const i32x4*>(s_q + m * kp + k);
+        }
+        acc[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], xf[u][b], acc[b], 0, 0, 0);
+      }
     }
   }
 #pragma unroll
@@ -377,7 +463,7 @@ __global__ __launch_bounds__(256) void int8_few_kernel(const Int8Args g, const v
 bool i8_self(int M, int K) { return M <= I8_SELF && K <= I8_SELF_K; }
 constexpr int I8_FEW = 64;
 
-long i8_pitch(int K) { return ((long)K + I8_BK - 1) / I8_BK * I8_BK; }
+long i8_pitch(int K) { return ((long)K + I8_ROW - 1) / I8_ROW * I8_ROW; }
 size_t i8_scale_offset(long M, int K) { return ((size_t)M * i8_pitch(K) + 255) / 256 * 256; }
 
 template <bool BF16, bool VEC>
@@ -412,18 +498,39 @@ void i8_launch_few(const Int8Args& g, const void* x, long ldx, int x_vec, hipStr
   }
 }
 
-template <bool YB>
-void i8_launch_tiles(Int8Args& g, hipStream_t st) {
-  const long big = (long)((g.M + 127) / 128) * ((g.N + 127) / 128);
-  if (big >= 256) {
-    g.tiles_m = (g.M + 127) / 128;
-    g.tiles_n = (g.N + 127) / 128;
-    hipLaunchKernelGGL((int8_tile_kernel<YB, 2, 2>), dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(256), 0, st, g);
-  } else {
-    g.tiles_m = (g.M + 63) / 64;
-    g.tiles_n = (g.N + 63) / 64;
-    hipLaunchKernelGGL((int8_tile_kernel<YB, 1, 1>), dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(256), 0, st, g);
+template <bool YB, int TM, int TN, int WM, int WN, int STAGES, int OCC>
+int i8_launch_tile(Int8Args& g, hipStream_t st) {
+  constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, LDS = STAGES * (BM + BN) * I8_BK;
+  const auto kernel = &int8_tile_kernel<YB, TM, TN, WM, WN, STAGES, OCC>;
+  if constexpr (LDS > 65536) {
+    // more dynamic LDS than 64 KB has to be asked for, once per kernel and device
+    static std::mutex lock;
+    static unsigned long long asked = 0;   // a bit for each of the first 64 devices
+    int dev = 0;
+    VQAF_REQUIRE(hipGetDevice(&dev) == hipSuccess && dev < 64, VQAF_E_LAUNCH);
+    std::lock_guard<std::mutex> hold(lock);
+    if (!(asked >> dev & 1ull)) {
+      VQAF_REQUIRE(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       LDS) == hipSuccess, VQAF_E_LAUNCH);
+      asked |= 1ull << dev;
+    }
   }
+  g.tiles_m = (g.M + BM - 1) / BM;
+  g.tiles_n = (g.N + BN - 1) / BN;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(64 * WM * WN), LDS, st, g);
+  return VQAF_OK;
+}
+
+template <bool YB>
+int i8_launch_tiles(Int8Args& g, hipStream_t st) {
+  // 256 x 256 tiles, one workgroup of eight waves per CU, once they nearly fill the chip (12608 x 768 x 2304: 450 tiles,
+  // 38 us against 43 us on 128 x 128; 2048 x 4096 x 4096: 128 tiles, 52 against 44 us); 128 x 128 tiles, two
+  // workgroups per CU, down to one for each CU (1920 x 768 x 2304: 270 tiles, 4 us faster than 64 x 64); then 64 x 64 in
+  // a ring twice as deep, where few workgroups have to hide the latency by themselves.
+  const long t256 = (long)((g.M + 255) / 256) * ((g.N + 255) / 256), t128 = (long)((g.M + 127) / 128) * ((g.N + 127) / 128);
+  if (t256 >= 144) return i8_launch_tile<YB, 4, 2, 2, 4, 4, 2>(g, st);
+  if (t128 >= 256) return i8_launch_tile<YB, 2, 2, 2, 2, 4, 2>(g, st);
+  return i8_launch_tile<YB, 1, 1, 2, 2, 8, 2>(g, st);
 }
 
 }  // namespace
@@ -485,7 +592,8 @@ extern "C" int vqaf_int8_linear(const void* x, long ldx, int x_dtype, const int8
     yb ? i8_launch_few<true, true, false>(g, x, ldx, 0, st) : i8_launch_few<true, false, false>(g, x, ldx, 0, st);
   } else {
     VQAF_REQUIRE(vqaf_internal_zero_block(&g.zeros) == VQAF_OK, VQAF_E_LAUNCH);
-    yb ? i8_launch_tiles<true>(g, st) : i8_launch_tiles<false>(g, st);
+    const int rc = yb ? i8_launch_tiles<true>(g, st) : i8_launch_tiles<false>(g, st);
+    if (rc != VQAF_OK) return rc;
   }
   VQAF_LAUNCH_CHECK();
 }
