@@ -6,7 +6,6 @@ device memory, streams and autograd bookkeeping only; the arithmetic is in the k
 """
 from __future__ import annotations
 
-import contextlib
 import weakref
 from typing import NamedTuple, Optional, Tuple
 
@@ -827,17 +826,31 @@ class TokenLogprobs(NamedTuple):
     top_indices: Optional[torch.Tensor]
 
 
-def _raw_stream(device: torch.device) -> int:
-    """The current stream of `device` as the C ABI takes it (stream_ptr without building a stream object)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
+_raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index, without building a stream object
+_current_device = torch._C._cuda_getDevice
 
 
-def _on(device: torch.device):
-    """Makes `device` the current one for the launches inside (a launch goes to the current device, whatever its
-    stream)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _launch(device: torch.device, entry: str, *args) -> None:
+    """Calls a C entry point whose last argument is the stream, on `device`'s current stream.  A launch goes to the
+    current device whatever its stream, so another device is made current around it."""
+    lib = load()
+    index = device.index
+    if index == _current_device():
+        status = getattr(lib, entry)(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            status = getattr(lib, entry)(*args, _raw_stream(index))
+    if status != 0:
+        check(status, entry)
+
+
+def _first_order(backward):
+    """once_differentiable without its cost where nothing records gradients of gradients."""
+    recorded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def _answer_rows(logits: torch.Tensor):
@@ -846,8 +859,12 @@ def _answer_rows(logits: torch.Tensor):
         raise ValueError(f"logits need a dimension of classes, got shape {tuple(logits.shape)}")
     require_gpu(logits)
     dtype_code(logits)
+    x = logits
+    if x.dim() == 2 and x.is_contiguous():
+        return x, x.shape[1]
     C = logits.shape[-1]
-    x = logits if logits.dim() == 2 else logits.reshape(-1, C)
+    if x.dim() != 2:
+        x = x.reshape(-1, C)
     if C > 1 and x.stride(1) != 1:
         x = x.contiguous()
     return x, (x.stride(0) if x.shape[0] > 1 else C)
@@ -856,12 +873,18 @@ def _answer_rows(logits: torch.Tensor):
 def _grad_rows(x: torch.Tensor, ld: int) -> torch.Tensor:
     """An (R,C) tensor of x's dtype whose rows lie on the 16-byte grid as x's do."""
     R, C = x.shape
+    if ld == C and x.data_ptr() % 16 == 0:
+        return torch.empty((R, C), dtype=x.dtype, device=x.device)
     per = 16 // x.element_size()
     off, ldg = (x.data_ptr() // x.element_size()) % per, C + (ld - C) % per
-    if off == 0 and ldg == C:
-        return torch.empty(R, C, dtype=x.dtype, device=x.device)
     buf = torch.empty(off + R * ldg, dtype=x.dtype, device=x.device)
     return buf.as_strided((R, C), (ldg, 1), off)
+
+
+def _grad_pitch(x: torch.Tensor, ld: int) -> int:
+    """Row pitch of _grad_rows(x, ld)."""
+    C = x.shape[1]
+    return C if ld == C else C + (ld - C) % (16 // x.element_size())
 
 
 def _temperature(t: float) -> float:
@@ -872,23 +895,28 @@ def _temperature(t: float) -> float:
 
 
 def _f32(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if g is None else g.to(torch.float32).contiguous()
+    if g is None or (g.dtype is torch.float32 and g.is_contiguous()):
+        return g
+    return g.to(torch.float32).contiguous()
+
+
+def _addr(t: Optional[torch.Tensor]) -> Optional[int]:
+    """Address of a tensor made or checked here (None passes NULL)."""
+    return None if t is None else t.data_ptr()
 
 
 def _logprobs_forward(x, ld, targets, top, temperature, entropy, stats):
     """One launch; (logprobs, entropy, top_logprobs, top_indices, stats), None where not asked for."""
     R, C = x.shape
-    dev = x.device
+    dev, f32 = x.device, torch.float32
     T = 0 if targets is None else targets.shape[1]
-    lp = torch.empty(R, T, dtype=torch.float32, device=dev) if targets is not None else None
-    ent = torch.empty(R, dtype=torch.float32, device=dev) if entropy else None
-    tl = torch.empty(R, top, dtype=torch.float32, device=dev) if top else None
-    ti = torch.empty(R, top, dtype=torch.int64, device=dev) if top else None
-    st = torch.empty(R, 2, dtype=torch.float32, device=dev) if stats else None
-    with _on(dev):
-        check(load().vqaf_token_logprobs(x.data_ptr(), ld, ptr(targets), R, C, T, top, dtype_code(x), temperature,
-                                         ptr(lp), ptr(ent), ptr(tl), ptr(ti), ptr(st), _raw_stream(dev)),
-              "vqaf_token_logprobs")
+    lp = None if targets is None else torch.empty((R, T), dtype=f32, device=dev)
+    ent = torch.empty(R, dtype=f32, device=dev) if entropy else None
+    tl = torch.empty((R, top), dtype=f32, device=dev) if top else None
+    ti = torch.empty((R, top), dtype=torch.int64, device=dev) if top else None
+    st = torch.empty((R, 2), dtype=f32, device=dev) if stats else None
+    _launch(dev, "vqaf_token_logprobs", x.data_ptr(), ld, _addr(targets), R, C, T, top, dtype_code(x), temperature,
+            _addr(lp), _addr(ent), _addr(tl), _addr(ti), _addr(st))
     return lp, ent, tl, ti, st
 
 
@@ -904,21 +932,19 @@ class _TokenLogprobs(torch.autograd.Function):
         return lp, ent, tl, ti
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, g_lp, g_ent, g_top, _g_idx):
         x, targets, ti, st, ent = ctx.saved_tensors
         ld, T, top, temperature = ctx.meta
         if g_lp is None and g_ent is None and g_top is None:
-            return (None,) * 6
+            return None, None, None, None, None, None
         R, C = x.shape
         g_lp, g_ent, g_top = _f32(g_lp), _f32(g_ent), _f32(g_top)
         grad = _grad_rows(x, ld)
-        with _on(x.device):
-            check(load().vqaf_token_logprobs_bwd(x.data_ptr(), ld, ptr(targets), ptr(ti), R, C, T, top, dtype_code(x),
-                                                 temperature, ptr(st), ptr(ent), ptr(g_lp), ptr(g_ent), ptr(g_top),
-                                                 grad.data_ptr(), grad.stride(0), _raw_stream(x.device)),
-                  "vqaf_token_logprobs_bwd")
-        return (grad,) + (None,) * 5
+        _launch(x.device, "vqaf_token_logprobs_bwd", x.data_ptr(), ld, _addr(targets), _addr(ti), R, C, T, top,
+                dtype_code(x), temperature, st.data_ptr(), _addr(ent), _addr(g_lp), _addr(g_ent), _addr(g_top),
+                grad.data_ptr(), _grad_pitch(x, ld))
+        return grad, None, None, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0, temperature: float = 1.0,
@@ -950,7 +976,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
         T = 1 if given == lead else given[-1]
         if T > ANSWERS_MAX:
             raise ValueError(f"at most {ANSWERS_MAX} targets for each row, got {T}")
-        tg = targets.to(torch.int64).reshape(R, T).contiguous()
+        tg = targets.to(torch.int64).contiguous().view(R, T)
     if R == 0:
         z = x.sum(1, dtype=torch.float32)
         lp = None if tg is None else (z[:, None].expand(0, tg.shape[1]) * 1.0)
@@ -972,15 +998,13 @@ def _distill_forward(x, ld, teacher, indices, temperature, tail, scale, needs):
     R, C = x.shape
     dev = x.device
     rows = torch.empty(R, dtype=torch.float32, device=dev)
-    stats = torch.empty(R, 5, dtype=torch.float64, device=dev) if needs else None
+    stats = torch.empty((R, 5), dtype=torch.float64, device=dev) if needs else None
     whole = scale is not None
     grad = _grad_rows(x, ld) if needs and whole else None
     loss = torch.empty((), dtype=torch.float32, device=dev) if whole else None
-    with _on(dev):
-        check(load().vqaf_distill(x.data_ptr(), ld, teacher.data_ptr(), indices.data_ptr(), R, C, teacher.shape[1],
-                                  dtype_code(x), temperature, tail, rows.data_ptr(), ptr(stats),
-                                  None if grad is None else grad.data_ptr(), 0 if grad is None else grad.stride(0),
-                                  scale if whole else 1.0, ptr(loss), _raw_stream(dev)), "vqaf_distill")
+    _launch(dev, "vqaf_distill", x.data_ptr(), ld, teacher.data_ptr(), indices.data_ptr(), R, C, teacher.shape[1],
+            dtype_code(x), temperature, tail, rows.data_ptr(), _addr(stats), _addr(grad),
+            0 if grad is None else _grad_pitch(x, ld), scale if whole else 1.0, _addr(loss))
     return (loss if whole else rows), stats, grad
 
 
@@ -995,7 +1019,7 @@ class _Distill(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, up):
         grad, ctx.unit = ctx.unit, None   # handed out once: a second backward forms its own
         ready = grad is not None
@@ -1005,12 +1029,9 @@ class _Distill(torch.autograd.Function):
             if not ready:
                 grad = _grad_rows(x, ld)
             up = _f32(up)
-            with _on(x.device):
-                check(load().vqaf_distill_bwd(x.data_ptr(), ld, teacher.data_ptr(), indices.data_ptr(), x.shape[0],
-                                              x.shape[1], teacher.shape[1], dtype_code(x), temperature, stats.data_ptr(),
-                                              up.data_ptr(), int(scale is None), int(ready),
-                                              1.0 if scale is None else scale, grad.data_ptr(), grad.stride(0),
-                                              _raw_stream(x.device)), "vqaf_distill_bwd")
+            _launch(x.device, "vqaf_distill_bwd", x.data_ptr(), ld, teacher.data_ptr(), indices.data_ptr(), x.shape[0],
+                    x.shape[1], teacher.shape[1], dtype_code(x), temperature, stats.data_ptr(), up.data_ptr(),
+                    int(scale is None), int(ready), 1.0 if scale is None else scale, grad.data_ptr(), _grad_pitch(x, ld))
         return grad, None, None, None, None, None, None
 
 
@@ -1047,8 +1068,11 @@ def distill_loss(logits: torch.Tensor, teacher: torch.Tensor, indices: torch.Ten
     if R == 0:
         rows = x.sum(1, dtype=torch.float32)
         return rows.view(lead) if reduction == "none" else rows.sum() if reduction == "sum" else rows.mean()
-    v = teacher.detach().to(torch.float32).reshape(R, K).contiguous()
-    idx = indices.to(torch.int64).reshape(R, K).contiguous()
+    v = _f32(teacher.detach())
+    idx = indices if indices.dtype is torch.int64 else indices.to(torch.int64)
+    if len(lead) != 1:
+        v, idx = v.reshape(R, K), idx.reshape(R, K)
+    idx = idx.contiguous()
     scale = 1.0 / R if reduction == "mean" else 1.0 if reduction == "sum" else None
     if x.requires_grad and torch.is_grad_enabled():
         out = _Distill.apply(x, ld, v, idx, temperature, int(bool(tail)), scale)
@@ -1196,9 +1220,8 @@ def quantize_rows(x: torch.Tensor):
     q = torch.empty(M, pitch, dtype=torch.int8, device=x.device)
     scale = torch.empty(M, dtype=torch.float32, device=x.device)
     if M:
-        with _on(x.device):
-            check(load().vqaf_quantize_rows(x2.data_ptr(), ld, M, K, dtype_code(x2), q.data_ptr(), pitch, ptr(scale),
-                                            _raw_stream(x.device)), "vqaf_quantize_rows")
+        _launch(x.device, "vqaf_quantize_rows", x2.data_ptr(), ld, M, K, dtype_code(x2), q.data_ptr(), pitch,
+                scale.data_ptr())
     lead = x.shape[:-1]
     return (q[:, :K] if len(lead) == 1 else q.view(*lead, pitch)[..., :K]), scale.view(lead)
 
@@ -1247,14 +1270,11 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         weight, ldw = whole, whole.shape[1]
     y = torch.empty(M, N, dtype=dt, device=x.device)
     if M:
-        lib = load()
-        need = lib.vqaf_int8_linear_workspace_bytes(M, K)
+        need = load().vqaf_int8_linear_workspace_bytes(M, K)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        with _on(x.device):
-            check(lib.vqaf_int8_linear(x2.data_ptr(), ld, dtype_code(x2), weight.data_ptr(), ldw,
-                                       ptr(weight_scale.contiguous()), ptr(bias),
-                                       dtype_code(bias) if bias is not None else 0, M, N, K, y.data_ptr(), N, code, ptr(ws),
-                                       need, _raw_stream(x.device)), "vqaf_int8_linear")
+        _launch(x.device, "vqaf_int8_linear", x2.data_ptr(), ld, dtype_code(x2), weight.data_ptr(), ldw,
+                weight_scale.contiguous().data_ptr(), _addr(bias), dtype_code(bias) if bias is not None else 0, M, N, K,
+                y.data_ptr(), N, code, _addr(ws), need)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
