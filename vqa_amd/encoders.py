@@ -253,7 +253,64 @@ def _affine(x, w, b):
     return F.linear(x, w, b)
 
 
+class Int8Linear(nn.Module):
+    """A Linear layer (or several with one input, their outputs side by side) held in eight-bit integers with a scale for
+    each output channel, for scoring: the tokens are quantised row by row on the way in (ops.int8_linear).  It has no
+    gradient.  Made by `quantize_int8`; `dtype` is that of the parameters it was made from, and follows `.to()`; the
+    scales stay f32."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, dtype=torch.float32, device=None):
+        super().__init__()
+        self.in_features, self.out_features = in_features, out_features
+        pitch = (in_features + 127) // 128 * 128   # rows of whole 128-byte pieces, as ops.quantize_rows lays them out
+        self.register_buffer("weight_q", torch.zeros(out_features, pitch, dtype=torch.int8, device=device))
+        self.register_buffer("weight_scale", torch.ones(out_features, dtype=torch.float32, device=device))
+        self.register_buffer("bias", torch.zeros(out_features, dtype=dtype, device=device) if bias else None)
+        self.register_buffer("_like", torch.empty(0, dtype=dtype, device=device), persistent=False)
+
+    @classmethod
+    @torch.no_grad()
+    def from_linear(cls, *layers: nn.Linear) -> "Int8Linear":
+        from . import ops
+        w = torch.cat([lin.weight.detach() for lin in layers], 0)
+        if len({lin.bias is None for lin in layers}) != 1:
+            raise ValueError("layers with and without bias cannot be held side by side")
+        bias = layers[0].bias is not None
+        m = cls(w.shape[1], w.shape[0], bias, w.dtype, w.device)
+        q, scale = ops.quantize_rows(w if w.dtype in (torch.float32, torch.bfloat16) else w.float())
+        m.weight_q[:, :w.shape[1]] = q
+        m.weight_scale.copy_(scale)
+        if bias:
+            m.bias.copy_(torch.cat([lin.bias.detach() for lin in layers], 0))
+        m.train(layers[0].training)
+        return m
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self._like.dtype
+
+    def _apply(self, fn, recurse=True):
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != torch.float32:   # a change of type is for the parameters it stands in for
+            self.weight_scale = scale.to(self.weight_q.device)
+        return self
+
+    def forward(self, x):
+        from . import ops
+        return ops.int8_linear(x, self.weight_q[:, :self.in_features], self.weight_scale, self.bias)
+
+    def extra_repr(self):
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+def _dtype_of(lin) -> torch.dtype:
+    return lin.dtype if isinstance(lin, Int8Linear) else lin.weight.dtype
+
+
 def _linear(x: torch.Tensor, lin: nn.Linear) -> torch.Tensor:
+    if isinstance(lin, Int8Linear):
+        return lin(x)
     w, b = lin.weight, lin.bias
     if w.dtype != x.dtype:
         w = w.to(x.dtype)
@@ -268,6 +325,11 @@ def _packed_qkv(x, q: nn.Linear, k: nn.Linear, v: nn.Linear) -> torch.Tensor:
     if w.dtype != x.dtype:
         w, b = w.to(x.dtype), b.to(x.dtype)
     return _affine(x, w, b)
+
+
+def _qkv_of(x, att) -> torch.Tensor:
+    """The packed projections of an attention block, whose three layers `quantize_int8` holds side by side."""
+    return att.packed(x) if att.packed is not None else _packed_qkv(x, att.query, att.key, att.value)
 
 
 # --------------------------------------------------------------------------------------------------
@@ -401,6 +463,7 @@ class _ViTSelfAttention(nn.Module):
     def __init__(self, E):
         super().__init__()
         self.query, self.key, self.value = nn.Linear(E, E), nn.Linear(E, E), nn.Linear(E, E)
+        self.packed = None  # an Int8Linear of all three once quantize_int8() has taken their place
 
 
 class _Dense(nn.Module):
@@ -432,7 +495,7 @@ class _ViTLayer(nn.Module):
         """y = layernorm_before(s) of this layer; returns (layernorm of the NEXT consumer's input, stream)
         as a pair so that every residual add runs inside the LayerNorm kernel that follows it."""
         a = self.attention.attention
-        ctx = self_attention(_packed_qkv(y, a.query, a.key, a.value), None, self.heads,
+        ctx = self_attention(_qkv_of(y, a), None, self.heads,
                              self.p_attn if self.training else 0.0, rng)
         att = F.dropout(_linear(ctx, self.attention.output.dense), self.p, self.training)
         y2, s2 = add_layer_norm(att, s, self.layernorm_after.weight, self.layernorm_after.bias, self.eps)
@@ -560,6 +623,7 @@ class _BertSelfAttention(nn.Module):
     def __init__(self, E):
         super().__init__()
         self.query, self.key, self.value = nn.Linear(E, E), nn.Linear(E, E), nn.Linear(E, E)
+        self.packed = None  # an Int8Linear of all three once quantize_int8() has taken their place
 
 
 class _BertSelfOutput(nn.Module):
@@ -630,7 +694,7 @@ class _BertLayer(nn.Module):
 
     def forward(self, x, key_bias, rng=None):
         a = self.attention.self
-        qkv = _packed_qkv(x, a.query, a.key, a.value)
+        qkv = _qkv_of(x, a)
         if self.lora is not None:
             qkv = qkv + self.lora(x, self.training)
         ctx = self_attention(qkv, key_bias, self.heads,
@@ -668,6 +732,39 @@ class BertModel(nn.Module):
         for lyr in self.encoder.layer:
             x = lyr(x, key_bias, rng)
         return x, self.pooler(x)
+
+
+# --------------------------------------------------------------------------------------------------
+# eight-bit scoring
+# --------------------------------------------------------------------------------------------------
+@torch.no_grad()
+def quantize_int8(module: nn.Module) -> nn.Module:
+    """Puts the Linear layers under `module` (an encoder, or a whole VQAModel) into eight-bit integers for scoring, in
+    place: every nn.Linear becomes an `Int8Linear`, the three projections of an attention block one of them.  Left as
+    they are: LoRA adapters, the attention modules of the fusion (their weights score tokens and keep indices) and patch
+    embeddings.  The module has to be on the GPU and in eval mode; afterwards it runs under torch.no_grad() only.  A
+    classifier wrapped for DP-SGD is refused."""
+    from .dp import GradSampleModule
+    if isinstance(module, nn.Linear):
+        raise TypeError("quantize_int8 changes the layers of a module in place; for one layer use Int8Linear.from_linear")
+    if module.training:
+        raise RuntimeError("quantize_int8 is for scoring: call eval() first")
+    if any(isinstance(m, GradSampleModule) for m in module.modules()):
+        raise RuntimeError("a module wrapped for DP-SGD cannot be held in eight bits")
+
+    def visit(m):
+        if isinstance(m, (_QkvLora, nn.MultiheadAttention)):
+            return
+        if isinstance(m, (_ViTSelfAttention, _BertSelfAttention)) and m.packed is None:
+            m.packed = Int8Linear.from_linear(m.query, m.key, m.value)
+            m.query = m.key = m.value = None
+        for name, child in list(m.named_children()):
+            if type(child) is nn.Linear:
+                setattr(m, name, Int8Linear.from_linear(child))
+            else:
+                visit(child)
+    visit(module)
+    return module
 
 
 # --------------------------------------------------------------------------------------------------
@@ -735,7 +832,7 @@ class ViT(nn.Module):
 
     def forward(self, images):
         h, pooled = self.vit(images)
-        dt = self.seq_projection.weight.dtype  # the stack computes in bf16; results leave in the parameters' dtype
+        dt = _dtype_of(self.seq_projection)  # the stack computes in bf16; results leave in the parameters' dtype
         return _linear(h, self.seq_projection).to(dt), _linear(pooled, self.global_projection).to(dt)
 
 
@@ -759,7 +856,7 @@ class Bert(nn.Module):
 
     def forward(self, input_ids, attention_mask):
         h, pooled = self.bert(input_ids, attention_mask)
-        dt = self.seq_projection.weight.dtype
+        dt = _dtype_of(self.seq_projection)
         return _linear(h, self.seq_projection).to(dt), _linear(pooled, self.global_projection).to(dt)
 
 

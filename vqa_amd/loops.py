@@ -36,6 +36,33 @@ def _main_reducer(optimizer) -> "vdist.GradReducer | None":
     return red if red.world() > 1 else None
 
 
+def _zero_grad(optimizer) -> None:
+    for opt in (optimizer['main'], optimizer['classifier']) if isinstance(optimizer, dict) else (optimizer,):
+        opt.zero_grad()
+
+
+def _step(optimizer, reducer, batch: int) -> None:
+    if reducer is not None:   # replicas: the mean over the ranks' joint batch, as one process would see it
+        reducer.reduce(batch)
+    for opt in (optimizer['main'], optimizer['classifier']) if isinstance(optimizer, dict) else (optimizer,):
+        opt.step()
+
+
+def _empty_batch(optimizer, main_opt, reducer, device) -> None:
+    """The step of a rank whose Poisson-sampled batch is empty: the other ranks are waiting in the collectives, in this
+    order: non-private gradients, then the classifier's clipped sums.  This rank contributes zeros to the first and takes
+    the same averaged step as everyone else; Opacus still takes (and accounts for) the noise-only step of the private
+    part."""
+    if reducer is not None:
+        main_opt.zero_grad()
+        reducer.reduce(0)
+        main_opt.step()
+    if isinstance(optimizer, dict) and hasattr(optimizer['classifier'], 'empty_step'):
+        optimizer['classifier'].empty_step(device)
+    elif hasattr(optimizer, 'empty_step'):
+        optimizer.empty_step(device)
+
+
 def train(model: nn.Module, train_loader, optimizer, criterion, device, model_type: str = "VQAModel",
           use_dp_sgd: bool = False, lambda_ib: float = 0.01, capture: bool = False, pad_to: int = 0
           ) -> Tuple[float, float]:
@@ -66,18 +93,7 @@ def train(model: nn.Module, train_loader, optimizer, criterion, device, model_ty
     n = 0
     for batch in train_loader:
         if batch is None:  # an empty Poisson-sampled batch
-            # the other ranks are waiting in the collectives, in this order: non-private gradients,
-            # then the classifier's clipped sums.  This rank contributes zeros to the first and takes
-            # the same averaged step as everyone else; Opacus still takes (and accounts for) the
-            # noise-only step of the private part.
-            if reducer is not None:
-                main_opt.zero_grad()
-                reducer.reduce(0)
-                main_opt.step()
-            if split and hasattr(optimizer['classifier'], 'empty_step'):
-                optimizer['classifier'].empty_step(device)
-            elif hasattr(optimizer, 'empty_step'):
-                optimizer.empty_step(device)
+            _empty_batch(optimizer, main_opt, reducer, device)
             continue
         images, ids, mask, answers = _batch(batch, device)
         if graphed is not None:
@@ -87,28 +103,61 @@ def train(model: nn.Module, train_loader, optimizer, criterion, device, model_ty
             tot_correct += (outputs.detach().argmax(dim=1) == answers).sum()
             n += b
             continue
-        if split:                                   # utils/src.py:66-70
-            optimizer['main'].zero_grad()
-            optimizer['classifier'].zero_grad()
-        else:
-            optimizer.zero_grad()
+        _zero_grad(optimizer)                       # utils/src.py:66-70
         outputs = model(images=images, input_ids=ids, attention_mask=mask)   # :91-95
         loss = criterion(outputs, answers)                                   # :96
         loss.backward(gradient=ops.unit_gradient(loss))                      # :99 (the same unit gradient, cached)
         b = images.size(0)
-        if reducer is not None:   # replicas: the mean over the ranks' joint batch, as one process would see it
-            reducer.reduce(b)
-        if split:                                                            # :102-106
-            optimizer['main'].step()
-            optimizer['classifier'].step()
-        else:
-            optimizer.step()
+        _step(optimizer, reducer, b)                                         # :102-106
         tot_loss += loss.detach().double() * b                              # :109 without .item()
         tot_correct += (outputs.detach().argmax(dim=1) == answers).sum()    # :110
         n += b
     if n == 0:
         return 0.0, 0.0
     return float(tot_loss.item() / n), float(tot_correct.item() / n * 100.0)
+
+
+def distill(model: nn.Module, teacher: nn.Module, train_loader, optimizer, device, top: int = 16, temperature: float = 2.0,
+            tail: bool = False, hard_weight: float = 0.0) -> Tuple[float, float]:
+    """One epoch of `model` on the answers of `teacher` instead of labels, with train()'s call order and optimizers (a
+    torch optimizer, a DPOptimizer or the dict of both): the teacher's `top` answers at `temperature`
+    (ops.token_logprobs) are the targets of ops.distill_loss.  A student that has seen only another model's answers is the
+    usual alternative to DP-SGD against the attacks that vqa_amd.mia scores.  hard_weight > 0 mixes the labels' mean
+    cross-entropy in: (1 - hard_weight) * distillation + hard_weight * cross-entropy.  The teacher runs in eval mode
+    without gradients; held in eight bits (encoders.quantize_int8) it labels faster.  Returns (average loss, agreement of
+    the best answers in %)."""
+    if not 0.0 <= hard_weight < 1.0:
+        raise ValueError(f"hard_weight has to be in [0, 1), got {hard_weight}")
+    model.train()
+    teacher.eval()
+    main_opt = optimizer['main'] if isinstance(optimizer, dict) else optimizer
+    reducer = _main_reducer(main_opt)
+    tot_loss = torch.zeros((), dtype=torch.float64, device=device)
+    tot_agree = torch.zeros((), dtype=torch.int64, device=device)
+    n = 0
+    for batch in train_loader:
+        if batch is None:  # an empty Poisson-sampled batch
+            _empty_batch(optimizer, main_opt, reducer, device)
+            continue
+        images, ids, mask, answers = _batch(batch, device)
+        with torch.no_grad():
+            said = teacher(images=images, input_ids=ids, attention_mask=mask)
+            said = said[0] if isinstance(said, tuple) else said
+            label = ops.token_logprobs(said, top=min(top, said.shape[-1]), temperature=temperature, entropy=False)
+        _zero_grad(optimizer)
+        outputs = model(images=images, input_ids=ids, attention_mask=mask)
+        loss = ops.distill_loss(outputs, label.top_logprobs, label.top_indices, temperature=temperature, tail=tail)
+        if hard_weight > 0.0:
+            loss = (1.0 - hard_weight) * loss + hard_weight * ops.cross_entropy_mean(outputs, answers)
+        loss.backward(gradient=ops.unit_gradient(loss))
+        b = images.size(0)
+        _step(optimizer, reducer, b)
+        tot_loss += loss.detach().double() * b
+        tot_agree += (outputs.detach().argmax(dim=1) == label.top_indices[:, 0]).sum()
+        n += b
+    if n == 0:
+        return 0.0, 0.0
+    return float(tot_loss.item() / n), float(tot_agree.item() / n * 100.0)
 
 
 class _MaskedMeanCE(torch.autograd.Function):

@@ -22,6 +22,13 @@ def score_logits(logits: torch.Tensor, targets: Optional[torch.Tensor] = None):
     return loss, conf, pred
 
 
+@torch.no_grad()
+def score_answers(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0, temperature: float = 1.0):
+    """Log probabilities of the given answers, entropy of the answer distribution and its `top` alternatives
+    (ops.TokenLogprobs) from one read of the logits: what the loss and the confidence leave out."""
+    return ops.token_logprobs(logits, targets, top=top, temperature=temperature)
+
+
 def _forward(model, batch, device):
     images = batch['image'].to(device)
     inputs = batch['inputs']
@@ -72,3 +79,20 @@ def evaluate_privacy_confidence(model, dataloader, device, threshold=0.6, is_mem
     return {'confidences': conf,
             'ground_truth': np.full(conf.shape, 1 if is_member else 0),
             'predictions': conf >= threshold}
+
+
+@torch.no_grad()
+def evaluate_privacy_entropy(model, dataloader, device, threshold=0.5, is_member=True,
+                             model_type="VQAModel") -> Dict[str, np.ndarray]:
+    """The third score of the threshold attacks, beside the loss and the confidence (attack/metric_src.py:318-426 has
+    those two): entropy of the answer distribution <= threshold predicts "member" (a model is surer of what it was
+    trained on, whether right or not, and no label is needed)."""
+    model.eval()
+    chunks = []
+    for batch in dataloader:
+        logits, _ = _forward(model, batch, device)
+        chunks.append(score_answers(logits).entropy)
+    entropy = _gather(torch.cat(chunks)).cpu().numpy()
+    return {'entropies': entropy,
+            'ground_truth': np.full(entropy.shape, 1 if is_member else 0),
+            'predictions': entropy <= threshold}
