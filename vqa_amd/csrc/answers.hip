@@ -168,7 +168,7 @@ __global__ __launch_bounds__(NT, W) void logprob_block_kernel(const LogprobArgs 
   constexpr int V = Piece<BF16>::V, NW = NT / 64;
   __shared__ TopShared<NT> sh;
   __shared__ float s_max[NW];
-  __shared__ double s_sum[2][NW];
+  __shared__ double s_sum[2][NW], s_log;
   const long r = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   RowPieces<BF16, NT, E> row;
@@ -193,15 +193,15 @@ __global__ __launch_bounds__(NT, W) void logprob_block_kernel(const LogprobArgs 
   double S = 0.0, Wt = 0.0;
   const float hi = a.temp.hi;
   row.walk([&](const float (&v)[V], int, int) {
-    float e[V], w[V];
+    float e[V], w = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float t = (v[j] - m) * hi;
       e[j] = an_exp2(t);
-      w[j] = e[j] * an_floor(t);
+      w = fmaf(e[j], an_floor(t), w);
     }
     S += (double)an_tree<V>(e);
-    Wt += (double)an_tree<V>(w);
+    Wt += (double)w;
   });
   S = dpp_wave_sum(S);
   Wt = dpp_wave_sum(Wt);
@@ -223,22 +223,25 @@ __global__ __launch_bounds__(NT, W) void logprob_block_kernel(const LogprobArgs 
   }
   const bool empty = m == -INFINITY;
   const bool broken = !empty && !(S == S);   // a NaN or +inf in the row
-  const double mean_t = AN_LN2 * (Wt / S);
-  const double log_s = empty ? -INFINITY : log(S) - a.temp.delta * mean_t;
   const void* xr = an_row<BF16>(a.x, a.ld, r);
-  if (tid == 0) {
-    if (a.entropy != nullptr) a.entropy[r] = empty ? 0.f : (float)(log_s - mean_t * (1.0 - a.temp.delta));
-    if (a.stats != nullptr) {
-      a.stats[2 * r] = m;
-      a.stats[2 * r + 1] = empty ? 1.f : (float)(S * (1.0 - a.temp.delta * mean_t));
+  if (wave == 0) {   // the row's results; the other waves only need log S, and only for the alternatives
+    const double mean_t = AN_LN2 * (Wt / S);
+    const double log_s = empty ? -INFINITY : log(S) - a.temp.delta * mean_t;
+    if (lane == 0) {
+      s_log = log_s;
+      if (a.entropy != nullptr) a.entropy[r] = empty ? 0.f : (float)(log_s - mean_t * (1.0 - a.temp.delta));
+      if (a.stats != nullptr) {
+        a.stats[2 * r] = m;
+        a.stats[2 * r + 1] = empty ? 1.f : (float)(S * (1.0 - a.temp.delta * mean_t));
+      }
     }
-  }
-  for (int i = tid; i < a.T; i += NT) {
-    const int64_t t = a.targets[r * a.T + i];
-    float lp = 0.f;                                         // a negative target is none
-    if (t >= a.C) lp = NAN;
-    else if (t >= 0) lp = an_logprob(an_at<BF16>(xr, t), m, log_s, a.temp.inv_t);
-    a.logprobs[r * a.T + i] = lp;
+    for (int i = lane; i < a.T; i += 64) {
+      const int64_t t = a.targets[r * a.T + i];
+      float lp = 0.f;                                         // a negative target is none
+      if (t >= a.C) lp = NAN;
+      else if (t >= 0) lp = an_logprob(an_at<BF16>(xr, t), m, log_s, a.temp.inv_t);
+      a.logprobs[r * a.T + i] = lp;
+    }
   }
   if (a.K == 0) return;
 
@@ -265,6 +268,7 @@ __global__ __launch_bounds__(NT, W) void logprob_block_kernel(const LogprobArgs 
   const int n = sh.n;
   if (tid < 16) sh.cand[n + tid] = 0;   // below every candidate
   __syncthreads();
+  const double log_s = s_log;
   for (int i = tid; i < n; i += NT) {
     const u64 mine = sh.cand[i];
     const int k = an_rank(sh.cand, n, mine);

@@ -166,9 +166,9 @@ template <int NT>
 struct DistillShared {
   DistillList list;
   float s_max[NT / 64];
-  double s_sum[NT / 64];
-  int bad, repeats;
-  DistillStat st;
+  double s_sum[2][NT / 64];
+  int bad, repeats, none;
+  float mass, slope;   // over S, the slope times the gradient's scale
 };
 
 // The elements of a piece whose bits are set become -inf.
@@ -231,8 +231,21 @@ __global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs 
   for (int i = 1; i < NW; ++i) m = fmaxf(m, sh.s_max[i]);
   if (m == -INFINITY && an_block_nan<BF16, NT>(row.s)) m = NAN;
 
-  double S = 0.0;   // TAIL: over the classes outside the list
-  const float hi = a.temp.hi, lo = a.temp.lo;
+  // Sums of e = 2^t and of e t; TAIL: over the classes outside the list.  One factor only: what its rounding shifts is taken
+  // out of the sum below, to first order.
+  double S = 0.0, Wt = 0.0;
+  const float hi = a.temp.hi;
+  const auto add = [&](float (&e)[V]) {
+    float w = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float t = (e[j] - m) * hi;
+      e[j] = an_exp2(t);
+      w = fmaf(e[j], an_floor(t), w);
+    }
+    S += (double)an_tree<V>(e);
+    Wt += (double)w;
+  };
   const auto marks = [&](int c) { return c < row.s.pieces ? s_mark[(c * V) >> 5] >> ((c * V) & 31) : 0u; };
   float held[HOLD ? E : 1][V];
   int at = tid;
@@ -250,9 +263,7 @@ __global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs 
     for (int i = 0; i < E; ++i) {
       float e[V];
       an_unpack<BF16>(row.raw[i], e);
-#pragma unroll
-      for (int j = 0; j < V; ++j) e[j] = an_exp2(an_arg(e[j], m, hi, lo));
-      S += (double)an_tree<V>(e);
+      add(e);
       if constexpr (HOLD) {
 #pragma unroll
         for (int j = 0; j < V; ++j) held[i][j] = e[j];
@@ -263,33 +274,40 @@ __global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs 
     row.walk_raw([&](const u32x4 p, int c, int) {
       float e[V];
       an_unpack<BF16>(TAIL ? an_drop<BF16>(p, marks(c)) : p, e);
-#pragma unroll
-      for (int j = 0; j < V; ++j) e[j] = an_exp2(an_arg(e[j], m, hi, lo));
-      S += (double)an_tree<V>(e);
+      add(e);
     });
   }
   S = dpp_wave_sum(S);
-  if (lane == 0) sh.s_sum[wave] = S;
+  Wt = dpp_wave_sum(Wt);
+  if (lane == 0) {
+    sh.s_sum[0][wave] = S;
+    sh.s_sum[1][wave] = Wt;
+  }
   __syncthreads();
   if (wave == 0) {
-    S = 0.0;
+    S = Wt = 0.0;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) S += sh.s_sum[i];
+    for (int i = 0; i < NW; ++i) {
+      S += sh.s_sum[0][i];
+      Wt += sh.s_sum[1][i];
+    }
+    S -= a.temp.delta * AN_LN2 * Wt;
     double loss;
     // (more than 1024 classes and at most 128 answers: never all of them)
     const DistillStat st = an_distill_row(sh.list, a.K, sh.bad != 0, m, S, S, false, TAIL, a.temp.inv_t, loss);
     if (lane == 0) {
-      sh.st = st;
       a.row_loss[r] = (float)(a.t2 * loss);
       if (a.stats != nullptr) a.stats[r] = st;
+      sh.none = an_no_gradient(st) ? 1 : 0;
+      const double inv = sh.none ? 0.0 : 1.0 / st.S;
+      sh.mass = (float)(st.mass * inv);
+      sh.slope = (float)(st.slope * inv) * a.scale;
     }
   }
   if (a.grad == nullptr) return;   // uniform
   __syncthreads();
-  const DistillStat st = sh.st;
-  const bool none = an_no_gradient(st);
-  const double inv = none ? 0.0 : 1.0 / st.S;
-  const float mass = (float)(st.mass * inv), slope = (float)(st.slope * inv) * a.scale;
+  const bool none = sh.none != 0;
+  const float mass = sh.mass, slope = sh.slope;
   unsigned char* grow = reinterpret_cast<unsigned char*>(a.grad) + r * a.ldg * (BF16 ? 2 : 4);
   asm volatile("" : "+v"(at));
   if constexpr (HOLD) {
@@ -309,14 +327,14 @@ __global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs 
       if (here >= row.s.pieces) return;
       float g[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) g[j] = none ? 0.f : an_exp2(an_arg(v[j], m, hi, lo)) * slope;
+      for (int j = 0; j < V; ++j) g[j] = none ? 0.f : an_exp2((v[j] - m) * hi) * slope;
       an_store<BF16>(grow, here * V - row.s.shift, a.C, g);
     });
   }
   __syncthreads();
   const float sc = a.scale;
   an_write_named<BF16>(sh.list.idx, sh.list.q, a.K, sh.repeats != 0, tid, NT, 0, a.C, xr, grow,
-                       [&](float x) { return none ? 0.f : sc * (an_exp2(an_arg(x, m, hi, lo)) * mass); },
+                       [&](float x) { return none ? 0.f : sc * (an_exp2((x - m) * hi) * mass); },
                        [&](float q) { return none ? 0.f : -sc * q; });
 }
 
