@@ -920,6 +920,12 @@ def _logprobs_forward(x, ld, targets, top, temperature, entropy, stats):
     return lp, ent, tl, ti, st
 
 
+def _token_indices(t: torch.Tensor, what: str) -> torch.Tensor:
+    if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
+        raise TypeError(f"{what} are token indices, got {t.dtype}")
+    return t.to(torch.int64)
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, ld, targets, top, temperature, entropy):
@@ -969,14 +975,14 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
         given = targets.shape
         if given != lead and given[:-1] != lead:
             raise ValueError(f"targets of shape {tuple(given)} do not fit logits of shape {tuple(logits.shape)}")
-        if targets.dtype.is_floating_point or targets.dtype.is_complex or targets.dtype == torch.bool:
-            raise TypeError(f"targets are token indices, got {targets.dtype}")
+        if targets.dtype is not torch.int64:
+            targets = _token_indices(targets, "targets")
         if targets.device != logits.device:
             raise ValueError(f"targets are on {targets.device}, logits on {logits.device}")
         T = 1 if given == lead else given[-1]
         if T > ANSWERS_MAX:
             raise ValueError(f"at most {ANSWERS_MAX} targets for each row, got {T}")
-        tg = targets.to(torch.int64).contiguous().view(R, T)
+        tg = targets.contiguous().view(R, T)
     if R == 0:
         z = x.sum(1, dtype=torch.float32)
         lp = None if tg is None else (z[:, None].expand(0, tg.shape[1]) * 1.0)
@@ -997,15 +1003,20 @@ def _distill_forward(x, ld, teacher, indices, temperature, tail, scale, needs):
     backward needs them, the gradient also where there is no sum."""
     R, C = x.shape
     dev = x.device
-    rows = torch.empty(R, dtype=torch.float32, device=dev)
-    stats = torch.empty((R, 5), dtype=torch.float64, device=dev) if needs else None
-    whole = scale is not None
-    grad = _grad_rows(x, ld) if needs and whole else None
-    loss = torch.empty((), dtype=torch.float32, device=dev) if whole else None
+    if scale is None:
+        rows = torch.empty(R, dtype=torch.float32, device=dev)
+        stats = torch.empty(5 * R, dtype=torch.float64, device=dev) if needs else None
+        _launch(dev, "vqaf_distill", x.data_ptr(), ld, teacher.data_ptr(), indices.data_ptr(), R, C, teacher.shape[1],
+                dtype_code(x), temperature, tail, rows.data_ptr(), _addr(stats), None, 0, 1.0, None)
+        return rows, stats, None
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    room = torch.empty(6 * R if needs else R, dtype=torch.float64, device=dev)   # 5 R statistics, R row losses behind them
+    at = room.data_ptr()
+    grad = _grad_rows(x, ld) if needs else None
     _launch(dev, "vqaf_distill", x.data_ptr(), ld, teacher.data_ptr(), indices.data_ptr(), R, C, teacher.shape[1],
-            dtype_code(x), temperature, tail, rows.data_ptr(), _addr(stats), _addr(grad),
-            0 if grad is None else _grad_pitch(x, ld), scale if whole else 1.0, _addr(loss))
-    return (loss if whole else rows), stats, grad
+            dtype_code(x), temperature, tail, at + 40 * R if needs else at, at if needs else None, _addr(grad),
+            _grad_pitch(x, ld), scale, loss.data_ptr())
+    return loss, room, grad
 
 
 class _Distill(torch.autograd.Function):
@@ -1023,8 +1034,8 @@ class _Distill(torch.autograd.Function):
     def backward(ctx, up):
         grad, ctx.unit = ctx.unit, None   # handed out once: a second backward forms its own
         ready = grad is not None
-        x, teacher, indices, stats = ctx.saved_tensors   # (also tells of logits changed in place since)
         if not ready or up is not _unit_grads.get((up.device, up.dtype)):
+            x, teacher, indices, stats = ctx.saved_tensors   # (also tells of logits changed in place since)
             ld, temperature, scale = ctx.meta
             if not ready:
                 grad = _grad_rows(x, ld)
@@ -1051,28 +1062,26 @@ def distill_loss(logits: torch.Tensor, teacher: torch.Tensor, indices: torch.Ten
         raise ValueError(f"reduction has to be mean, sum or none, got {reduction!r}")
     x, ld = _answer_rows(logits)
     R, C = x.shape
-    lead = logits.shape[:-1]
+    shape, dev = teacher.shape, logits.device
+    lead, K = logits.shape[:-1], shape[-1] if shape else 0
     temperature = _temperature(temperature)
-    if teacher.shape != indices.shape or teacher.shape[:-1] != lead or teacher.dim() != logits.dim():
-        raise ValueError(f"teacher {tuple(teacher.shape)} and indices {tuple(indices.shape)} do not fit logits of shape "
+    if indices.shape != shape or len(shape) != len(lead) + 1 or shape[:-1] != lead:
+        raise ValueError(f"teacher {tuple(shape)} and indices {tuple(indices.shape)} do not fit logits of shape "
                          f"{tuple(logits.shape)}")
-    K = teacher.shape[-1]
     if not 1 <= K <= ANSWERS_MAX:
         raise ValueError(f"between 1 and {ANSWERS_MAX} answers for each row, got {K}")
     if not teacher.dtype.is_floating_point:
         raise TypeError(f"teacher holds log probabilities, got {teacher.dtype}")
-    if indices.dtype.is_floating_point or indices.dtype.is_complex or indices.dtype == torch.bool:
-        raise TypeError(f"indices are token indices, got {indices.dtype}")
-    if teacher.device != logits.device or indices.device != logits.device:
-        raise ValueError(f"logits are on {logits.device}, teacher on {teacher.device}, indices on {indices.device}")
+    if indices.dtype is not torch.int64:
+        indices = _token_indices(indices, "indices")
+    if teacher.device != dev or indices.device != dev:
+        raise ValueError(f"logits are on {dev}, teacher on {teacher.device}, indices on {indices.device}")
     if R == 0:
         rows = x.sum(1, dtype=torch.float32)
         return rows.view(lead) if reduction == "none" else rows.sum() if reduction == "sum" else rows.mean()
-    v = _f32(teacher.detach())
-    idx = indices if indices.dtype is torch.int64 else indices.to(torch.int64)
+    v, idx = _f32(teacher.detach() if teacher.requires_grad else teacher), indices.contiguous()
     if len(lead) != 1:
         v, idx = v.reshape(R, K), idx.reshape(R, K)
-    idx = idx.contiguous()
     scale = 1.0 / R if reduction == "mean" else 1.0 if reduction == "sum" else None
     if x.requires_grad and torch.is_grad_enabled():
         out = _Distill.apply(x, ld, v, idx, temperature, int(bool(tail)), scale)
