@@ -84,7 +84,8 @@ def test_borders_between_steps_and_the_range_s_ends(dev, dtype):
 
 SHAPES = [(1, 1, 1), (1, 768, 2304), (2, 100, 17), (4, 8192, 33), (4, 8200, 5), (5, 64, 16), (16, 130, 430), (17, 768, 48),
           (33, 200, 100), (64, 1024, 64), (64, 40, 3), (65, 768, 64), (100, 129, 65), (129, 16, 130), (300, 768, 768),
-          (257, 4096, 31), (1000, 1024, 430), (1920, 768, 512), (2500, 256, 2050), (4100, 100, 1030)]
+          (257, 4096, 31), (1000, 1024, 430), (1920, 768, 512), (2500, 256, 2050), (4100, 100, 1030),
+          (3000, 200, 3001), (9300, 64, 1001)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -165,8 +166,8 @@ def test_refusals(dev):
 
 def test_replayed_graph_and_streams(dev):
     from vqa_amd import ops
-    wq, ws = ops.quantize_rows(_x(96, 256, torch.float32, 6).to(dev))
-    xs = [[_x(M, 256, torch.bfloat16, 10 * M + i).to(dev) for i in range(3)] for M in (2, 40, 500)]
+    wq, ws = ops.quantize_rows(_x(2304, 256, torch.float32, 6).to(dev))
+    xs = [[_x(M, 256, torch.bfloat16, 10 * M + i).to(dev) for i in range(3)] for M in (2, 40, 500, 5000)]
     want = [[ops.int8_linear(x, wq, ws) for x in row] for row in xs]
     buf = [row[0].clone() for row in xs]
     torch.cuda.synchronize()

@@ -87,6 +87,70 @@ __device__ __forceinline__ u32x2 i8_quant8(const float (&v)[8], float s, float i
   return bad ? u32x2{0, 0} : r;
 }
 
+// The same eight values as they lie in memory (bf16 takes half the registers of f32).
+template <bool BF16>
+struct I8Raw {
+  u32x4 r[BF16 ? 1 : 2];
+};
+template <bool BF16, bool VEC>
+__device__ __forceinline__ I8Raw<BF16> i8_load8_raw(const void* row, int k, int K) {
+  I8Raw<BF16> o;
+  if (VEC && k + 8 <= K) {
+    const u32x4* p = reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned char*>(row) + (size_t)k * (BF16 ? 2 : 4));
+    o.r[0] = p[0];
+    if constexpr (!BF16) o.r[1] = p[1];
+  } else {
+    unsigned w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (k + j < K) {
+        if constexpr (BF16) w[j >> 1] |= (unsigned)reinterpret_cast<const bf16_t*>(row)[k + j] << (16 * (j & 1));
+        else w[j] = reinterpret_cast<const unsigned*>(row)[k + j];
+      }
+    o.r[0] = u32x4{w[0], w[1], w[2], w[3]};
+    if constexpr (!BF16) o.r[1] = u32x4{w[4], w[5], w[6], w[7]};
+  }
+  return o;
+}
+template <bool BF16>
+__device__ __forceinline__ void i8_unpack(const I8Raw<BF16>& o, float (&v)[8]) {
+  if constexpr (BF16) {
+    const u32x4 r = o.r[0];
+    v[0] = bf16_lo(r.x); v[1] = bf16_hi(r.x); v[2] = bf16_lo(r.y); v[3] = bf16_hi(r.y);
+    v[4] = bf16_lo(r.z); v[5] = bf16_hi(r.z); v[6] = bf16_lo(r.w); v[7] = bf16_hi(r.w);
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      v[4 * h] = __uint_as_float(o.r[h].x); v[4 * h + 1] = __uint_as_float(o.r[h].y);
+      v[4 * h + 2] = __uint_as_float(o.r[h].z); v[4 * h + 3] = __uint_as_float(o.r[h].w);
+    }
+  }
+}
+// Running maximum of the magnitudes' bits: pairs of 16 (bf16) or one of 32.
+typedef unsigned short i8_u16x2 __attribute__((ext_vector_type(2)));
+template <bool BF16>
+__device__ __forceinline__ unsigned i8_amax_raw(const I8Raw<BF16>& o, unsigned top) {
+  if constexpr (BF16) {
+    const unsigned w[4] = {o.r[0].x, o.r[0].y, o.r[0].z, o.r[0].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      top = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(i8_u16x2, top),
+                                                                   __builtin_bit_cast(i8_u16x2, w[j] & 0x7fff7fffu)));
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned w[4] = {o.r[h].x, o.r[h].y, o.r[h].z, o.r[h].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = max(top, w[j] & 0x7fffffffu);
+    }
+  }
+  return top;
+}
+template <bool BF16>
+__device__ __forceinline__ unsigned i8_amax_bits(unsigned top) {   // as the bits of an f32
+  return BF16 ? max(top << 16, top & 0xffff0000u) : top;
+}
+
 // One wave per row: E x 512 columns in registers, or (E = 0) the row read twice.  Writes zeros up to the row's pitch.
 template <bool BF16, bool VEC, int E>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantArgs a) {
@@ -97,18 +161,20 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantArgs a) {
   int8_t* out = a.q + m * a.ldq;
   unsigned top = 0;
   if constexpr (E > 0) {
-    float v[E][8];
+    I8Raw<BF16> x[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) i8_load8<BF16, VEC>(row, i * 512 + lane * 8, a.K, v[i]);
+    for (int i = 0; i < E; ++i) x[i] = i8_load8_raw<BF16, VEC>(row, i * 512 + lane * 8, a.K);
 #pragma unroll
-    for (int i = 0; i < E; ++i) top = i8_amax8(v[i], top);
-    top = dpp_wave_umax(top);
+    for (int i = 0; i < E; ++i) top = i8_amax_raw<BF16>(x[i], top);
+    top = dpp_wave_umax(i8_amax_bits<BF16>(top));
     const bool bad = i8_bad(top);
     const float s = i8_scale(__uint_as_float(top)), inv = 1.0f / s;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const int k = i * 512 + lane * 8;
-      if (k < a.ldq) *reinterpret_cast<u32x2*>(out + k) = i8_quant8(v[i], s, inv, bad);
+      float v[8];
+      i8_unpack<BF16>(x[i], v);
+      if (k < a.ldq) *reinterpret_cast<u32x2*>(out + k) = i8_quant8(v, s, inv, bad);
     }
     if (lane == 0) a.scale[m] = bad ? NAN : s;
   } else {
