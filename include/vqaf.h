@@ -719,7 +719,7 @@ int vqaf_scale_cast(const float* in, const float* scale, size_t n, int out_dtype
  * With z = x / temperature: logprobs (R,T) f32 = log softmax(z) at targets (R,T) int64; entropy (R) f32 of softmax(z);
  * top_logprobs / top_indices (R,K) f32 / int64, the K largest in falling order, ties to the lowest index, NaN first.
  * logits (R,C) `dtype`, rows `ld` >= 0 elements apart (0: one row repeated), inner stride 1, any element alignment.
- * T, K <= 128, K <= C; either may be 0, entropy may be NULL.  stats (R,2) f32, or NULL, receives what the backward
+ * T, K <= 128, K <= C <= 2^28; T and K may be 0, entropy may be NULL.  stats (R,2) f32, or NULL, receives what the backward
  * needs.  temperature in [2^-20, 2^20].
  * A negative target is none (log probability 0, no gradient); one past the classes gives NaN.  -inf logits have
  * probability 0.  A row of nothing but -inf has log probabilities -inf, entropy 0 and a zero gradient; a row with a

@@ -10,6 +10,8 @@ count roundings for arithmetic in units u = 2^-24 (half an f32 step, relative):
              over a wave
   logarithm  of the sum as f32: one step of the result, 2 u |log S|
   products   u each
+  underflow  the hardware exponential gives 0 below 2^-126, so e (and p = e / S, S >= 1) may be off by 2^-126 absolutely;
+             a gradient multiplies that by the factor that p has in it
 """
 from __future__ import annotations
 
@@ -18,6 +20,7 @@ import math
 import torch
 
 U = 2.0 ** -24
+FLUSH = 2.0 ** -126
 
 
 def _half_step(dtype: torch.dtype) -> float:
@@ -130,6 +133,7 @@ def token_logprobs_grad(logits, temperature, targets=None, g_logprobs=None, g_en
     tol = mag * ((2 * t + 14) * U + S)
     tol = tol + p * h.abs()[:, None] * (2 * t * U + S + 3 * U * lpf.abs() + entropy_bound(H, p, t)[:, None])
     tol = tol + size * 160 * U   # up to 128 + 32 terms added one by one
+    tol = tol + FLUSH * (amag[:, None] + h.abs()[:, None] * (torch.where(lp > -math.inf, lp, 0.0).abs() + H.abs()[:, None]))
     g, tol = g / temperature, tol / temperature + 4 * U * (g / temperature).abs()
     g[empty] = 0.0
     tol[empty] = 0.0
@@ -179,6 +183,7 @@ def distill(logits, teacher, indices, temperature=1.0, tail=False):
     # p as above; slope and mass to f32; q to f32, summed where an answer is named again, subtracted, scaled
     tol = p * slope.abs() * ((2 * t + 10) * U + tol_s[:, None])
     tol = tol + p * cut[:, None] * outside * (held_bound + tol_s + 2 * U)[:, None] + target * 140 * U
+    tol = tol + FLUSH * slope.abs()
     g, tol = g * temperature, tol * temperature + 4 * U * (g * temperature).abs()
     none = ~live.any(1)
     loss, loss_tol = torch.where(none, 0.0, loss), torch.where(none, 0.0, loss_tol)

@@ -116,7 +116,13 @@ def test_layouts_forward_and_gradient(dev, C, dtype):
 @pytest.mark.parametrize("C", [5, 430, 1023, 1030, 9001, 30522, 66000])
 def test_masked_rows_ties_and_broken_rows(dev, C, dtype):
     low = torch.finfo(dtype).min
-    x = _logits(12, C, dtype, C + 1)
+    x = _logits(16, C, dtype, C + 1)
+    x[12] = 0.0                                           # a few above one long tie
+    x[12, [0, C // 2, C - 1]] = torch.tensor([1.0, 2.0, 1.0], dtype=dtype)
+    x[13] = torch.arange(C) % 3 == 1                      # ties spread over the row
+    x[14] = -torch.arange(C).to(dtype) / 64               # all negative, sorted
+    x[15] = -5.0                                          # negative and tied, NaN with a sign bit among them
+    x[15, C // 4] = -math.nan
     x[0] = -math.inf                                      # a mask that leaves nothing
     x[1] = low                                            # masks of the type's lowest value, everywhere
     x[2, 1:] = low                                        # one live entry
@@ -132,13 +138,13 @@ def test_masked_rows_ties_and_broken_rows(dev, C, dtype):
     x[10, C // 3] = -3.0                                  # one live entry among masked ones
     x[11, : C - 1] = torch.finfo(dtype).max / 2           # the range's far ends
     x[11, C - 1] = low
-    tg = torch.full((12,), C // 3)
+    tg = torch.full((16,), C // 3)
     for top in sorted({1, min(C, 3), min(C, 40), min(C, 128)}):
         _check_logprobs(x, tg, top, 1.0, dev)
     from vqa_amd import ops
     xd = x.to(dev).requires_grad_()
     r = ops.token_logprobs(xd, tg.to(dev), temperature=0.5)
-    up = torch.linspace(-1, 1, 12)
+    up = torch.linspace(-1, 1, 16)
     g, = torch.autograd.grad((r.logprobs, r.entropy), xd, (up.to(dev), up.flip(0).to(dev)))
     want, tol = ao.token_logprobs_grad(x, 0.5, tg, up, up.flip(0))
     _close(g, want, tol, "gradient")
@@ -411,3 +417,78 @@ def test_row_past_32_bit_offsets(dev):
     wg, tol = ao.token_logprobs_grad(last, 1.0, torch.full((3,), 5), torch.ones(3))
     _close(g[-3:], wg, tol, "gradient")
     assert float(g[:1000].abs().max()) == 0.0
+
+
+def test_one_row_without_a_batch(dev):
+    from vqa_amd import ops
+    x = _logits(1, 77, torch.float32, 2)
+    xd = x[0].to(dev).requires_grad_()
+    r = ops.token_logprobs(xd, torch.tensor(4, device=dev), top=3)
+    assert r.logprobs.shape == () and r.entropy.shape == () and r.top_indices.shape == (3,)
+    many = ops.token_logprobs(xd, torch.tensor([4, 5], device=dev))
+    assert many.logprobs.shape == (2,) and torch.equal(many.logprobs[0], r.logprobs)
+    none = ops.token_logprobs(xd, torch.empty(0, dtype=torch.int64, device=dev))
+    assert none.logprobs.shape == (0,)
+    loss = ops.distill_loss(xd, r.top_logprobs, r.top_indices)
+    g, = torch.autograd.grad(loss + none.entropy * 0, xd)
+    _, _, want, tol = ao.distill(x, r.top_logprobs.detach().cpu()[None], r.top_indices.cpu()[None])
+    _close(g, want[0], tol[0] + 2.0 ** -23 * (want[0].abs() + tol[0]), "gradient")
+
+
+@pytest.mark.parametrize("C", [40, 3000])
+def test_gradient_of_one_row_shared_by_all(dev, C):
+    """A broadcast row: the gradient of every row, added."""
+    from vqa_amd import ops
+    x = _logits(1, C, torch.float32, 6)
+    leaf = x.to(dev).requires_grad_()
+    tg = torch.arange(5) * 3
+    r = ops.token_logprobs(leaf.expand(5, C), tg.to(dev))
+    g, = torch.autograd.grad(r.logprobs.sum(), leaf)
+    want, tol = ao.token_logprobs_grad(x.expand(5, C), 1.0, tg, torch.ones(5))
+    _close(g, want.sum(0, keepdim=True), tol.sum(0, keepdim=True) + 4 * ao.U * want.abs().sum(0, keepdim=True), "shared row")
+
+
+def test_no_gradient_of_a_gradient(dev):
+    from vqa_amd import ops
+    x = _logits(3, 50, torch.float32, 1).to(dev).requires_grad_()
+    g, = torch.autograd.grad(ops.token_logprobs(x).entropy.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+        torch.autograd.grad(g.sum(), x)
+    v, idx = torch.full((3, 2), -1.0, device=dev), torch.tensor([[0, 1]] * 3, device=dev)
+    g, = torch.autograd.grad(ops.distill_loss(x, v, idx), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+        torch.autograd.grad(g.sum(), x)
+
+
+def test_logits_changed_in_place_are_noticed(dev):
+    from vqa_amd import ops
+    x = _logits(3, 50, torch.float32, 1).to(dev).requires_grad_()
+    y = x * 1.0
+    r = ops.token_logprobs(y)
+    y.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.entropy.sum().backward()
+
+
+def test_refusals(dev):
+    from vqa_amd import ops
+    x = torch.zeros(4, 10, device=dev)
+    tg, v, idx = torch.zeros(4, dtype=torch.long, device=dev), torch.zeros(4, 2, device=dev), torch.zeros(4, 2, dtype=torch.long, device=dev)
+    for kw in (dict(targets=tg[:3]), dict(targets=tg.cpu()), dict(top=11), dict(top=-1), dict(temperature=0.0),
+               dict(targets=tg[:, None].expand(4, 129))):
+        with pytest.raises(ValueError):
+            ops.token_logprobs(x, **kw)
+    for kw in (dict(targets=tg.float()), dict(targets=tg.bool())):
+        with pytest.raises(TypeError):
+            ops.token_logprobs(x, **kw)
+    with pytest.raises(TypeError):
+        ops.token_logprobs(x.half())
+    with pytest.raises(ValueError):
+        ops.token_logprobs(torch.zeros(4, 200, device=dev), top=129)
+    for a, b, kw in ((v[:3], idx, {}), (v, idx[:, :1], {}), (v[:, :0], idx[:, :0], {}), (v, idx.cpu(), {}), (v, idx, dict(temperature=-1)),
+                     (v[0], idx[0], {}), (torch.zeros(4, 129, device=dev), torch.zeros(4, 129, dtype=torch.long, device=dev), {})):
+        with pytest.raises(ValueError):
+            ops.distill_loss(x, a, b, **kw)
+    for a, b in ((v.long(), idx), (v, idx.float())):
+        with pytest.raises(TypeError):
+            ops.distill_loss(x, a, b)

@@ -224,7 +224,7 @@ struct RowPieces {
       return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w))) >= thr;
     }
   }
-  // f(v, el) for the pieces that may hold a value of at least thr: few, so they are read again one by one (they are in
+  // f(v, el) for the pieces that may hold a value of at least thr, until it returns false: few, so they are read again one by one (they are in
   // the caches) rather than looked through in registers, which would unroll f once for each of them
   template <class F>
   __device__ __forceinline__ void walk_reaching(float thr, F f) const {
@@ -244,7 +244,7 @@ struct RowPieces {
       if (c < s.pieces && (E > 0 || reaches(r, thr))) {
         float v[V];
         an_unpack<BF16>(r, v);
-        f(v, c * V - s.shift);
+        if (!f(v, c * V - s.shift)) break;
       }
       if (E == 0) c += NT;
     }
@@ -499,7 +499,7 @@ constexpr int an_waves(int e) {
 
 bool an_shape_ok(long ld, int R, int C, int K, double temperature) {
   // (temperatures between 2^-20 and 2^20: their factors stay far inside f32)
-  return R > 0 && C > 0 && C < 0x7ffffff0 && ld >= 0 && K >= 0 && K <= AN_TOP_MAX && K <= C && temperature >= 9.5367431640625e-07 &&
+  return R > 0 && C > 0 && C <= (1 << 28) && ld >= 0 && K >= 0 && K <= AN_TOP_MAX && K <= C && temperature >= 9.5367431640625e-07 &&
          temperature <= 1048576.0;
 }
 // The gradient's rows have to lie on their 16-byte grid as the logits' do.

@@ -65,7 +65,7 @@ struct TopShared {
   __attribute__((aligned(16))) u64 cand[AN_CAP + 16];   // and room for the ranking's last step
   int n;
   float thr;
-  int cnt[2];
+  int cnt[1], round[2][NT / 64];
 };
 
 // how many of the workgroup's elements pass `f` (all threads call; two barriers)
@@ -86,44 +86,71 @@ __device__ __forceinline__ int an_block_count(const ROW& row, int* cnt, F f) {
   return cnt[0];
 }
 
-// The K best of a row into sh.cand, by counting alone: the K-th key bit by bit, then the index up to which elements
-// equal to it belong.  For rows whose candidates overflow the list (long ties: a masked row has nothing but) and rows
-// with NaN; 63 passes at most.
+// The K best of a row into sh.cand, by counting: for rows whose candidates overflow the list (a long tie: a masked or
+// padded row has nothing else) and rows with NaN.  `from`: a key that at least K elements reach.  The K-th key is that one
+// if fewer than K lie above it, else it is found bit by bit; of the elements equal to it the first in the order of the
+// index are taken, a round of pieces at a time.
 template <bool BF16, int NT>
-__device__ __forceinline__ void an_top_by_counting(const Span& span, TopShared<NT>& sh, int K) {
-  constexpr int V = Piece<BF16>::V;
+__device__ __forceinline__ void an_top_by_counting(const Span& span, TopShared<NT>& sh, int K, unsigned from) {
+  constexpr int V = Piece<BF16>::V, NW = NT / 64;
   RowPieces<BF16, NT, 0> row;   // reads the row again: the common path's registers stay its own
   row.s = span;
-  unsigned t = 0;
-  for (int b = 31; b >= 0; --b) {
-    const unsigned mid = t | (1u << b);
-    if (an_block_count<NT>(row, sh.cnt, [&](float x, int) { return an_key(x) >= mid; }) >= K) t = mid;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  unsigned t = from;
+  int above = an_block_count<NT>(row, sh.cnt, [&](float x, int) { return an_key(x) > t; });
+  if (above >= K) {
+    t = 0;
+    for (int b = 31; b >= 0; --b) {
+      const unsigned mid = t | (1u << b);
+      if (an_block_count<NT>(row, sh.cnt, [&](float x, int) { return an_key(x) >= mid; }) >= K) t = mid;
+    }
+    above = an_block_count<NT>(row, sh.cnt, [&](float x, int) { return an_key(x) > t; });
   }
-  const int above = an_block_count<NT>(row, sh.cnt, [&](float x, int) { return an_key(x) > t; });
   const int need = K - above;   // of the elements equal to t, >= 1
-  int last = 0;                 // the lowest index bound that admits `need` of them: [0, last]
-  {
-    int lo = 0, hi = row.s.C - 1;
-    while (lo < hi) {
-      const int mid = lo + ((hi - lo) >> 1);
-      if (an_block_count<NT>(row, sh.cnt, [&](float x, int j) { return an_key(x) == t && j <= mid; }) >= need) hi = mid;
-      else lo = mid + 1;
-    }
-    last = lo;
-  }
   __syncthreads();
-  if (threadIdx.x == 0) sh.n = 0;
+  if (tid == 0) sh.n = 0;
   __syncthreads();
-  row.walk([&](const float (&v)[V], int, int el) {
+  int taken = 0, higher = 0;    // of the equal ones and of the others, in the rounds so far
+  for (int c0 = 0; c0 < row.s.pieces && (taken < need || higher < above); c0 += NT) {
+    const int c = c0 + tid, el = c * V - row.s.shift;
+    float v[V];
+    int eq = 0, gt = 0;
+    if (c < row.s.pieces) {
+      an_unpack<BF16>(row.finish(row.fetch(c), c), v);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int col = el + j;
-      if (col < 0 || col >= row.s.C) continue;
-      const unsigned k = an_key(v[j]);
-      if (k > t || (k == t && col <= last)) sh.cand[atomicAdd(&sh.n, 1) & (AN_CAP - 1)] = an_pack(k, col);
+      for (int j = 0; j < V; ++j) {
+        const bool in = el + j >= 0 && el + j < row.s.C;
+        eq += in && an_key(v[j]) == t ? 1 : 0;
+        gt += in && an_key(v[j]) > t ? 1 : 0;
+      }
     }
-  });
-  __syncthreads();
+    int upto = eq;              // equal elements up to this thread, first in its wave, then in the workgroup
+    for (int o = 1; o < 64; o <<= 1) {
+      const int left = __shfl_up(upto, o, 64);
+      upto += lane >= o ? left : 0;
+    }
+    const int others = (int)dpp_wave_uadd((unsigned)gt);
+    if (lane == 63) sh.round[0][wave] = upto;
+    if (lane == 0) sh.round[1][wave] = others;
+    __syncthreads();
+    int before = taken + upto - eq;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (w < wave) before += sh.round[0][w];
+      taken += sh.round[0][w];
+      higher += sh.round[1][w];
+    }
+    if (eq + gt > 0) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (el + j < 0 || el + j >= row.s.C) continue;
+        const unsigned k = an_key(v[j]);
+        // (exactly K in all: `above` above t, `need` equal to it)
+        if (k > t || (k == t && before++ < need)) sh.cand[atomicAdd(&sh.n, 1) & (AN_CAP - 1)] = an_pack(k, el + j);
+      }
+    }
+    __syncthreads();
+  }
 }
 
 // Wave 0: a value that at least K, and not many more than K, of the threads' maxima reach.  At least K elements of the
@@ -252,19 +279,25 @@ __global__ __launch_bounds__(NT, W) void logprob_block_kernel(const LogprobArgs 
     const float thr = sh.thr;
     if (sh.tmax[tid] >= thr) {
       row.walk_reaching(thr, [&](const float (&v)[V], int el) {
+        int hits = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) hits += v[j] >= thr && el + j >= 0 && el + j < a.C ? 1 : 0;
+        if (hits == 0) return true;
+        int at = atomicAdd(&sh.n, hits);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           if (v[j] >= thr && el + j >= 0 && el + j < a.C) {
-            const int at = atomicAdd(&sh.n, 1);
             if (at < AN_CAP) sh.cand[at] = an_pack(an_key(v[j]), el + j);
+            ++at;
           }
         }
+        return at <= AN_CAP;   // past the list's end there is no use in the rest
       });
     }
     __syncthreads();
     counted = sh.n > AN_CAP;   // uniform
   }
-  if (counted) an_top_by_counting<BF16, NT>(row.s, sh, a.K);
+  if (counted) an_top_by_counting<BF16, NT>(row.s, sh, a.K, broken ? 0u : an_key(sh.thr));
   const int n = sh.n;
   if (tid < 16) sh.cand[n + tid] = 0;   // below every candidate
   __syncthreads();
