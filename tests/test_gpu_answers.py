@@ -492,3 +492,85 @@ def test_refusals(dev):
     for a, b in ((v.long(), idx), (v, idx.float())):
         with pytest.raises(TypeError):
             ops.distill_loss(x, a, b)
+
+
+def test_backward_replayed_without_its_forward(dev):
+    """The forward and the backward captured into graphs of their own, the backward replayed with other incoming
+    gradients: nothing of the replay before may be left in the gradient."""
+    from vqa_amd import ops
+    for C in (430, 30522):
+        x = _logits(9, C, torch.bfloat16, 7).to(dev).requires_grad_()
+        v, i = ops.token_logprobs(_logits(9, C, torch.bfloat16, 8).to(dev), top=5)[2:]
+        up = torch.ones((), device=dev)
+        torch.cuda.synchronize()
+        s = torch.cuda.Stream()
+        fwd, bwd = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(fwd, stream=s):
+            loss = ops.distill_loss(x, v, i, reduction="sum")
+        with torch.cuda.graph(bwd, pool=fwd.pool(), stream=s):
+            got, = torch.autograd.grad(loss, x, up)
+        ups = (2.0, 1.0, 0.5, 1.0, -3.0, 1.0)
+        kept = []
+        fwd.replay()
+        for u in ups:
+            up.fill_(u)
+            bwd.replay()
+            kept.append(got.clone())
+        torch.cuda.synchronize()
+        del loss
+        for u, g in zip(ups, kept):
+            xe = x.detach().clone().requires_grad_()
+            le = ops.distill_loss(xe, v, i, reduction="sum")
+            torch.autograd.grad(le, xe, retain_graph=True)   # takes the forward's gradient: the next is formed as the graph's
+            want, = torch.autograd.grad(le, xe, torch.full((), u, device=dev))
+            assert torch.equal(g, want), u
+
+
+def test_more_rows_than_a_launch_takes(dev):
+    """Rows in several launches (a launch has fewer than 2^32 threads): the rows on both sides of a border and the last."""
+    from vqa_amd import ops
+    R = (1 << 25) + 9          # a wave each
+    few = _logits(64, 3, torch.bfloat16, 3).to(dev)
+    x = few.repeat(R // 64 + 1, 1)[:R].requires_grad_()
+    at = torch.tensor([0, 1, (1 << 25) - 1, 1 << 25, (1 << 25) + 1, R - 1], device=dev)
+    f = few[at % 64].requires_grad_()
+    big, small = ops.token_logprobs(x, top=2), ops.token_logprobs(f, top=2)
+    for a, b in zip(big[1:], small[1:]):
+        assert torch.equal(a[at], b)
+    ga, = torch.autograd.grad(big.entropy.sum(), x)
+    gb, = torch.autograd.grad(small.entropy.sum(), f)
+    assert torch.equal(ga[at], gb)
+    v, i = big.top_logprobs.detach().roll(1, 0), big.top_indices
+    del big, ga
+    la, lb = (ops.distill_loss(a, b, c, reduction="none") for a, b, c in ((x, v, i), (f, v[at], i[at])))
+    assert torch.equal(la[at], lb)
+    ga, = torch.autograd.grad(la.sum(), x)
+    gb, = torch.autograd.grad(lb.sum(), f)
+    assert torch.equal(ga[at], gb)
+    del x, v, i, la, ga
+    R = (1 << 23) + 3          # a workgroup each: one row repeated
+    one = _logits(1, 1025, torch.bfloat16, 4).to(dev)
+    x = one.expand(R, 1025).requires_grad_()
+    got = ops.token_logprobs(x, top=1)
+    want = ops.token_logprobs(one, top=1)
+    for a, b in zip(got[1:], want[1:]):
+        assert torch.equal(a[-4:], b.expand(4, *b.shape[1:])) and torch.equal(a[:1], b)
+    loss = ops.distill_loss(x, got.top_logprobs.detach(), got.top_indices, tail=True, reduction="sum")
+    g, = torch.autograd.grad(loss, x, ops.unit_gradient(loss))
+    assert bool((g[0] != 0).any())
+    assert torch.equal(g[-4:], g[:1].expand(4, 1025)) and torch.equal(g[(1 << 23) - 1:(1 << 23) + 1], g[:1].expand(2, 1025))
+    ge, = torch.autograd.grad(got.entropy.sum(), x)
+    assert bool((ge[0] != 0).any())
+    assert torch.equal(ge[-4:], ge[:1].expand(4, 1025))
+
+
+def test_more_rows_or_classes_than_an_int_holds(dev):
+    from vqa_amd import ops
+    z = torch.zeros(1, device=dev)
+    with pytest.raises(ValueError, match="rows"):
+        ops.token_logprobs(z.expand(2 ** 32 + 5))
+    with pytest.raises(ValueError, match="rows"):
+        ops.token_logprobs(z.view(1, 1).expand(2 ** 32 + 5, 1))
+    with pytest.raises(ValueError, match="rows"):
+        ops.distill_loss(z.view(1, 1).expand(2 ** 32 + 5, 1), z.view(1, 1).expand(2 ** 32 + 5, 1),
+                         torch.zeros(1, 1, dtype=torch.int64, device=dev).expand(2 ** 32 + 5, 1))

@@ -192,3 +192,26 @@ def test_replayed_graph_and_streams(dev):
                 got.append(ops.int8_linear(xs[2][2], wq, ws))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want[2][2]) for g in got)
+
+
+def test_more_rows_than_a_launch_takes(dev):
+    """Rows in several launches (a launch has fewer than 2^32 threads): the rows on both sides of a border and the last."""
+    from vqa_amd import ops
+    M = (1 << 25) + 9
+    few = _x(64, 5, torch.bfloat16, 3).to(dev)
+    at = torch.tensor([0, 1, (1 << 25) - 1, 1 << 25, (1 << 25) + 1, M - 1], device=dev)
+    q, s = ops.quantize_rows(few.repeat(M // 64 + 1, 1)[:M])
+    wq, ws = ops.quantize_rows(few)
+    assert torch.equal(q[at], wq[at % 64]) and torch.equal(s[at], ws[at % 64])
+
+
+def test_more_rows_than_an_int_holds(dev):
+    from vqa_amd import ops
+    z = torch.zeros(1, 1, device=dev)
+    w, s = ops.quantize_rows(z)
+    with pytest.raises(ValueError, match="rows"):
+        ops.quantize_rows(z.expand(2 ** 32 + 5, 1))
+    with pytest.raises(ValueError, match="rows"):
+        ops.int8_linear(z.expand(2 ** 32 + 5, 1), w, s)
+    with pytest.raises(ValueError, match="fit"):
+        ops.int8_linear(z, w.expand(2 ** 32 + 5, 1), s)

@@ -1,28 +1,23 @@
 // What a model answers with: log probabilities of given tokens, the entropy of the answer distribution and its top
-// alternatives (forward and backward), and the distillation loss against a teacher's top answers with its gradient.
-// They score the answers for the membership attacks (attack/metric_src.py:302-426 reads a loss and a maximum per
-// sample; these are the finer scores) and train a student on them in place of hard labels (utils/src.py:96).
+// alternatives, forward and backward.  They score the answers for the membership attacks (attack/metric_src.py:302-426
+// reads a loss and a maximum per sample; these are the finer scores) and label them for a student (distill.hip).
 //
 // With z = x / T, m = max z, e_j = exp(z_j - m), S = sum_j e_j, p_j = e_j / S:
 //   log p_t = z_t - m - log S            H = log S - sum_j e_j (z_j - m) / S
 //   d log p_t / dx_j = (1{j = t} - p_j) / T            dH / dx_j = -p_j (log p_j + H) / T
-// and for a teacher's answers i_k with probabilities q_k (rest r, held by no answer of the list):
-//   L = T^2 [ sum_k q_k (log q_k - log p_{i_k}) + r (log r - log P) ],     P = sum of p_j outside the list
-//   dL / dx_j = T [ p_j (sum q + r) - sum_{k: i_k = j} q_k ] on the list,  T p_j [ sum q + r - r / P ] elsewhere.
 //
-// All of it is bound by the row of logits: read once (and its gradient written once).  A row therefore stays in
-// registers from its one read to its last use: rows of up to 1024 classes in one wave (four rows to a workgroup),
-// longer ones in a workgroup of 256 to 1024 threads, which covers 65536 classes; longer rows are read again for each
-// use.  Loads are whole 16-byte pieces on 16-byte addresses, whatever the row's own alignment (a vocabulary of 50265
-// puts every second bf16 row on an odd address): the row is cut at the pieces' borders and what lies outside it is
-// masked in registers.
+// All of it is bound by the row of logits, read once (and its gradient written once).  A row therefore stays in registers
+// from its one read to its last use: rows of up to 1024 classes in one wave (four rows to a workgroup), longer ones in a
+// workgroup of 256 threads with up to 50 pieces of 16 bytes each -- a row costs the fewest registers beside its own that
+// way, so the most rows are in flight on a CU (30522 bf16 classes: five; with 512 threads it was three, with 1024 two) --
+// and past about 66000 classes the row is read again for each use.  Loads are whole 16-byte pieces on 16-byte addresses,
+// whatever the row's own alignment (a vocabulary of 50265 puts every second bf16 row on an odd address): the row is cut at
+// the pieces' borders and what lies outside it is masked in registers.
 //
-// Precision.  The divergence of two close distributions is a small difference of large terms, so the normaliser, the
-// entropy's sum and the loss are carried in 64 bits: sums of eight in f32, sums of those in f64; the exponent
-// (x - m) log2(e) / T is formed with the two-term constant, because the rounding of a single one would shift every
-// term of a row the same way.  Rows of one wave, whose few terms do not average their rounding out, take the
-// exponential itself in f64 (a Taylor polynomial after range reduction; the f64 vector rate of this chip is the f32
-// one).  Probabilities, and with them the gradients, are f32 and rounded once into their type.
+// Precision: sums of eight in f32, sums of those in f64, the logarithm in f64 (rows of one wave: f32 with the sum's
+// rounding put back).  The exponent takes one f32 factor log2(e) / T (1 + delta); its rounding would shift every term the
+// same way, so delta times the mean exponent, which the entropy needs anyway, is taken out of log S.  Probabilities and
+// gradients are f32, rounded once into their type.
 
 #include "answers.h"
 
@@ -39,7 +34,7 @@ struct LogprobArgs {
   float* top_logprobs;
   int64_t* top_indices;
   float* stats;   // (R,2): m, S
-  long ld, R;
+  long ld, R, r0;   // r0: the launch's first row
   int C, T, K;
   AnTemp temp;
 };
@@ -190,13 +185,19 @@ __device__ __forceinline__ float an_threshold(const float* tmax, int threads_wit
   return an_unkey(lo);
 }
 
+// One read of the row into registers, its maximum (bf16: on packed pairs as integers), the sums of e and e t, and the
+// alternatives.  Those reach the K-th largest of the threads' maxima, or very nearly only they do: the threads that hold
+// such values look through their pieces once more, and the short list that results is ranked by counting.
+// Measured, 1920 rows of 30522 bf16 classes: 29 us without alternatives (4.0 TB/s), 35 us with 20 (3.3 TB/s), 41 with 64;
+// 1001 x 50265: 27 us without (3.7 TB/s).  Half of the time is vector instructions (14 for each value, 7 of them for e and e t);
+// 1920 rows are one and a half rounds of what fits on the chip.
 template <bool BF16, int NT, int E, int W>
 __global__ __launch_bounds__(NT, W) void logprob_block_kernel(const LogprobArgs a) {
   constexpr int V = Piece<BF16>::V, NW = NT / 64;
   __shared__ TopShared<NT> sh;
   __shared__ float s_max[NW];
   __shared__ double s_sum[2][NW], s_log;
-  const long r = blockIdx.x;
+  const long r = a.r0 + blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   RowPieces<BF16, NT, E> row;
   row.s = an_span<BF16>(a.x, a.ld, r, a.R, a.C);
@@ -356,11 +357,14 @@ __device__ __forceinline__ void an_wave_select(const unsigned (&key)[E], unsigne
   }
 }
 
+// Measured, 25000 rows of 430 f32 classes: 11.5 us without targets and alternatives (3.7 TB/s), 13.4 with a target each,
+// 20 with three alternatives, 25 with 20, 54 with 64: a row is some 300 instructions of one wave, most of them for the
+// alternatives.  One row alone takes 4 us.
 template <bool BF16, int E>
 __global__ __launch_bounds__(64 * AN_WAVES, E <= 8 ? 8 : 5) void logprob_wave_kernel(const LogprobArgs a) {
   __shared__ __attribute__((aligned(16))) u64 s_cand[AN_WAVES][AN_WCAP + 16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long r = (long)blockIdx.x * AN_WAVES + wave;
+  const long r = a.r0 + (long)blockIdx.x * AN_WAVES + wave;
   if (r >= a.R) return;   // no barrier below: a wave keeps to its own row
   const void* xr = an_row<BF16>(a.x, a.ld, r);
   float v[E];
@@ -568,16 +572,22 @@ struct LogprobGrad {
 };
 
 template <bool BF16>
-void an_launch_logprobs(const LogprobArgs& a, hipStream_t st) {
+void an_launch_logprobs(LogprobArgs a, hipStream_t st) {
   if (a.C <= AN_WAVE_C) {
     an_by_wave(a.C, [&](auto e) {
-      hipLaunchKernelGGL((logprob_wave_kernel<BF16, decltype(e)::value>), dim3((unsigned)((a.R + AN_WAVES - 1) / AN_WAVES)),
-                         dim3(64 * AN_WAVES), 0, st, a);
+      an_by_launch(a.R, 64, [&](long r0, long n) {
+        a.r0 = r0;
+        hipLaunchKernelGGL((logprob_wave_kernel<BF16, decltype(e)::value>), dim3((unsigned)((n + AN_WAVES - 1) / AN_WAVES)),
+                           dim3(64 * AN_WAVES), 0, st, a);
+      });
     });
   } else {
     an_by_block<BF16>(a.C, [&](auto nt, auto e) {
-      hipLaunchKernelGGL((logprob_block_kernel<BF16, decltype(nt)::value, decltype(e)::value, an_waves(decltype(e)::value)>), dim3((unsigned)a.R),
-                         dim3(decltype(nt)::value), 0, st, a);
+      constexpr int NT = decltype(nt)::value, E = decltype(e)::value;
+      an_by_launch(a.R, NT, [&](long r0, long n) {
+        a.r0 = r0;
+        hipLaunchKernelGGL((logprob_block_kernel<BF16, NT, E, an_waves(E)>), dim3((unsigned)n), dim3(NT), 0, st, a);
+      });
     });
   }
 }
@@ -597,7 +607,7 @@ extern "C" int vqaf_token_logprobs(const void* logits, long ld, const int64_t* t
   LogprobArgs a;
   a.x = logits; a.targets = targets; a.logprobs = logprobs; a.entropy = entropy;
   a.top_logprobs = top_logprobs; a.top_indices = top_indices; a.stats = stats;
-  a.ld = ld; a.R = R; a.C = C; a.T = T; a.K = K;
+  a.ld = ld; a.R = R; a.r0 = 0; a.C = C; a.T = T; a.K = K;
   a.temp = an_temp(temperature);
   if (dtype == VQAF_BF16) an_launch_logprobs<true>(a, (hipStream_t)stream);
   else an_launch_logprobs<false>(a, (hipStream_t)stream);

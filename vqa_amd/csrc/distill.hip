@@ -4,6 +4,11 @@
 //   L = T^2 [ sum_k q_k (log q_k - log p_{i_k}) + r (log r - log P) ],     P = sum of p_j outside the list
 //   dL / dx_j = T [ p_j (sum q + r) - sum_{k: i_k = j} q_k ] on the list,  T p_j [ sum q + r - r / P ] elsewhere.
 // Rows are held and walked as in answers.hip; the gradient for an incoming gradient of 1 leaves from the same read.
+//
+// Precision.  The divergence of two close distributions is a small difference of large terms, so the list's terms, the
+// logarithms and the loss are f64, and the sums over the row as in answers.hip (the factor's error taken out through
+// sum e t).  Rows of one wave, whose few terms do not average their rounding out, take the exponential itself in f64 (a
+// Taylor polynomial after range reduction; the f64 vector rate of this chip is the f32 one).
 
 #include "answers.h"
 
@@ -71,7 +76,7 @@ struct DistillArgs {
   float* row_loss;
   DistillStat* stats;   // or NULL
   void* grad;           // or NULL
-  long ld, ldg, R;
+  long ld, ldg, R, r0;  // r0: the launch's first row
   int C, K, tail;
   float scale;          // of the gradient: T * (1 or 1 / R)
   double t2;            // T^2
@@ -192,13 +197,17 @@ __device__ __forceinline__ u32x4 an_drop(u32x4 r, unsigned bits) {
 // taken out of the registers before the exponentials, so that the rest is summed by itself (1 - sum p would lose what is
 // left of it where the student agrees with its teacher), and their own terms are added by the list.
 // HOLD: the exponentials stay in registers for the gradient (f32: in the place of the logits; bf16: in twice the
-// registers, where that still leaves two workgroups to a CU); otherwise they are formed again.
+// registers, only for short rows); otherwise they are formed again.
+// Measured, 1920 rows of 30522 bf16 classes, 64 answers, with the rest as an event and the gradient: 65 us (3.6 TB/s read
+// and written; 45 us without the gradient); 511 x 50265 f32, 100 answers, loss only: 35 us (2.9 TB/s: two workgroups to
+// a CU hold all the rows at once, so that loads, sums and reductions of a row follow one another).  25 vector instructions a
+// value take two thirds of that.
 template <bool BF16, int NT, int E, bool TAIL, bool HOLD, int W>
 __global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs a) {
   constexpr int V = Piece<BF16>::V, NW = NT / 64;
   __shared__ DistillShared<NT> sh;
   extern __shared__ unsigned s_mark[];   // one bit per element of the pieces
-  const long r = blockIdx.x;
+  const long r = a.r0 + blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   RowPieces<BF16, NT, E> row;
   row.s = an_span<BF16>(a.x, a.ld, r, a.R, a.C);
@@ -338,12 +347,14 @@ __global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs 
                        [&](float q) { return none ? 0.f : -sc * q; });
 }
 
+// One wave per row of up to 1024 classes.  Measured, 64 x 430 bf16 and 1024 x 430 f32 with gradient: 7 us, a chain of
+// reductions and f64 logarithms.
 template <bool BF16, int E>
 __global__ __launch_bounds__(64 * AN_WAVES) void distill_wave_kernel(const DistillArgs a) {
   __shared__ DistillList s_list[AN_WAVES];
   __shared__ unsigned s_mark[AN_WAVES][AN_WAVE_C / 32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long r = (long)blockIdx.x * AN_WAVES + wave;
+  const long r = a.r0 + (long)blockIdx.x * AN_WAVES + wave;
   if (r >= a.R) return;   // no barrier below: a wave keeps to its own row
   DistillList& list = s_list[wave];
   unsigned* mark = s_mark[wave];
@@ -431,11 +442,14 @@ __global__ __launch_bounds__(1024) void answer_sum_kernel(const float* x, long n
 }
 
 template <bool BF16>
-int an_launch_distill(const DistillArgs& a, hipStream_t st) {
+int an_launch_distill(DistillArgs a, hipStream_t st) {
   if (a.C <= AN_WAVE_C) {
     an_by_wave(a.C, [&](auto e) {
-      hipLaunchKernelGGL((distill_wave_kernel<BF16, decltype(e)::value>), dim3((unsigned)((a.R + AN_WAVES - 1) / AN_WAVES)),
-                         dim3(64 * AN_WAVES), 0, st, a);
+      an_by_launch(a.R, 64, [&](long r0, long n) {
+        a.r0 = r0;
+        hipLaunchKernelGGL((distill_wave_kernel<BF16, decltype(e)::value>), dim3((unsigned)((n + AN_WAVES - 1) / AN_WAVES)),
+                           dim3(64 * AN_WAVES), 0, st, a);
+      });
     });
   } else {
     const size_t mark = ((size_t)a.C + 2 * Piece<BF16>::V + 31) / 32 * 4;
@@ -444,8 +458,11 @@ int an_launch_distill(const DistillArgs& a, hipStream_t st) {
       constexpr int NT = decltype(nt)::value, E = decltype(e)::value;
       constexpr bool HOLD = E > 0 && (!BF16 || E <= 4);
       constexpr int W = an_waves(BF16 && HOLD ? 2 * E + 2 : E + 2);
-      if (a.tail) hipLaunchKernelGGL((distill_block_kernel<BF16, NT, E, true, HOLD, W>), dim3((unsigned)a.R), dim3(NT), mark, st, a);
-      else hipLaunchKernelGGL((distill_block_kernel<BF16, NT, E, false, HOLD, W>), dim3((unsigned)a.R), dim3(NT), mark, st, a);
+      an_by_launch(a.R, NT, [&](long r0, long n) {
+        a.r0 = r0;
+        if (a.tail) hipLaunchKernelGGL((distill_block_kernel<BF16, NT, E, true, HOLD, W>), dim3((unsigned)n), dim3(NT), mark, st, a);
+        else hipLaunchKernelGGL((distill_block_kernel<BF16, NT, E, false, HOLD, W>), dim3((unsigned)n), dim3(NT), mark, st, a);
+      });
     });
   }
   VQAF_LAUNCH_CHECK();
@@ -465,7 +482,7 @@ extern "C" int vqaf_distill(const void* logits, long ld, const float* teacher, c
   DistillArgs a;
   a.x = logits; a.teacher = teacher; a.indices = indices; a.row_loss = row_loss;
   a.stats = reinterpret_cast<DistillStat*>(stats); a.grad = grad;
-  a.ld = ld; a.ldg = ld_grad; a.R = R; a.C = C; a.K = K; a.tail = tail != 0;
+  a.ld = ld; a.ldg = ld_grad; a.R = R; a.r0 = 0; a.C = C; a.K = K; a.tail = tail != 0;
   a.scale = (float)(temperature * scale);
   a.t2 = temperature * temperature;
   a.temp = an_temp(temperature);

@@ -8,11 +8,10 @@
 // sign of x - (q +- 1/2) s, one fused multiply-add, decides.  A row with NaN or an infinity gets the scale NaN, which
 // makes its outputs NaN.
 //
-// Three kernels.  Many tokens: one pass writes the rows as integers (bound by its bytes), and a matrix product on
-// 32x32x32 integer MFMAs with the tile shape and LDS-DMA images of the bf16 Linear kernel: the 128-byte rows of a k-step
-// hold 128 values instead of 64.  Up to 64 tokens: the product is bound by the weights' bytes and by latency, so a
-// workgroup takes 16 output channels, its waves cut the contraction among themselves and read the weights straight into
-// MFMA operands.  Up to a few tokens the workgroups also quantise the rows themselves and one launch does it all.
+// Many tokens: one pass writes the rows as integers, bound by its bytes, and a matrix product on 32x32x32 integer MFMAs
+// reads them through a ring of stages in shared memory.  Up to 64 tokens: the product is bound by the weights' bytes and
+// by latency, so a workgroup takes 16 output channels, its waves cut the contraction among themselves and read the weights
+// straight into MFMA operands.  Up to four tokens the workgroups quantise the rows themselves and one launch does it all.
 
 #include <mutex>
 
@@ -47,7 +46,7 @@ struct QuantArgs {
   const void* x;
   int8_t* q;
   float* scale;
-  long ldx, ldq, M;
+  long ldx, ldq, M, m0;   // m0: the launch's first row
   int K;
 };
 
@@ -152,10 +151,11 @@ __device__ __forceinline__ unsigned i8_amax_bits(unsigned top) {   // as the bit
 }
 
 // One wave per row: E x 512 columns in registers, or (E = 0) the row read twice.  Writes zeros up to the row's pitch.
+// Measured, bf16: 8191 x 4096 23 us (4.4 TB/s read and written), 12608 x 768 10 us (2.9 TB/s: a row is only 1.5 KB).
 template <bool BF16, bool VEC, int E>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantArgs a) {
   const int lane = threadIdx.x & 63;
-  const long m = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const long m = a.m0 + (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (m >= a.M) return;
   const void* row = reinterpret_cast<const unsigned char*>(a.x) + m * a.ldx * (BF16 ? 2 : 4);
   int8_t* out = a.q + m * a.ldq;
@@ -291,6 +291,9 @@ __device__ __forceinline__ void i8_write_tile(const Int8Args& g, i32x16 (&acc)[T
 // k-steps of 64 values go through a ring of STAGES stages in shared memory, all but one of them in flight, one barrier a
 // step.  The fragment reads are inline assembly: for a read it can see, the compiler waits until every LDS-DMA has landed
 // and would drain the ring.  Each block of reads waits for itself; the other waves of the SIMD multiply meanwhile.
+// Measured: 8191 x 4096 x 4096 138-150 us (1.8-2.0 P operations/s; the library's product of 8192 x 8192 x 8192 reaches
+// 2.06), 12608 x 768 x 2304 42 us (1.06 P: twelve k-steps, then 128 KB of output a workgroup that nothing overlaps, in two
+// rounds of tiles of which the second is three quarters full), 1920 x 768 x 768 on 64 x 64 tiles 9 us.
 constexpr int I8_BK = 64;
 
 // piece c (16 values) of row r of a [rows][64] image lies at position c ^ i8_swz(r): sixteen rows on sixteen slots
@@ -423,7 +426,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void int8_tile_kernel(const Int8
 }
 
 // ---------------------------------------------------------------------------------------------
-// Few tokens: 16 output channels per workgroup, the contraction cut among its four waves
+// Few tokens: 16 output channels per workgroup, the contraction cut among its four waves.  Measured: one token, 768 x 2304
+// 4.2 us and 4096 x 4096 6.7 us (2.5 TB/s of weights), the quantiser and the launch included
 // ---------------------------------------------------------------------------------------------
 constexpr int I8_SELF = 4;          // tokens whose rows the workgroups quantise themselves
 constexpr int I8_SELF_K = 8192;     // and the columns up to which they do
@@ -533,8 +537,8 @@ long i8_pitch(int K) { return ((long)K + I8_ROW - 1) / I8_ROW * I8_ROW; }
 size_t i8_scale_offset(long M, int K) { return ((size_t)M * i8_pitch(K) + 255) / 256 * 256; }
 
 template <bool BF16, bool VEC>
-void i8_launch_quant(const QuantArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)((a.M + 3) / 4)), block(256);
+void i8_launch_quant(const QuantArgs& a, long n, hipStream_t st) {
+  const dim3 grid((unsigned)((n + 3) / 4)), block(256);
   if (a.ldq <= 512) hipLaunchKernelGGL((quantize_rows_kernel<BF16, VEC, 1>), grid, block, 0, st, a);
   else if (a.ldq <= 1024) hipLaunchKernelGGL((quantize_rows_kernel<BF16, VEC, 2>), grid, block, 0, st, a);
   else if (a.ldq <= 2048) hipLaunchKernelGGL((quantize_rows_kernel<BF16, VEC, 4>), grid, block, 0, st, a);
@@ -547,8 +551,12 @@ void i8_quant(const void* x, long ldx, int M, int K, int dtype, int8_t* q, long 
   QuantArgs a;
   a.x = x; a.q = q; a.scale = scale; a.ldx = ldx; a.ldq = ldq; a.M = M; a.K = K;
   const bool vec = i8_vec(x, ldx, dtype);
-  if (dtype == VQAF_BF16) vec ? i8_launch_quant<true, true>(a, st) : i8_launch_quant<true, false>(a, st);
-  else vec ? i8_launch_quant<false, true>(a, st) : i8_launch_quant<false, false>(a, st);
+  // a launch may have fewer than 2^32 threads
+  for (a.m0 = 0; a.m0 < M; a.m0 += 1L << 25) {
+    const long n = M - a.m0 < (1L << 25) ? M - a.m0 : 1L << 25;
+    if (dtype == VQAF_BF16) vec ? i8_launch_quant<true, true>(a, n, st) : i8_launch_quant<true, false>(a, n, st);
+    else vec ? i8_launch_quant<false, true>(a, n, st) : i8_launch_quant<false, false>(a, n, st);
+  }
 }
 
 template <bool XB, bool YB, bool SELF>
@@ -590,9 +598,10 @@ int i8_launch_tile(Int8Args& g, hipStream_t st) {
 template <bool YB>
 int i8_launch_tiles(Int8Args& g, hipStream_t st) {
   // 256 x 256 tiles, one workgroup of eight waves per CU, once they nearly fill the chip (12608 x 768 x 2304: 450 tiles,
-  // 38 us against 43 us on 128 x 128; 2048 x 4096 x 4096: 128 tiles, 52 against 44 us); 128 x 128 tiles, two
-  // workgroups per CU, down to one for each CU (1920 x 768 x 2304: 270 tiles, 4 us faster than 64 x 64); then 64 x 64 in
-  // a ring twice as deep, where few workgroups have to hide the latency by themselves.
+  // 49 us with the quantiser against 62 us on 128 x 128; 2048 x 4096 x 4096: 128 tiles, 66 against 58 us); 128 x 128
+  // tiles, two workgroups per CU, down to one for each CU (1920 x 768 x 2304: 270 tiles, 17 us against 21 us on 64 x 64;
+  // 500 x 4096 x 1024: 32 tiles, 34 against 25 us); then 64 x 64 in a ring twice as deep, where few workgroups have to
+  // hide the latency by themselves.
   const long t256 = (long)((g.M + 255) / 256) * ((g.N + 255) / 256), t128 = (long)((g.M + 127) / 128) * ((g.N + 127) / 128);
   if (t256 >= 144) return i8_launch_tile<YB, 4, 2, 2, 4, 4, 2>(g, st);
   if (t128 >= 256) return i8_launch_tile<YB, 2, 2, 2, 2, 4, 2>(g, st);
@@ -624,7 +633,7 @@ extern "C" int vqaf_int8_linear(const void* x, long ldx, int x_dtype, const int8
   VQAF_REQUIRE(x && w && w_scale && y, VQAF_E_NULL);
   VQAF_REQUIRE(M > 0 && N > 0 && K > 0 && K <= I8_MAX_K && ldx >= 0 && ldw >= (K + 15) / 16 * 16 && ldw % 16 == 0 && ldy >= N,
                VQAF_E_SHAPE);
-  VQAF_REQUIRE((long)((M + 63) / 64) * ((N + 63) / 64) < 0x7fffffffL, VQAF_E_SHAPE);
+  VQAF_REQUIRE(N <= 1 << 27 && (long)((M + 63L) / 64) * ((N + 63) / 64) < 0x7fffffffL, VQAF_E_SHAPE);
   VQAF_REQUIRE(vqaf_dtype_ok(x_dtype) && vqaf_dtype_ok(y_dtype) && (bias == nullptr || vqaf_dtype_ok(bias_dtype)), VQAF_E_DTYPE);
   VQAF_REQUIRE(vqaf_aligned16(w) && reinterpret_cast<uintptr_t>(x) % vqaf_esize(x_dtype) == 0 &&
                reinterpret_cast<uintptr_t>(y) % vqaf_esize(y_dtype) == 0 && reinterpret_cast<uintptr_t>(w_scale) % 4 == 0 &&

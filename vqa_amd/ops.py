@@ -816,6 +816,7 @@ def unit_gradient(loss: torch.Tensor) -> torch.Tensor:
 # Answer scores and distillation
 # --------------------------------------------------------------------------------------------
 ANSWERS_MAX = 128  # given tokens, alternatives and teacher's answers per row
+ANSWERS_MAX_CLASSES = 2 ** 28
 
 
 class TokenLogprobs(NamedTuple):
@@ -860,9 +861,11 @@ def _answer_rows(logits: torch.Tensor):
     require_gpu(logits)
     dtype_code(logits)
     x = logits
-    if x.dim() == 2 and x.is_contiguous():
-        return x, x.shape[1]
     C = logits.shape[-1]
+    if C > ANSWERS_MAX_CLASSES or logits.numel() // C >= 2 ** 31:
+        raise ValueError(f"logits of at most 2^31 - 1 rows of {ANSWERS_MAX_CLASSES} classes, got shape {tuple(logits.shape)}")
+    if x.dim() == 2 and x.is_contiguous():
+        return x, C
     if x.dim() != 2:
         x = x.reshape(-1, C)
     if C > 1 and x.stride(1) != 1:
@@ -1025,6 +1028,7 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, ld, teacher, indices, temperature, tail, scale):
         out, stats, ctx.unit = _distill_forward(x, ld, teacher, indices, temperature, tail, scale, True)
+        ctx.recorded = torch.cuda.is_current_stream_capturing()
         ctx.save_for_backward(x, teacher, indices, stats)
         ctx.meta = (ld, temperature, scale)
         return out
@@ -1034,6 +1038,9 @@ class _Distill(torch.autograd.Function):
     def backward(ctx, up):
         grad, ctx.unit = ctx.unit, None   # handed out once: a second backward forms its own
         ready = grad is not None
+        recording = torch.cuda.is_current_stream_capturing()
+        if recording and not ctx.recorded:
+            ready = False   # the graph replays without this forward: it forms the gradient itself every time
         if not ready or up is not _unit_grads.get((up.device, up.dtype)):
             x, teacher, indices, stats = ctx.saved_tensors   # (also tells of logits changed in place since)
             ld, temperature, scale = ctx.meta
@@ -1042,7 +1049,7 @@ class _Distill(torch.autograd.Function):
             up = _f32(up)
             _launch(x.device, "vqaf_distill_bwd", x.data_ptr(), ld, teacher.data_ptr(), indices.data_ptr(), x.shape[0],
                     x.shape[1], teacher.shape[1], dtype_code(x), temperature, stats.data_ptr(), up.data_ptr(),
-                    int(scale is None), int(ready), 1.0 if scale is None else scale, grad.data_ptr(), _grad_pitch(x, ld))
+                    int(scale is None), int(ready and not recording), 1.0 if scale is None else scale, grad.data_ptr(), _grad_pitch(x, ld))
         return grad, None, None, None, None, None, None
 
 
@@ -1210,8 +1217,8 @@ def _int8_rows(x: torch.Tensor, what: str):
     dtype_code(x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{what} needs a last dimension, got shape {tuple(x.shape)}")
-    if x.shape[-1] > INT8_MAX_K:
-        raise ValueError(f"{what}: at most {INT8_MAX_K} columns, got {x.shape[-1]}")
+    if x.shape[-1] > INT8_MAX_K or x.numel() // x.shape[-1] >= 2 ** 31:
+        raise ValueError(f"{what}: at most 2^31 - 1 rows of {INT8_MAX_K} columns, got {tuple(x.shape)}")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if x2.shape[1] > 1 and x2.stride(1) != 1:
         x2 = x2.contiguous()
@@ -1250,7 +1257,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         raise TypeError(f"weight has to be (N,K) int8, got {tuple(weight.shape)} {weight.dtype}")
     N, K = weight.shape
     M = x2.shape[0]
-    if x2.shape[1] != K or N < 1:
+    if x2.shape[1] != K or not 1 <= N <= 2 ** 27:
         raise ValueError(f"x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
     if weight_scale.shape != (N,) or weight_scale.dtype != torch.float32:
         raise ValueError(f"weight_scale has to be ({N},) float32, got {tuple(weight_scale.shape)} {weight_scale.dtype}")
