@@ -216,3 +216,21 @@ def test_a_teacher_in_eight_bits_labels_scores_and_teaches(dev):
     moved = [n for n, p in student.named_parameters() if not torch.equal(p, before[n])]
     assert any(n.startswith("classifier") for n in moved) and any(n.startswith("vision_encoder") for n in moved)
     assert all(torch.isfinite(p).all() for p in student.parameters())
+
+
+def test_distillation_with_a_common_module(dev):
+    """A module that student and teacher share runs in eval mode for the labels and in training mode for the student."""
+    from vqa_amd import loops
+
+    class Common(nn.Linear):
+        def forward(self, x):
+            modes.append((torch.is_grad_enabled(), self.training))
+            return super().forward(x)
+    modes = []
+    a, b = Toy(4, 3, 0).to(dev), Toy(4, 3, 1).to(dev)
+    a.head = b.head = Common(4, 3).to(dev)
+    loops.distill(a, b, _loader(2, 5, 4, 3, 2), torch.optim.SGD(a.parameters(), lr=0.1), dev, top=2)
+    assert modes == [(False, False), (True, True)] * 2 and a.training
+    modes.clear()
+    loops.distill(a, a, _loader(1, 5, 4, 3, 2), torch.optim.SGD(a.parameters(), lr=0.1), dev, top=2)
+    assert modes == [(False, False), (True, True)]

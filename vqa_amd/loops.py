@@ -124,12 +124,13 @@ def distill(model: nn.Module, teacher: nn.Module, train_loader, optimizer, devic
     (ops.token_logprobs) are the targets of ops.distill_loss.  A student that has seen only another model's answers is the
     usual alternative to DP-SGD against the attacks that vqa_amd.mia scores.  hard_weight > 0 mixes the labels' mean
     cross-entropy in: (1 - hard_weight) * distillation + hard_weight * cross-entropy.  The teacher runs in eval mode
-    without gradients; held in eight bits (encoders.quantize_int8) it labels faster.  Returns (average loss, agreement of
+    without gradients, also in modules that it shares with the student; held in eight bits (encoders.quantize_int8) it labels faster.  Returns (average loss, agreement of
     the best answers in %)."""
     if not 0.0 <= hard_weight < 1.0:
         raise ValueError(f"hard_weight has to be in [0, 1), got {hard_weight}")
-    model.train()
     teacher.eval()
+    model.train()
+    shared = not set(model.modules()).isdisjoint(teacher.modules())   # (a common encoder, or the model itself)
     main_opt = optimizer['main'] if isinstance(optimizer, dict) else optimizer
     reducer = _main_reducer(main_opt)
     tot_loss = torch.zeros((), dtype=torch.float64, device=device)
@@ -140,10 +141,14 @@ def distill(model: nn.Module, teacher: nn.Module, train_loader, optimizer, devic
             _empty_batch(optimizer, main_opt, reducer, device)
             continue
         images, ids, mask, answers = _batch(batch, device)
+        if shared:
+            teacher.eval()
         with torch.no_grad():
             said = teacher(images=images, input_ids=ids, attention_mask=mask)
             said = said[0] if isinstance(said, tuple) else said
             label = ops.token_logprobs(said, top=min(top, said.shape[-1]), temperature=temperature, entropy=False)
+        if shared:
+            model.train()
         _zero_grad(optimizer)
         outputs = model(images=images, input_ids=ids, attention_mask=mask)
         loss = ops.distill_loss(outputs, label.top_logprobs, label.top_indices, temperature=temperature, tail=tail)
