@@ -534,12 +534,14 @@ def test_more_rows_than_a_launch_takes(dev):
     x = few.repeat(R // 64 + 1, 1)[:R].requires_grad_()
     at = torch.tensor([0, 1, (1 << 25) - 1, 1 << 25, (1 << 25) + 1, R - 1], device=dev)
     f = few[at % 64].requires_grad_()
-    big, small = ops.token_logprobs(x, top=2), ops.token_logprobs(f, top=2)
-    for a, b in zip(big[1:], small[1:]):
-        assert torch.equal(a[at], b)
+    # (against the definition: the order of a row's sums follows its alignment and the kernel that its row count takes)
+    big, want = ops.token_logprobs(x, top=2), ao.token_logprobs(few[at % 64].cpu(), top=2)
+    for name in ("entropy", "top_logprobs"):
+        _close(getattr(big, name)[at], want[name], want[name + "_tol"], name)
+    assert torch.equal(big.top_indices[at].cpu(), want["top_indices"])
     ga, = torch.autograd.grad(big.entropy.sum(), x)
-    gb, = torch.autograd.grad(small.entropy.sum(), f)
-    assert torch.equal(ga[at], gb)
+    g, tol = ao.token_logprobs_grad(few[at % 64].cpu(), 1.0, g_entropy=torch.ones(6))
+    _close(ga[at], g, tol, "entropy gradient")
     v, i = big.top_logprobs.detach().roll(1, 0), big.top_indices
     del big, ga
     la, lb = (ops.distill_loss(a, b, c, reduction="none") for a, b, c in ((x, v, i), (f, v[at], i[at])))
@@ -574,3 +576,45 @@ def test_more_rows_or_classes_than_an_int_holds(dev):
     with pytest.raises(ValueError, match="rows"):
         ops.distill_loss(z.view(1, 1).expand(2 ** 32 + 5, 1), z.view(1, 1).expand(2 ** 32 + 5, 1),
                          torch.zeros(1, 1, dtype=torch.int64, device=dev).expand(2 ** 32 + 5, 1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("C", [1, 2, 7, 13, 64, 65, 127, 128, 200, 257, 320, 385, 430, 448, 511, 512])
+def test_many_short_rows(dev, C, dtype):
+    """Row counts from which rows share a wave: masked, tied and broken rows next to ordinary ones, any alignment."""
+    from vqa_amd import ops
+    few = _logits(37, C, dtype, C)
+    few[1] = -math.inf
+    few[2, : C - 1] = -math.inf
+    few[3] = 0.25                                        # a tie of all
+    few[4, ::2] = torch.finfo(dtype).min
+    few[5, C // 2] = math.nan
+    few[6, 0] = math.inf
+    few[7] = math.nan
+    few[8] = -few[8].abs() - 1                           # nothing above zero
+    few[9, C // 3:] = few[9].max()                       # a long tie
+    few[10, C // 2:] = -math.inf
+    few[11] = -math.inf
+    few[11, -1] = -math.nan
+    few[12, ::3] = -0.0
+    few[12, 1::3] = 0.0
+    few[13] *= 1000
+    R = 8192 + 5
+    idx = (torch.arange(R) * 11) % 37
+    tg = (torch.arange(37)[:, None] * 5 + torch.arange(19)) % (C + 1) - 1
+    for top, T, off, ld in ((0, 1.0, 0, C), (1, 0.7, 0, C), (min(3, C), 1.0, 1, C + 3), (min(8, C), 4.0, 3, C + 1), (min(5, C), 1.0, 5, C)):
+        want = ao.token_logprobs(few, tg, top, T)
+        buf = torch.full((off + R * ld,), math.nan, dtype=dtype, device=dev)
+        x = buf.as_strided((R, C), (ld, 1), off)
+        x.copy_(few[idx].to(dev))
+        got = ops.token_logprobs(x, tg[idx].to(dev), top=top, temperature=T)
+        for name in ("entropy", "logprobs") + (("top_logprobs",) if top else ()):
+            _close(getattr(got, name), want[name][idx].reshape(getattr(got, name).shape),
+                   want[name + "_tol"][idx].nan_to_num(0.0).reshape(getattr(got, name).shape), name)
+        if top:   # (no bound, a broken row: no target there is exactly 0)
+            assert torch.equal(got.top_indices.cpu(), want["top_indices"][idx])
+    x = few[idx].to(dev).requires_grad_()
+    ok = ~torch.isnan(few).any(1) & ~(few == math.inf).any(1)
+    g, = torch.autograd.grad(ops.token_logprobs(x).entropy.sum(), x)
+    want, tol = ao.token_logprobs_grad(few, 1.0, None, None, torch.ones(37))
+    _close(g[ok[idx].to(dev)], want[idx[ok[idx]]], tol[idx[ok[idx]]], "entropy gradient")

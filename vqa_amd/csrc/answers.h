@@ -169,22 +169,30 @@ __device__ __forceinline__ u32x4 an_load_edge(const Span& s, int el) {
   return u32x4{w[0], w[1], w[2], w[3]};
 }
 
-// The pieces tid, tid + NT, ... of a row, in registers (E > 0) or read again on every walk (E == 0).
+// The pieces id, id + NT, ... of a row, in registers (E > 0) or read again on every walk (E == 0).  The row belongs to a
+// workgroup of NT threads, or (NT = 16) to sixteen lanes.
 template <bool BF16, int NT, int E>
 struct RowPieces {
   static constexpr int V = Piece<BF16>::V;
   Span s;
   u32x4 raw[E > 0 ? E : 1];
 
-  // One piece.  Pieces past the row, and those that reach outside the matrix, read piece 1 instead, which lies inside
-  // the row (rows here have more than 1024 classes).
+  static __device__ __forceinline__ int id() { return NT == 16 ? (int)threadIdx.x & 15 : (int)threadIdx.x; }
+  // One piece.  A workgroup's rows have more than 1024 classes: pieces past the row, and those that reach outside the
+  // matrix, read piece 1 instead, which lies inside the row.  Sixteen lanes' rows may be shorter: they read nothing then.
   __device__ __forceinline__ u32x4 fetch(int c) const {
     const bool safe = c >= s.skip_lo && c < s.pieces - s.skip_hi;
-    return *reinterpret_cast<const u32x4*>(s.first + (size_t)(safe ? (unsigned)c * 16u : 16u));
+    if constexpr (NT == 16) {
+      u32x4 r = {0, 0, 0, 0};
+      if (safe) r = *reinterpret_cast<const u32x4*>(s.first + (size_t)((unsigned)c * 16u));
+      return r;
+    } else {
+      return *reinterpret_cast<const u32x4*>(s.first + (size_t)(safe ? (unsigned)c * 16u : 16u));
+    }
   }
   __device__ __forceinline__ u32x4 finish(u32x4 r, int c) const {
     const int el = c * V - s.shift;
-    if (s.skip_lo + s.skip_hi != 0) {   // uniform
+    if (s.skip_lo + s.skip_hi != 0) {   // the first or the last row
       if ((c == 0 && s.skip_lo) || (c == s.pieces - 1 && s.skip_hi)) r = an_load_edge<BF16>(s, el);
     }
     return an_mask<BF16>(r, el, s.C);
@@ -192,9 +200,9 @@ struct RowPieces {
   __device__ __forceinline__ void load() {
     if constexpr (E > 0) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) raw[i] = fetch((int)threadIdx.x + i * NT);
+      for (int i = 0; i < E; ++i) raw[i] = fetch(id() + i * NT);
 #pragma unroll
-      for (int i = 0; i < E; ++i) raw[i] = finish(raw[i], (int)threadIdx.x + i * NT);
+      for (int i = 0; i < E; ++i) raw[i] = finish(raw[i], id() + i * NT);
     }
   }
   // The thread's largest value; NaN counts as the largest or not at all.
@@ -235,10 +243,10 @@ struct RowPieces {
 #pragma unroll
       for (int i = 0; i < E; ++i) hit |= reaches(raw[i], thr) ? 1ull << i : 0ull;
     }
-    int c = threadIdx.x;
+    int c = id();
     while (E > 0 ? hit != 0 : c < s.pieces) {
       if (E > 0) {
-        c = (int)threadIdx.x + (__ffsll((long long)hit) - 1) * NT;
+        c = id() + (__ffsll((long long)hit) - 1) * NT;
         hit &= hit - 1;
       }
       const u32x4 r = c < s.pieces ? finish(fetch(c), c) : u32x4{0, 0, 0, 0};
@@ -262,9 +270,9 @@ struct RowPieces {
   __device__ __forceinline__ void walk_raw(F f) const {
     if constexpr (E > 0) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) f(raw[i], (int)threadIdx.x + i * NT, ((int)threadIdx.x + i * NT) * V - s.shift);
+      for (int i = 0; i < E; ++i) f(raw[i], id() + i * NT, (id() + i * NT) * V - s.shift);
     } else {
-      for (int c = threadIdx.x; c < s.pieces; c += NT) f(finish(fetch(c), c), c, c * V - s.shift);
+      for (int c = id(); c < s.pieces; c += NT) f(finish(fetch(c), c), c, c * V - s.shift);
     }
   }
   // f(v, c, el): the V values of piece c, the first of them in column el; columns outside [0, C) hold -inf
@@ -275,11 +283,11 @@ struct RowPieces {
       for (int i = 0; i < E; ++i) {
         float v[V];
         an_unpack<BF16>(raw[i], v);
-        f(v, (int)threadIdx.x + i * NT, ((int)threadIdx.x + i * NT) * V - s.shift);
+        f(v, id() + i * NT, (id() + i * NT) * V - s.shift);
         __builtin_amdgcn_sched_barrier(0);   // one piece's temporaries at a time: other waves fill the gaps
       }
     } else {
-      for (int c = threadIdx.x; c < s.pieces; c += NT) {
+      for (int c = id(); c < s.pieces; c += NT) {
         float v[V];
         an_unpack<BF16>(finish(fetch(c), c), v);
         f(v, c, c * V - s.shift);

@@ -7,12 +7,12 @@
 //   d log p_t / dx_j = (1{j = t} - p_j) / T            dH / dx_j = -p_j (log p_j + H) / T
 //
 // All of it is bound by the row of logits, read once (and its gradient written once).  A row therefore stays in registers
-// from its one read to its last use: rows of up to 1024 classes in one wave (four rows to a workgroup), longer ones in a
-// workgroup of 256 threads with up to 50 pieces of 16 bytes each -- a row costs the fewest registers beside its own that
-// way, so the most rows are in flight on a CU (30522 bf16 classes: five; with 512 threads it was three, with 1024 two) --
-// and past about 66000 classes the row is read again for each use.  Loads are whole 16-byte pieces on 16-byte addresses,
-// whatever the row's own alignment (a vocabulary of 50265 puts every second bf16 row on an odd address): the row is cut at
-// the pieces' borders and what lies outside it is masked in registers.
+// from its one read to its last use: rows of up to 1024 classes in one wave (many rows of up to 512 classes: four to a
+// wave), longer ones in a workgroup of 256 threads with up to 50 pieces of 16 bytes each -- a row costs the fewest
+// registers beside its own that way, so the most rows are in flight on a CU (30522 bf16 classes: five; with 512 threads it
+// was three, with 1024 two) -- and past about 66000 classes the row is read again for each use.  Loads are whole 16-byte
+// pieces on 16-byte addresses, whatever the row's own alignment (a vocabulary of 50265 puts every second bf16 row on an odd
+// address): the row is cut at the pieces' borders and what lies outside it is masked in registers.
 //
 // Precision: sums of eight in f32, sums of those in f64, the logarithm in f64 (rows of one wave: f32 with the sum's
 // rounding put back).  The exponent takes one f32 factor log2(e) / T (1 + delta); its rounding would shift every term the
@@ -357,9 +357,9 @@ __device__ __forceinline__ void an_wave_select(const unsigned (&key)[E], unsigne
   }
 }
 
-// Measured, 25000 rows of 430 f32 classes: 11.5 us without targets and alternatives (3.7 TB/s), 13.4 with a target each,
-// 20 with three alternatives, 25 with 20, 54 with 64: a row is some 300 instructions of one wave, most of them for the
-// alternatives.  One row alone takes 4 us.
+// Measured, 430 f32 classes: 1024 rows with a target 2.8 us, with three alternatives 4.1, with 20 5 us; 25000 rows with a
+// target and 20 alternatives 25 us, with 64 54 us: a row is some 300 instructions of one wave, most of them for the
+// alternatives.
 template <bool BF16, int E>
 __global__ __launch_bounds__(64 * AN_WAVES, E <= 8 ? 8 : 5) void logprob_wave_kernel(const LogprobArgs a) {
   __shared__ __attribute__((aligned(16))) u64 s_cand[AN_WAVES][AN_WCAP + 16];
@@ -505,6 +505,162 @@ __global__ __launch_bounds__(64 * AN_WAVES, E <= 8 ? 8 : 5) void logprob_wave_ke
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Log probabilities: four rows of up to 512 classes per wave, a row to sixteen lanes
+// ---------------------------------------------------------------------------------------------
+// Taken from 8192 rows on, for up to eight alternatives.  With many rows the instructions of the reductions and of the
+// alternatives count, and here four rows share them; with few the latency does, and a whole wave to a row has less of it.
+// Measured, 430 f32 classes with a target and 0 / 3 / 8 alternatives: 25000 rows 11.2 / 15.4 / 18.2 us (3.8 TB/s without
+// alternatives) against 13.1 / 19.6 / 23.0 with a wave to a row, 8192 rows 5.9 / 8.0 / 9.4 against 6.8 / 9.4 / 10.8, 4096
+// rows 4.4 / 6.3 / 7.6 against 4.7 / 6.4 / 7.1, 1024 rows 3.4 / 5.3 / 6.4 against 2.8 / 4.1 / 4.4; 25000 rows of 430 bf16
+// classes 10.3 / 14.8 / 17.4 against 15.6 / 21.4 / 24.5.  Loads are 16-byte pieces as in the longer rows: single elements
+// of sixteen lanes cost the bf16 rows 19.5 us.
+constexpr int AN_GROUP_FROM = 8192;
+constexpr int AN_GROUP_C = 512, AN_GROUP_K = 8, AN_GROUP_ROWS = 16;   // classes, alternatives, rows per workgroup
+constexpr int AN_GCAP = 48;                                           // candidates a row lists
+
+// the sixteen bits of a ballot that belong to the lane's row
+__device__ __forceinline__ unsigned an_group_bits(u64 who, int lane) {
+  const unsigned half = lane & 32 ? (unsigned)(who >> 32) : (unsigned)who;
+  return (half >> (lane & 16)) & 0xffffu;
+}
+
+template <bool BF16, int E>
+__global__ __launch_bounds__(64 * AN_WAVES, E * (BF16 ? 2 : 1) <= 8 ? 8 : 7) void logprob_group_kernel(const LogprobArgs a) {
+  constexpr int V = Piece<BF16>::V;
+  __shared__ __attribute__((aligned(16))) u64 s_cand[AN_GROUP_ROWS][AN_GCAP + 16];
+  const int lane = threadIdx.x & 63, l = lane & 15, group = threadIdx.x >> 4;
+  const long rl = a.r0 + (long)blockIdx.x * AN_GROUP_ROWS + group;
+  const bool live = rl < a.R;
+  const long r = live ? rl : a.R - 1;   // (lanes without a row go along with the last one and write nothing)
+  const void* xr = an_row<BF16>(a.x, a.ld, r);
+  RowPieces<BF16, 16, E> row;
+  row.s = an_span<BF16>(a.x, a.ld, r, a.R, a.C);
+  row.load();
+  int64_t t = -1;
+  if (l < a.T) t = a.targets[r * a.T + l];   // the first 16; more are read below
+  const float best = row.max();
+  float m = dpp_row_max(best);
+  if (__ballot(m == -INFINITY) != 0) {   // (the maximum may leave NaN out)
+    bool nan = false;
+    row.walk([&](const float (&v)[V], int, int) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) nan |= v[j] != v[j];
+    });
+    if (an_group_bits(__ballot(nan), lane) != 0 && m == -INFINITY) m = NAN;
+  }
+  const bool empty = m == -INFINITY;
+  float xt = t >= 0 && t < a.C ? an_at<BF16>(xr, t) : 0.f;   // on its way under the exponentials
+  double S = 0.0;
+  float Wt = 0.f;
+  const float hi = a.temp.hi;
+  row.renew();
+  row.walk([&](const float (&v)[V], int, int) {
+    float e[V], w = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float u = (v[j] - m) * hi;
+      e[j] = an_exp2(u);
+      w = fmaf(e[j], an_floor(u), w);
+    }
+    S += (double)an_tree<V>(e);
+    Wt += w;
+  });
+  S = dpp_row_sum(S);
+  const float w = dpp_row_sum(Wt), s32 = (float)S;
+  // log S: the f32 logarithm of the rounded sum and the rounding's share
+  const float mean_t = (float)AN_LN2 * (w / s32);
+  const double log_s = empty ? -INFINITY
+                             : (double)logf(s32) + (double)((float)(S - (double)s32) * __builtin_amdgcn_rcpf(s32)) - a.temp.delta * mean_t;
+  if (l == 0 && live) {
+    if (a.entropy != nullptr) a.entropy[r] = empty ? 0.f : (float)(log_s - (double)mean_t);
+    if (a.stats != nullptr) {
+      a.stats[2 * r] = m;
+      a.stats[2 * r + 1] = empty ? 1.f : s32 * (1.f - (float)a.temp.delta * mean_t);
+    }
+  }
+  for (int i = l; i < a.T; i += 16) {
+    if (i >= 16) {
+      t = a.targets[r * a.T + i];
+      xt = t >= 0 && t < a.C ? an_at<BF16>(xr, t) : 0.f;
+    }
+    // (negative: none)
+    if (live) a.logprobs[r * a.T + i] = t < 0 ? 0.f : t >= a.C ? NAN : an_logprob(xt, m, log_s, a.temp.inv_t);
+  }
+  if (a.K == 0) return;
+
+  // what the K-th largest of the lanes' maxima reaches
+  u64* cand = s_cand[group];
+  unsigned left = l < row.s.pieces ? an_key(best) : 0u, low = dpp_row_umax(left);
+  for (int k = 1; k < a.K; ++k) {
+    const unsigned who = an_group_bits(__ballot(left == low), lane);
+    left = l == __ffs((int)who) - 1 ? 0u : left;
+    low = dpp_row_umax(left);
+  }
+  if (low < AN_KEY_MINF) low = AN_KEY_MINF;   // fewer lanes than answers: a short row, all of it
+  const float thr = an_unkey(low);
+  // which of the lane's values those are, their places in the list, and the values read again (there are few)
+  unsigned hit[(E * V + 31) / 32] = {};
+  row.renew();
+  {
+    int b = 0;
+    row.walk([&](const float (&v)[V], int, int el) {
+#pragma unroll
+      for (int j = 0; j < V; ++j, ++b) hit[b / 32] |= v[j] >= thr && (thr > -INFINITY || (el + j >= 0 && el + j < a.C)) ? 1u << (b % 32) : 0u;
+    });
+  }
+  int mine = 0;
+#pragma unroll
+  for (int i = 0; i < (E * V + 31) / 32; ++i) mine += __popc(hit[i]);
+  int at = mine;
+  at += (int)dpp_move<0x111, 0xf>(0u, (unsigned)at);   // sums over the lanes so far (row_shr)
+  at += (int)dpp_move<0x112, 0xf>(0u, (unsigned)at);
+  at += (int)dpp_move<0x114, 0xf>(0u, (unsigned)at);
+  at += (int)dpp_move<0x118, 0xf>(0u, (unsigned)at);
+  int n = __shfl(at, lane | 15, 64);
+  at -= mine;
+#pragma unroll
+  for (int i = 0; i < (E * V + 31) / 32; ++i) {
+    unsigned h = hit[i];
+    while (h != 0 && at < AN_GCAP) {
+      const int b = i * 32 + __ffs((int)h) - 1;
+      h &= h - 1;
+      const int col = (l + 16 * (b / V)) * V + b % V - row.s.shift;
+      cand[at++] = an_pack(an_key(an_at<BF16>(xr, col)), col);
+    }
+  }
+  // long ties and NaN: the whole wave takes the row by its keys, one such row after the other
+  const bool broken = !empty && !(S == S);
+  u64 over = __ballot(n > AN_GCAP || broken);
+  while (over != 0) {
+    constexpr int EW = (E * V + 3) / 4;
+    const int of = (__ffsll((long long)over) - 1) & 48;   // first lane of that row
+    const int in = (int)((threadIdx.x & ~63u) + of) / 16;
+    const long which = a.r0 + (long)blockIdx.x * AN_GROUP_ROWS + in;
+    const void* p = an_row<BF16>(a.x, a.ld, which < a.R ? which : a.R - 1);
+    unsigned key[EW];
+#pragma unroll
+    for (int i = 0; i < EW; ++i) key[i] = lane + 64 * i < a.C ? an_key(an_at<BF16>(p, lane + 64 * i)) : 0u;
+    an_wave_select<EW>(key, AN_KEY_MINF, a.K, s_cand[in]);
+    if ((lane & 48) == of) n = a.K;
+    over &= ~(0xffffull << of);
+  }
+  cand[n + l] = 0;
+  __builtin_amdgcn_wave_barrier();
+  __threadfence_block();
+  for (int i = l; i < n; i += 16) {
+    const u64 c = cand[i];
+    int before = 0;
+    for (int j = 0; j < n; j += 4)
+#pragma unroll
+      for (int o = 0; o < 4; ++o) before += cand[j + o] > c ? 1 : 0;
+    if (before < a.K && live) {
+      a.top_indices[r * a.K + before] = an_index(c);
+      a.top_logprobs[r * a.K + before] = an_logprob(an_unkey((unsigned)(c >> 32)), m, log_s, a.temp.inv_t);
+    }
+  }
+}
+
 struct LogprobGrad {
   const int64_t* targets;
   const int64_t* top_indices;
@@ -573,7 +729,26 @@ struct LogprobGrad {
 
 template <bool BF16>
 void an_launch_logprobs(LogprobArgs a, hipStream_t st) {
-  if (a.C <= AN_WAVE_C) {
+  if (a.C <= AN_GROUP_C && a.K <= AN_GROUP_K && a.R >= AN_GROUP_FROM) {
+    const auto go = [&](auto e) {
+      an_by_launch(a.R, 16, [&](long r0, long n) {
+        a.r0 = r0;
+        hipLaunchKernelGGL((logprob_group_kernel<BF16, decltype(e)::value>), dim3((unsigned)((n + AN_GROUP_ROWS - 1) / AN_GROUP_ROWS)),
+                           dim3(64 * AN_WAVES), 0, st, a);
+      });
+    };
+    const int e = ((a.C + Piece<BF16>::V - 1) / Piece<BF16>::V + 1 + 15) / 16;   // (a piece more than an aligned row fills)
+    if (e <= 1) go(std::integral_constant<int, 1>());
+    else if (e <= 2) go(std::integral_constant<int, 2>());
+    else if (e <= 3) go(std::integral_constant<int, 3>());
+    else if (e <= 4) go(std::integral_constant<int, 4>());
+    else if (BF16 || e <= 5) go(std::integral_constant<int, 5>());
+    else if constexpr (!BF16) {
+      if (e <= 6) go(std::integral_constant<int, 6>());
+      else if (e <= 7) go(std::integral_constant<int, 7>());
+      else go(std::integral_constant<int, 9>());
+    }
+  } else if (a.C <= AN_WAVE_C) {
     an_by_wave(a.C, [&](auto e) {
       an_by_launch(a.R, 64, [&](long r0, long n) {
         a.r0 = r0;

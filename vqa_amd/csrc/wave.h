@@ -60,4 +60,36 @@ __device__ __forceinline__ double dpp_wave_sum(double x) {
   return __builtin_bit_cast(double, r);
 }
 
+// ---------------------------------------------------------------------------------------------
+// The same over each row of sixteen lanes: four rotations, the result in every lane of the row.
+// ---------------------------------------------------------------------------------------------
+template <class F>
+__device__ __forceinline__ unsigned dpp_row_u32(unsigned x, F f) {
+  x = f(x, dpp_move<0x121, 0xf>(x, x));
+  x = f(x, dpp_move<0x122, 0xf>(x, x));
+  x = f(x, dpp_move<0x124, 0xf>(x, x));
+  x = f(x, dpp_move<0x128, 0xf>(x, x));
+  return x;
+}
+__device__ __forceinline__ float dpp_row_max(float v) {
+  return __uint_as_float(dpp_row_u32(__float_as_uint(v), [](unsigned a, unsigned b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+__device__ __forceinline__ float dpp_row_sum(float v) {
+  return __uint_as_float(dpp_row_u32(__float_as_uint(v), [](unsigned a, unsigned b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+__device__ __forceinline__ unsigned dpp_row_umax(unsigned v) {
+  return dpp_row_u32(v, [](unsigned a, unsigned b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ double dpp_row_sum(double x) {
+  x = dpp_add<0x121, 0xf>(x);
+  x = dpp_add<0x122, 0xf>(x);
+  x = dpp_add<0x124, 0xf>(x);
+  x = dpp_add<0x128, 0xf>(x);
+  return x;
+}
+
 }  // namespace
