@@ -908,15 +908,16 @@ def _addr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-def _logprobs_forward(x, ld, targets, top, temperature, entropy, stats):
-    """One launch; (logprobs, entropy, top_logprobs, top_indices, stats), None where not asked for."""
+def _logprobs_forward(x, targets, call, stats):
+    """One launch; (logprobs, entropy, top_logprobs, top_indices, stats), None where not asked for, in the shapes that the
+    caller returns.  call: (row pitch, leading dimensions, targets of a row, alternatives, temperature, entropy)."""
+    ld, lead, T, top, temperature, entropy = call
     R, C = x.shape
     dev, f32 = x.device, torch.float32
-    T = 0 if targets is None else targets.shape[1]
-    lp = None if targets is None else torch.empty((R, T), dtype=f32, device=dev)
-    ent = torch.empty(R, dtype=f32, device=dev) if entropy else None
-    tl = torch.empty((R, top), dtype=f32, device=dev) if top else None
-    ti = torch.empty((R, top), dtype=torch.int64, device=dev) if top else None
+    lp = None if targets is None else torch.empty(targets.shape, dtype=f32, device=dev)
+    ent = torch.empty(lead, dtype=f32, device=dev) if entropy else None
+    tl = torch.empty((*lead, top), dtype=f32, device=dev) if top else None
+    ti = torch.empty((*lead, top), dtype=torch.int64, device=dev) if top else None
     st = torch.empty((R, 2), dtype=f32, device=dev) if stats else None
     _launch(dev, "vqaf_token_logprobs", x.data_ptr(), ld, _addr(targets), R, C, T, top, dtype_code(x), temperature,
             _addr(lp), _addr(ent), _addr(tl), _addr(ti), _addr(st))
@@ -931,10 +932,10 @@ def _token_indices(t: torch.Tensor, what: str) -> torch.Tensor:
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, ld, targets, top, temperature, entropy):
-        lp, ent, tl, ti, st = _logprobs_forward(x, ld, targets, top, temperature, entropy, True)
-        ctx.save_for_backward(x, targets, ti, st, ent)
-        ctx.meta = (ld, 0 if targets is None else targets.shape[1], top, temperature)
+    def forward(ctx, x, targets, call):
+        lp, ent, tl, ti, ctx.stats = _logprobs_forward(x, targets, call, True)
+        ctx.save_for_backward(x, targets, ti, ent)
+        ctx.call = call
         ctx.set_materialize_grads(False)
         if ti is not None:
             ctx.mark_non_differentiable(ti)
@@ -943,17 +944,17 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     @_first_order
     def backward(ctx, g_lp, g_ent, g_top, _g_idx):
-        x, targets, ti, st, ent = ctx.saved_tensors
-        ld, T, top, temperature = ctx.meta
         if g_lp is None and g_ent is None and g_top is None:
-            return None, None, None, None, None, None
+            return None, None, None
+        x, targets, ti, ent = ctx.saved_tensors
+        ld, _, T, top, temperature, _ = ctx.call
         R, C = x.shape
         g_lp, g_ent, g_top = _f32(g_lp), _f32(g_ent), _f32(g_top)
         grad = _grad_rows(x, ld)
         _launch(x.device, "vqaf_token_logprobs_bwd", x.data_ptr(), ld, _addr(targets), _addr(ti), R, C, T, top,
-                dtype_code(x), temperature, st.data_ptr(), _addr(ent), _addr(g_lp), _addr(g_ent), _addr(g_top),
+                dtype_code(x), temperature, ctx.stats.data_ptr(), _addr(ent), _addr(g_lp), _addr(g_ent), _addr(g_top),
                 grad.data_ptr(), _grad_pitch(x, ld))
-        return grad, None, None, None, None, None
+        return grad, None, None
 
 
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0, temperature: float = 1.0,
@@ -973,7 +974,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     top = int(top)
     if not 0 <= top <= min(C, ANSWERS_MAX):
         raise ValueError(f"top has to be in [0, {min(C, ANSWERS_MAX)}], got {top}")
-    tg, given = None, None
+    T, tg = 0, None
     if targets is not None:
         given = targets.shape
         if given != lead and given[:-1] != lead:
@@ -985,20 +986,17 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
         T = 1 if given == lead else given[-1]
         if T > ANSWERS_MAX:
             raise ValueError(f"at most {ANSWERS_MAX} targets for each row, got {T}")
-        tg = targets.contiguous().view(R, T)
+        tg = targets.contiguous()
     if R == 0:
-        z = x.sum(1, dtype=torch.float32)
-        lp = None if tg is None else (z[:, None].expand(0, tg.shape[1]) * 1.0)
-        ent, tl = (z if entropy else None), (z[:, None].expand(0, top) * 1.0 if top else None)
-        ti = torch.empty(0, top, dtype=torch.int64, device=x.device) if top else None
-    elif x.requires_grad and torch.is_grad_enabled():
-        lp, ent, tl, ti = _TokenLogprobs.apply(x, ld, tg, top, temperature, bool(entropy))
-    else:
-        lp, ent, tl, ti, _ = _logprobs_forward(x, ld, tg, top, temperature, entropy, False)
-    if len(lead) == 1:
-        return TokenLogprobs(lp.view(given) if lp is not None and given == lead else lp, ent, tl, ti)
-    return TokenLogprobs(None if lp is None else lp.view(given), None if ent is None else ent.view(lead),
-                         None if tl is None else tl.view(*lead, top), None if ti is None else ti.view(*lead, top))
+        z = x.sum(1, dtype=torch.float32).view(lead)
+        lp = None if tg is None else (z if given == lead else z[..., None].expand(given)) * 1.0
+        ent, tl = (z if entropy else None), (z[..., None].expand(*lead, top) * 1.0 if top else None)
+        ti = torch.empty((*lead, top), dtype=torch.int64, device=x.device) if top else None
+        return TokenLogprobs(lp, ent, tl, ti)
+    call = (ld, lead, T, top, temperature, bool(entropy))
+    if x.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobs(*_TokenLogprobs.apply(x, tg, call))
+    return TokenLogprobs(*_logprobs_forward(x, tg, call, False)[:4])
 
 
 def _distill_forward(x, ld, teacher, indices, temperature, tail, scale, needs):
