@@ -14,6 +14,7 @@
 // straight into MFMA operands.  Up to four tokens the workgroups quantise the rows themselves and one launch does it all.
 
 #include <mutex>
+#include <type_traits>
 
 #include "common.h"
 #include "wave.h"
@@ -219,34 +220,62 @@ __device__ __forceinline__ float i8_bias(const Int8Args& g, int n) {
   return g.bias_bf16 ? bf16_to_f32(reinterpret_cast<const bf16_t*>(g.bias)[n]) : reinterpret_cast<const float*>(g.bias)[n];
 }
 
+// Scales and bias of a wave's tokens and channels, asked for before the product so that they are there after it: a lane
+// has those of token 32 i + (lane & 31) and channel 32 j + (lane & 31).  The bias comes as its two halves, whatever its
+// type, so that nothing is decided, and nothing awaited, before the product.
+template <int TM, int TN>
+struct I8Scales {
+  float x[TM], w[TN];
+  unsigned short lo[TN], hi[TN];
+  __device__ __forceinline__ void load(const Int8Args& g, int m0, int n0, int lane) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) x[i] = g.x_scale[min(m0 + i * 32 + (lane & 31), g.M - 1)];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = min(n0 + j * 32 + (lane & 31), g.N - 1);
+      w[j] = g.w_scale[n];
+      const unsigned char* p = reinterpret_cast<const unsigned char*>(g.bias != nullptr ? g.bias : (const void*)g.zeros);
+      const long at = g.bias == nullptr ? 0 : (long)n * (g.bias_bf16 ? 2 : 4);
+      lo[j] = *reinterpret_cast<const unsigned short*>(p + at);
+      hi[j] = *reinterpret_cast<const unsigned short*>(p + at + (g.bias_bf16 ? 0 : 2));
+    }
+  }
+  __device__ __forceinline__ float bias(const Int8Args& g, int j) const {   // (bf16: both are the upper half)
+    return __uint_as_float((unsigned)hi[j] << 16 | (g.bias_bf16 ? 0u : lo[j]));
+  }
+};
+
 // A wave's 32 TM tokens x 32 TN channels from (m0, n0) on: scales, bias, rounding, and out through an image of 32 tokens
 // in shared memory, so that stores are whole 16-byte pieces of rows.
 // acc[i][j][e]: token 32 i + (lane & 31), channel 32 j + (e & 3) + 8 (e >> 2) + 4 (lane >> 5)
 template <bool OUT_BF16, int TM, int TN>
-__device__ __forceinline__ void i8_write_tile(const Int8Args& g, i32x16 (&acc)[TM][TN], unsigned char* img, int m0, int n0,
-                                              int lane) {
+__device__ __forceinline__ void i8_write_tile(const Int8Args& g, const I8Scales<TM, TN>& sc, i32x16 (&acc)[TM][TN], unsigned char* img,
+                                              int m0, int n0, int lane) {
   constexpr int ES = OUT_BF16 ? 2 : 4;
   constexpr int PITCH = 32 * TN * ES + (OUT_BF16 ? 8 : 16);
   const int half = lane >> 5;
-  float sx[TM];
+  float* chan = reinterpret_cast<float*>(img);   // the channels' scales and biases, from one lane each to all
 #pragma unroll
-  for (int i = 0; i < TM; ++i) sx[i] = g.x_scale[min(m0 + i * 32 + (lane & 31), g.M - 1)];
+  for (int j = 0; j < TN; ++j) {
+    chan[j * 64 + (lane & 31)] = sc.w[j];
+    chan[j * 64 + 32 + (lane & 31)] = sc.bias(g, j);
+  }
+  asm volatile("" ::: "memory");
 #pragma unroll
   for (int j = 0; j < TN; ++j) {   // in place: the sums become the outputs' bits
-    float sw[16], bv[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int n = min(n0 + j * 32 + (e & 3) + 8 * (e >> 2) + 4 * half, g.N - 1);
-      sw[e] = g.w_scale[n];
-      bv[e] = i8_bias(g, n);
+    for (int r = 0; r < 4; ++r) {
+      const f32x4 sw = *reinterpret_cast<const f32x4*>(chan + j * 64 + 8 * r + 4 * half);
+      const f32x4 bv = *reinterpret_cast<const f32x4*>(chan + j * 64 + 32 + 8 * r + 4 * half);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc[i][j][4 * r + e] = __float_as_int(fmaf((float)acc[i][j][4 * r + e] * sc.x[i], sw[e], bv[e]));
     }
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        acc[i][j][e] = __float_as_int(fmaf((float)acc[i][j][e] * sx[i], sw[e], bv[e]));
     __builtin_amdgcn_sched_barrier(0);
   }
+  asm volatile("" ::: "memory");
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -288,54 +317,140 @@ __device__ __forceinline__ void i8_write_tile(const Int8Args& g, i32x16 (&acc)[T
 }
 
 // The product: output tiles of 32 TM WM tokens x 32 TN WN channels, a workgroup of WM x WN waves of 32 TM x 32 TN each.
-// k-steps of 64 values go through a ring of STAGES stages in shared memory, all but one of them in flight, one barrier a
-// step.  The fragment reads are inline assembly: for a read it can see, the compiler waits until every LDS-DMA has landed
-// and would drain the ring.  Each block of reads waits for itself; the other waves of the SIMD multiply meanwhile.
-// Measured: 8191 x 4096 x 4096 138-150 us (1.8-2.0 P operations/s; the library's product of 8192 x 8192 x 8192 reaches
-// 2.06), 12608 x 768 x 2304 42 us (1.06 P: twelve k-steps, then 128 KB of output a workgroup that nothing overlaps, in two
-// rounds of tiles of which the second is three quarters full), 1920 x 768 x 768 on 64 x 64 tiles 9 us.
+// k-steps of 64 values go through a ring of STAGES stages in shared memory, all but the one being read in flight, one
+// barrier a step.  A wave reads the operands of a half step under the products of the half before.
+// Measured: 8191 x 4096 x 4096 135 us (2.04 P operations/s), 8192 x 8192 x 8192 490 us (2.24 P; the library's product
+// 2.06), where the chip's power sets the pace (1.8 GHz; the same with zeros 415 us at 2.3 GHz; matrix instructions alone, on
+// random operands in registers, 3.5 P).  12608 x 768 x 2304 37 us (1.21 P: twelve k-steps, then 128 KB of output a
+// workgroup that nothing overlaps, in two rounds of tiles of which the second is three quarters full), 1920 x 768 x 768 on
+// 64 x 64 tiles 7.8 us, 500 x 4096 x 1024 13 us.  With each half step's operands awaited before its products it was 145, 42,
+// 9.2 and 16.7 us; scales and bias asked for after the product cost 4 us of the second.
 constexpr int I8_BK = 64;
 
 // piece c (16 values) of row r of a [rows][64] image lies at position c ^ i8_swz(r): sixteen rows on sixteen slots
 __device__ __forceinline__ int i8_swz(int r) { return (r >> 2) & 3; }
 
-// one k32 step of a wave: TM token and TN channel fragments (blocks of 32 rows are 2048 bytes apart and swizzled alike)
+// The operands of a wave's k32 step: TM token and TN channel fragments (blocks of 32 rows are 2048 bytes apart in the
+// image and swizzled alike).
 template <int TM, int TN>
-__device__ __forceinline__ void i8_step(unsigned xa, unsigned wa, i32x16 (&acc)[TM][TN]) {
+struct I8Frag {
   i32x4 x[TM], w[TN];
+};
+// Inline assembly throughout: for a read that it can see, the compiler waits until every LDS-DMA has landed and would drain
+// the ring.  Each block waits for its own reads, and ends with as many idle states as a reader of the last sum needs.
+template <int TM, int TN>
+__device__ __forceinline__ void i8_read(I8Frag<TM, TN>& n, unsigned xa, unsigned wa) {
   if constexpr (TM == 4 && TN == 2) {
     asm volatile("ds_read_b128 %4, %7\n\t"
-                 "ds_read_b128 %0, %6\n\t"
                  "ds_read_b128 %5, %7 offset:2048\n\t"
+                 "ds_read_b128 %0, %6\n\t"
                  "ds_read_b128 %1, %6 offset:2048\n\t"
                  "ds_read_b128 %2, %6 offset:4096\n\t"
                  "ds_read_b128 %3, %6 offset:6144\n\t"
                  "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(w[0]), "=&v"(w[1])
+                 : "=&v"(n.x[0]), "=&v"(n.x[1]), "=&v"(n.x[2]), "=&v"(n.x[3]), "=&v"(n.w[0]), "=&v"(n.w[1])
                  : "v"(xa), "v"(wa)
                  : "memory");
   } else if constexpr (TM == 2 && TN == 2) {
     asm volatile("ds_read_b128 %2, %5\n\t"
-                 "ds_read_b128 %0, %4\n\t"
                  "ds_read_b128 %3, %5 offset:2048\n\t"
+                 "ds_read_b128 %0, %4\n\t"
                  "ds_read_b128 %1, %4 offset:2048\n\t"
                  "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(w[0]), "=&v"(w[1])
+                 : "=&v"(n.x[0]), "=&v"(n.x[1]), "=&v"(n.w[0]), "=&v"(n.w[1])
                  : "v"(xa), "v"(wa)
                  : "memory");
   } else {
-    static_assert(TM == 1 && TN == 1, "shapes with a block of reads");
+    static_assert(TM == 1 && TN == 1, "shapes with a block of their own");
     asm volatile("ds_read_b128 %1, %3\n\t"
                  "ds_read_b128 %0, %2\n\t"
                  "s_waitcnt lgkmcnt(0)"
-                 : "=&v"(x[0]), "=&v"(w[0])
+                 : "=&v"(n.x[0]), "=&v"(n.w[0])
                  : "v"(xa), "v"(wa)
                  : "memory");
   }
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[j], x[i], acc[i][j], 0, 0, 0);
+}
+// the products of c while the operands n of the next step arrive
+template <int TM, int TN>
+__device__ __forceinline__ void i8_step(i32x16 (&acc)[TM][TN], const I8Frag<TM, TN>& c, I8Frag<TM, TN>& n, unsigned xa, unsigned wa) {
+  if constexpr (TM == 4 && TN == 2) {
+    asm volatile("v_mfma_i32_32x32x32_i8 %0, %18, %14, %0\n\t"
+                 "ds_read_b128 %12, %21\n\t"
+                 "ds_read_b128 %8, %20\n\t"
+                 "ds_read_b128 %13, %21 offset:2048\n\t"
+                 "ds_read_b128 %9, %20 offset:2048\n\t"
+                 "ds_read_b128 %10, %20 offset:4096\n\t"
+                 "ds_read_b128 %11, %20 offset:6144\n\t"
+                 "v_mfma_i32_32x32x32_i8 %1, %19, %14, %1\n\t"
+                 "v_mfma_i32_32x32x32_i8 %2, %18, %15, %2\n\t"
+                 "v_mfma_i32_32x32x32_i8 %3, %19, %15, %3\n\t"
+                 "v_mfma_i32_32x32x32_i8 %4, %18, %16, %4\n\t"
+                 "v_mfma_i32_32x32x32_i8 %5, %19, %16, %5\n\t"
+                 "v_mfma_i32_32x32x32_i8 %6, %18, %17, %6\n\t"
+                 "v_mfma_i32_32x32x32_i8 %7, %19, %17, %7\n\t"
+                 "s_nop 11\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[1][0]), "+v"(acc[1][1]), "+v"(acc[2][0]), "+v"(acc[2][1]), "+v"(acc[3][0]), "+v"(acc[3][1]), "=&v"(n.x[0]), "=&v"(n.x[1]), "=&v"(n.x[2]), "=&v"(n.x[3]), "=&v"(n.w[0]), "=&v"(n.w[1])
+                 : "v"(c.x[0]), "v"(c.x[1]), "v"(c.x[2]), "v"(c.x[3]), "v"(c.w[0]), "v"(c.w[1]), "v"(xa), "v"(wa)
+                 : "memory");
+  } else if constexpr (TM == 2 && TN == 2) {
+    asm volatile("v_mfma_i32_32x32x32_i8 %0, %10, %8, %0\n\t"
+                 "ds_read_b128 %6, %13\n\t"
+                 "ds_read_b128 %4, %12\n\t"
+                 "ds_read_b128 %7, %13 offset:2048\n\t"
+                 "ds_read_b128 %5, %12 offset:2048\n\t"
+                 "v_mfma_i32_32x32x32_i8 %1, %11, %8, %1\n\t"
+                 "v_mfma_i32_32x32x32_i8 %2, %10, %9, %2\n\t"
+                 "v_mfma_i32_32x32x32_i8 %3, %11, %9, %3\n\t"
+                 "s_nop 11\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[1][0]), "+v"(acc[1][1]), "=&v"(n.x[0]), "=&v"(n.x[1]), "=&v"(n.w[0]), "=&v"(n.w[1])
+                 : "v"(c.x[0]), "v"(c.x[1]), "v"(c.w[0]), "v"(c.w[1]), "v"(xa), "v"(wa)
+                 : "memory");
+  } else {
+    static_assert(TM == 1 && TN == 1, "shapes with a block of their own");
+    asm volatile("v_mfma_i32_32x32x32_i8 %0, %4, %3, %0\n\t"
+                 "ds_read_b128 %2, %6\n\t"
+                 "ds_read_b128 %1, %5\n\t"
+                 "s_nop 11\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "+v"(acc[0][0]), "=&v"(n.x[0]), "=&v"(n.w[0])
+                 : "v"(c.x[0]), "v"(c.w[0]), "v"(xa), "v"(wa)
+                 : "memory");
+  }
+}
+template <int TM, int TN>
+__device__ __forceinline__ void i8_last(i32x16 (&acc)[TM][TN], const I8Frag<TM, TN>& c) {
+  if constexpr (TM == 4 && TN == 2) {
+    asm volatile("v_mfma_i32_32x32x32_i8 %0, %12, %8, %0\n\t"
+                 "v_mfma_i32_32x32x32_i8 %1, %13, %8, %1\n\t"
+                 "v_mfma_i32_32x32x32_i8 %2, %12, %9, %2\n\t"
+                 "v_mfma_i32_32x32x32_i8 %3, %13, %9, %3\n\t"
+                 "v_mfma_i32_32x32x32_i8 %4, %12, %10, %4\n\t"
+                 "v_mfma_i32_32x32x32_i8 %5, %13, %10, %5\n\t"
+                 "v_mfma_i32_32x32x32_i8 %6, %12, %11, %6\n\t"
+                 "v_mfma_i32_32x32x32_i8 %7, %13, %11, %7\n\t"
+                 "s_nop 15\n\t"
+                 "s_nop 15"
+                 : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[1][0]), "+v"(acc[1][1]), "+v"(acc[2][0]), "+v"(acc[2][1]), "+v"(acc[3][0]), "+v"(acc[3][1])
+                 : "v"(c.x[0]), "v"(c.x[1]), "v"(c.x[2]), "v"(c.x[3]), "v"(c.w[0]), "v"(c.w[1]));
+  } else if constexpr (TM == 2 && TN == 2) {
+    asm volatile("v_mfma_i32_32x32x32_i8 %0, %6, %4, %0\n\t"
+                 "v_mfma_i32_32x32x32_i8 %1, %7, %4, %1\n\t"
+                 "v_mfma_i32_32x32x32_i8 %2, %6, %5, %2\n\t"
+                 "v_mfma_i32_32x32x32_i8 %3, %7, %5, %3\n\t"
+                 "s_nop 15\n\t"
+                 "s_nop 15"
+                 : "+v"(acc[0][0]), "+v"(acc[0][1]), "+v"(acc[1][0]), "+v"(acc[1][1])
+                 : "v"(c.x[0]), "v"(c.x[1]), "v"(c.w[0]), "v"(c.w[1]));
+  } else {
+    static_assert(TM == 1 && TN == 1, "shapes with a block of their own");
+    asm volatile("v_mfma_i32_32x32x32_i8 %0, %2, %1, %0\n\t"
+                 "s_nop 15\n\t"
+                 "s_nop 15"
+                 : "+v"(acc[0][0])
+                 : "v"(c.x[0]), "v"(c.w[0]));
+  }
 }
 
 template <bool OUT_BF16, int TM, int TN, int WM, int WN, int STAGES, int OCC>
@@ -359,29 +474,41 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void int8_tile_kernel(const Int8
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN, half = lane >> 5;
 
-  // LDS-DMA sources: piece j * THREADS + tid -> (row piece / 4, position piece % 4)
-  const int8_t* xs[XJ];
-  const int8_t* ws[WJ];
+  I8Scales<TM, TN> scales;
+  scales.load(g, m0 + wm * 32 * TM, n0 + wn * 32 * TN, lane);
+
+  // LDS-DMA sources: piece j * THREADS + tid -> (row piece / 4, position piece % 4), as offsets from the tile's first rows;
+  // rows past the edge repeat the last one, and their outputs are not stored
+  const int8_t* xb = g.q + (long)m0 * g.ldq;
+  const int8_t* wb = g.w + (long)n0 * g.ldw;
+  unsigned xo[XJ], wo[WJ];
   int wk[WJ];
 #pragma unroll
   for (int j = 0; j < XJ; ++j) {
     const int p = j * THREADS + tid, row = p >> 2, c = (p & 3) ^ i8_swz(row);
-    xs[j] = g.q + (long)min(m0 + row, g.M - 1) * g.ldq + c * 16;   // rows past the edge repeat the last one;
+    xo[j] = (unsigned)min(row, g.M - 1 - m0) * (unsigned)g.ldq + c * 16;
   }
 #pragma unroll
   for (int j = 0; j < WJ; ++j) {
     const int p = j * THREADS + tid, row = p >> 2, c = (p & 3) ^ i8_swz(row);
-    ws[j] = g.w + (long)min(n0 + row, g.N - 1) * g.ldw + c * 16;   // their outputs are not stored
+    wo[j] = (unsigned)min(row, g.N - 1 - n0) * (unsigned)g.ldw + c * 16;
     wk[j] = c * 16;
   }
-  auto issue = [&](int t, int slot) {
+  const auto issue = [&](int t, int slot, bool whole) {
     unsigned char* st = i8_lds + slot * STAGE + wave * 1024;
     const int k0 = t * I8_BK;
+    const int8_t* xk = xb + k0;
+    const int8_t* wp = wb + k0;
 #pragma unroll
-    for (int j = 0; j < XJ; ++j) i8_glds16(xs[j] + k0, st + j * (THREADS * 16));
+    for (int j = 0; j < XJ; ++j) i8_glds16(xk + xo[j], st + j * (THREADS * 16));
+    if (whole || k0 + I8_BK <= g.K) {
 #pragma unroll
-    for (int j = 0; j < WJ; ++j)   // pieces past the weights' row (the tokens are zero there) come from the block of zeros
-      i8_glds16(k0 + wk[j] < g.K ? (const void*)(ws[j] + k0) : (const void*)g.zeros, st + XB + j * (THREADS * 16));
+      for (int j = 0; j < WJ; ++j) i8_glds16(wp + wo[j], st + XB + j * (THREADS * 16));
+    } else {   // pieces past the weights' row (the tokens are zero there) come from the block of zeros
+#pragma unroll
+      for (int j = 0; j < WJ; ++j)
+        i8_glds16(k0 + wk[j] < g.K ? (const void*)(wp + wo[j]) : (const void*)g.zeros, st + XB + j * (THREADS * 16));
+    }
   };
 
   const unsigned base = (unsigned)reinterpret_cast<size_t>((__attribute__((address_space(3))) unsigned char*)i8_lds);
@@ -402,27 +529,44 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void int8_tile_kernel(const Int8
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
 
-  const int T = (int)(g.ldq / I8_BK);
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s)
-    if (s < T) issue(s, s);
-  int slot = 0;
-  for (int t = 0; t < T; ++t) {
-    // stage t has landed when the instructions of the stages behind it are all that is left
-    const int behind = min(T - 1 - t, STAGES - 2);
-    if (behind == STAGES - 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * D) : "memory");
+  // Stages land in order: the oldest has when the instructions of the `behind` stages after it are all that is left.
+  const auto landed = [&](int behind) {
+    if (behind == STAGES - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * D) : "memory");
+    else if (behind == STAGES - 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * D) : "memory");
     else if (behind >= 2 && STAGES > 4) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * D) : "memory");
     else if (behind >= 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(D) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();   // everyone's has, and everyone is done with stage t - 1
-    if (t + STAGES - 1 < T) issue(t + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
-    const unsigned st = (unsigned)(slot * STAGE);
+  };
+  const int T = (int)(g.ldq / I8_BK);
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) i8_step<TM, TN>(xa[ks] + st, wa[ks] + st, acc);
+  for (int s = 0; s < STAGES; ++s)
+    if (s < T) issue(s, s, false);
+  landed(min(T, STAGES) - 1);
+  __builtin_amdgcn_s_barrier();
+  I8Frag<TM, TN> even, odd;
+  i8_read<TM, TN>(even, xa[0], wa[0]);
+  int slot = 0, t = 0;
+  // one stage: its second half is read under the first one's products, the next stage's first half under the second's
+  const auto turn = [&](auto steady) {
+    const unsigned st = (unsigned)(slot * STAGE);
+    i8_step<TM, TN>(acc, even, odd, xa[1] + st, wa[1] + st);
+    if constexpr (decltype(steady)::value) landed(STAGES - 2);
+    else landed(min(T - 2 - t, STAGES - 2));
+    __builtin_amdgcn_s_barrier();   // everyone's stage t + 1 has landed, and everyone has read stage t
+    if constexpr (decltype(steady)::value) issue(t + STAGES, slot, true);
+    else if (t + STAGES < T) issue(t + STAGES, slot, false);
     slot = slot == STAGES - 1 ? 0 : slot + 1;
-  }
+    const unsigned sn = (unsigned)(slot * STAGE);
+    i8_step<TM, TN>(acc, odd, even, xa[0] + sn, wa[0] + sn);
+    ++t;
+  };
+  const int whole = g.K / I8_BK - STAGES;
+  while (t < whole) turn(std::true_type());   // nothing to decide
+  do turn(std::false_type()); while (t + 1 < T);   // T is at least 2: rows of tokens are whole multiples of two stages
+  i8_step<TM, TN>(acc, even, odd, xa[1] + (unsigned)(slot * STAGE), wa[1] + (unsigned)(slot * STAGE));
+  i8_last<TM, TN>(acc, odd);
   __syncthreads();   // the ring becomes the waves' output images
-  i8_write_tile<OUT_BF16, TM, TN>(g, acc, i8_lds + wave * IMG, m0 + wm * 32 * TM, n0 + wn * 32 * TN, lane);
+  i8_write_tile<OUT_BF16, TM, TN>(g, scales, acc, i8_lds + wave * IMG, m0 + wm * 32 * TM, n0 + wn * 32 * TN, lane);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -598,9 +742,9 @@ int i8_launch_tile(Int8Args& g, hipStream_t st) {
 template <bool YB>
 int i8_launch_tiles(Int8Args& g, hipStream_t st) {
   // 256 x 256 tiles, one workgroup of eight waves per CU, once they nearly fill the chip (12608 x 768 x 2304: 450 tiles,
-  // 49 us with the quantiser against 62 us on 128 x 128; 2048 x 4096 x 4096: 128 tiles, 66 against 58 us); 128 x 128
-  // tiles, two workgroups per CU, down to one for each CU (1920 x 768 x 2304: 270 tiles, 17 us against 21 us on 64 x 64;
-  // 500 x 4096 x 1024: 32 tiles, 34 against 25 us); then 64 x 64 in a ring twice as deep, where few workgroups have to
+  // 37 us against 42 us on 128 x 128; 2048 x 4096 x 4096: 128 tiles, 54 against 49 us); 128 x 128 tiles, two
+  // workgroups per CU, down to one for each CU (1920 x 768 x 2304: 270 tiles, 13 us against 16.5 us on 64 x 64;
+  // 500 x 4096 x 1024: 32 tiles, 20 against 13 us); then 64 x 64 in a ring twice as deep, where few workgroups have to
   // hide the latency by themselves.
   const long t256 = (long)((g.M + 255) / 256) * ((g.N + 255) / 256), t128 = (long)((g.M + 127) / 128) * ((g.N + 127) / 128);
   if (t256 >= 144) return i8_launch_tile<YB, 4, 2, 2, 4, 4, 2>(g, st);
