@@ -215,3 +215,16 @@ def test_more_rows_than_an_int_holds(dev):
         ops.int8_linear(z.expand(2 ** 32 + 5, 1), w, s)
     with pytest.raises(ValueError, match="fit"):
         ops.int8_linear(z, w.expand(2 ** 32 + 5, 1), s)
+
+
+def test_weight_rows_far_apart(dev):
+    """Rows of weights whose offsets inside one tile pass 32 bits."""
+    from vqa_amd import ops
+    N, K, pitch = 160, 200, 1 << 25
+    w, s = ops.quantize_rows(_x(N, K, torch.float32, 1).to(dev))
+    buf = torch.empty(N * pitch, dtype=torch.int8, device=dev)
+    far = buf.as_strided((N, K), (pitch, 1))
+    far.copy_(w)
+    for M in (3, 40, 70, 20000, 37000):   # the last ones on 128 x 128 and 256 x 256 tiles
+        x = _x(M, K, torch.bfloat16, M).to(dev)
+        assert torch.equal(ops.int8_linear(x, far, s), ops.int8_linear(x, w, s))

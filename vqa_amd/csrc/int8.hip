@@ -481,7 +481,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void int8_tile_kernel(const Int8
   // rows past the edge repeat the last one, and their outputs are not stored
   const int8_t* xb = g.q + (long)m0 * g.ldq;
   const int8_t* wb = g.w + (long)n0 * g.ldw;
-  unsigned xo[XJ], wo[WJ];
+  unsigned xo[XJ];   // (tokens were laid out here: at most 256 rows of 128 KB)
+  size_t wo[WJ];
   int wk[WJ];
 #pragma unroll
   for (int j = 0; j < XJ; ++j) {
@@ -491,7 +492,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void int8_tile_kernel(const Int8
 #pragma unroll
   for (int j = 0; j < WJ; ++j) {
     const int p = j * THREADS + tid, row = p >> 2, c = (p & 3) ^ i8_swz(row);
-    wo[j] = (unsigned)min(row, g.N - 1 - n0) * (unsigned)g.ldw + c * 16;
+    wo[j] = (size_t)min(row, g.N - 1 - n0) * (size_t)g.ldw + c * 16;
     wk[j] = c * 16;
   }
   const auto issue = [&](int t, int slot, bool whole) {
