@@ -228,3 +228,16 @@ def test_weight_rows_far_apart(dev):
     for M in (3, 40, 70, 20000, 37000):   # the last ones on 128 x 128 and 256 x 256 tiles
         x = _x(M, K, torch.bfloat16, M).to(dev)
         assert torch.equal(ops.int8_linear(x, far, s), ops.int8_linear(x, w, s))
+
+
+@pytest.mark.parametrize("M,N", [(130, 100), (2000, 2000), (4609, 1800)])
+def test_every_number_of_stages(dev, M, N):
+    """Short and long contractions on each tile size: the ring's start, its steady turns and its end, whole and partial
+    last stages.  The integer sum stays below 2^24, so two f32 products are all that follows it."""
+    from vqa_amd import ops
+    for K in (1, 63, 64, 65, 127, 128, 129, 192, 255, 256, 257, 319, 320, 321, 384, 449, 512, 576, 577, 640, 704, 769, 1000):
+        x, w = _x(M, K, torch.bfloat16, K).to(dev), _x(N, K, torch.float32, K + 1).to(dev)
+        q, sx = ops.quantize_rows(x)
+        wq, sw = ops.quantize_rows(w)
+        want = (q.double() @ wq.double().t()).float() * sx[:, None] * sw
+        assert torch.equal(ops.int8_linear(x, wq, sw, out_dtype=torch.float32), want), K
