@@ -158,32 +158,45 @@ def distill(logits, teacher, indices, temperature=1.0, tail=False):
     loss = torch.where(q > 0, q * (v - lpk), 0.0).sum(1)
     mass = q.sum(1)
     rest = torch.zeros(R, dtype=torch.float64)
-    held = torch.ones(R, dtype=torch.float64)
     outside = torch.ones(R, C, dtype=torch.float64)
     outside = torch.where(torch.zeros(R, C, dtype=torch.float64).scatter_add_(1, at, live.double()) > 0, 0.0, outside)
-    held_bound = torch.zeros(R, dtype=torch.float64)
+    shared = torch.zeros(R, C, dtype=torch.float64)   # rest times each class's share of what the list leaves
+    t_out, held_bound = t, torch.zeros(R, dtype=torch.float64)
     if tail:
         rest = 1.0 - mass
         some = (rest > 2.0 ** -20) & (outside.sum(1) > 0) & live.any(1)
         rest = torch.where(some, rest, 0.0)
-        held = (p * outside).sum(1)
-        share = p * outside / held.clamp_min(1e-300)[:, None]
-        held_bound = (2 * (share * t).sum(1) + 6) * U
-        loss = loss + torch.where(some, rest * (torch.log(rest) - torch.log(held)), 0.0)
-    cut = torch.where((rest > 0) & (held > 0), rest / held.clamp_min(1e-300), 0.0)
+        # relative to their own maximum, and in logarithms: what the student leaves outside the list may lie below every
+        # number
+        x = logits.double()
+        xo = torch.where(outside > 0, x, -math.inf)
+        mo = torch.where(torch.isnan(xo), -math.inf, xo).amax(1, keepdim=True)
+        zo = (xo - torch.where(mo == -math.inf, 0.0, mo)) / temperature
+        so = torch.exp(zo).sum(1, keepdim=True)
+        share = torch.where(so > 0, torch.exp(zo) / so, 0.0)
+        held = (mo - m)[:, 0] / temperature + torch.log(so[:, 0]) + lp.amax(1)   # (the largest is -log S)
+        t_out = torch.where(share > 0, zo.abs() / math.log(2.0), 0.0)
+        held_bound = (2 * (share * t_out).sum(1) + 10) * U
+        loss = loss + torch.where(some, rest * (torch.log(rest) - held), 0.0)
+        shared = rest[:, None] * share
     total = mass + rest
-    slope = total[:, None] - cut[:, None] * outside
-    slope = torch.where((outside > 0) & ((rest > 0) & (held == 0))[:, None], 0.0, slope)
-    g = p * slope - target
+    g = p * total[:, None] - shared - target
     tol_s = sum_bound(p, t)
     loss_tol = total * tol_s + rest * (held_bound + tol_s) + 2.0 ** -36 * (1 + (q * v.clamp_min(-1e3).abs()).sum(1))
     # rounding to f32 once, and the f32 of a row that a mean reads
     t2 = temperature * temperature
     loss, loss_tol = loss * t2, loss_tol * t2 + 2 * U * (loss * t2).abs()
-    # p as above; slope and mass to f32; q to f32, summed where an answer is named again, subtracted, scaled
-    tol = p * slope.abs() * ((2 * t + 10) * U + tol_s[:, None])
-    tol = tol + p * cut[:, None] * outside * (held_bound + tol_s + 2 * U)[:, None] + target * 140 * U
-    tol = tol + FLUSH * slope.abs()
+    loss = torch.where(loss > torch.finfo(torch.float32).max, math.inf, loss)
+    # on the list, or without a tail: p as above, mass to f32; q to f32, summed where an answer is named again, subtracted,
+    # scaled
+    off = outside if tail else torch.zeros_like(outside)
+    tol = (1.0 - off) * p * total[:, None] * ((2 * t + 10) * U + tol_s[:, None]) + target * 140 * U
+    # elsewhere one exponential times one factor, the difference of the two parts' factors, formed in 64 bits: the
+    # exponential is off by its argument's difference, factor and product, 3 ln2 |t| u (2 |t| u and, as it is 0 past
+    # |t| = 126, another 10 u), the factor by what its two sums are, and as f32
+    tol = tol + off * ((p * total[:, None] - shared).abs() * (2 * t_out + 20) * U
+                       + (p * total[:, None]) * (tol_s + 2 * U)[:, None] + shared * (held_bound + 2 * U)[:, None])
+    tol = tol + FLUSH * (total + rest)[:, None]
     g, tol = g * temperature, tol * temperature + 4 * U * (g * temperature).abs()
     none = ~live.any(1)
     loss, loss_tol = torch.where(none, 0.0, loss), torch.where(none, 0.0, loss_tol)

@@ -3,6 +3,11 @@
 // r that no answer of the list holds, z = x / T, e_j = exp(z_j - max z), S = sum_j e_j, p_j = e_j / S:
 //   L = T^2 [ sum_k q_k (log q_k - log p_{i_k}) + r (log r - log P) ],     P = sum of p_j outside the list
 //   dL / dx_j = T [ p_j (sum q + r) - sum_{k: i_k = j} q_k ] on the list,  T p_j [ sum q + r - r / P ] elsewhere.
+// P may lie below every number where the student leaves next to nothing outside the list (a mask of -500, a small
+// temperature), and r / P above, so neither is formed: with e'_j = exp(z_j - m'), m' the largest z outside the list and S'
+// the sum of e' there,
+//   log P = m' - max z + log S' - log S,     dL / dx_j = T e'_j [ (sum q + r) exp(m' - max z) / S - r / S' ]  elsewhere,
+// where S and S' are at least 1 and the bracket lies between -1 and 1.
 // Rows are held and walked as in answers.hip; the gradient for an incoming gradient of 1 leaves from the same read.
 //
 // Precision.  The divergence of two close distributions is a small difference of large terms, so the list's terms, the
@@ -17,10 +22,13 @@ namespace {
 // ---------------------------------------------------------------------------------------------
 // Distillation loss, with the gradient of the sum (or mean) in the same pass
 // ---------------------------------------------------------------------------------------------
-// (R,5) f64: m, S, mass = sum q + r, slope = mass - r / P, log Q (q_k = exp(v_k - log Q))
+// 40 bytes a row: the row's largest logit, the one that `slope` goes with (tail: the largest outside the list; 0 where that
+// is -inf), S, mass = sum q + r, slope: the bracket above (no tail: mass / S), log Q (q_k = exp(v_k - log Q))
 struct DistillStat {
-  double m, S, mass, slope, log_q;
+  float m, m_out;
+  double S, mass, slope, log_q;
 };
+static_assert(sizeof(DistillStat) == 40, "five f64 a row");
 
 // a row that is all masked, or that no answer teaches (whatever its logits hold)
 __device__ __forceinline__ bool an_no_gradient(const DistillStat& s) {
@@ -36,8 +44,7 @@ struct DistillGrad {
   float scale;         // T * (1 for a sum, 1 / R for a mean)
   AnTemp temp;
   struct Row {
-    float m, mass, slope, hi, lo, g;
-    double log_q;
+    float m, m_out, mass, slope, hi, lo, g;
     bool empty;
   };
   __device__ __forceinline__ bool done() const { return skip_unit && up[0] == 1.0f; }
@@ -50,18 +57,18 @@ struct DistillGrad {
   __device__ __forceinline__ Row row(long r, int, int) const {
     Row w;
     const DistillStat s = stats[r];
-    w.m = (float)s.m;
+    w.m = s.m;
+    w.m_out = s.m_out;
     w.empty = an_no_gradient(s);
-    const double inv = w.empty ? 0.0 : 1.0 / s.S;
-    w.mass = (float)(s.mass * inv);
-    w.slope = (float)(s.slope * inv);
+    w.mass = (float)(s.mass / s.S);
+    w.slope = (float)s.slope;
     w.hi = temp.hi;
     w.lo = temp.lo;
     w.g = scale * up[r * up_step];
     return w;
   }
   static __device__ __forceinline__ float dense(const Row& w, float x) {
-    return w.empty ? 0.f : w.g * (an_exp2(an_arg(x, w.m, w.hi, w.lo)) * w.slope);
+    return w.empty ? 0.f : w.g * (an_exp2(an_arg(x, w.m_out, w.hi, w.lo)) * w.slope);
   }
   static __device__ __forceinline__ float base(const Row& w, float x) {
     return w.empty ? 0.f : w.g * (an_exp2(an_arg(x, w.m, w.hi, w.lo)) * w.mass);
@@ -90,24 +97,38 @@ struct DistillList {
   int idx[AN_TOP_MAX], again[AN_TOP_MAX];
 };
 
-// One wave: the row's statistics and loss from the sum of e over the classes outside the list (s_out) or, without a tail,
-// over all of them (s_all).  `all`: the list covers every class; `bad`: an answer lies past the classes.
-// Short loops on purpose: the pieces of the row are alive around this.
-__device__ __forceinline__ DistillStat an_distill_row(DistillList& list, int K, bool bad, float m, double s_all, double s_out,
-                                                      bool all, bool tail, double inv_t, double& loss) {
+// One wave: the row's statistics and loss.  m_dense, s: the largest logit of the classes outside the list (tail) or of all
+// of them, and the sum of exp((x - m_dense) / T) over those, relative to 0 where m_dense is -inf.  `all`: the list covers
+// every class; `bad`: an answer lies past the classes.  Short loops on purpose: the pieces of the row are alive around this.
+__device__ __forceinline__ DistillStat an_distill_row(DistillList& list, int K, bool bad, float m_dense, double s, bool all,
+                                                      bool tail, double inv_t, double& loss) {
   const int lane = threadIdx.x & 63;
-  const bool empty = m == -INFINITY;
   DistillStat st;
-  st.m = m;
-  st.S = s_all;
+  st.m = m_dense;
+  st.m_out = m_dense;
+  st.S = s;
   st.log_q = 0.0;
+  double part = 1.0;   // exp((m_dense - m) / T)
   bool some = true;
   if (tail) {
+    float top = -INFINITY;
+    bool nan = false;
+#pragma unroll 1
+    for (int k = lane; k < K; k += 64) {
+      if (list.idx[k] < 0) continue;
+      top = fmaxf(top, list.x[k]);
+      nan |= list.x[k] != list.x[k];
+    }
+    st.m = fmaxf(m_dense, dpp_wave_max(top));
+    // (maxima leave NaN out: a row of nothing else but -inf is not empty)
+    if (st.m == -INFINITY && (s != s || __ballot(nan) != 0)) st.m = NAN;
+    if (m_dense == -INFINITY) st.m_out = 0.f;
+    else part = an_exp(((double)m_dense - (double)st.m) * inv_t);
     double own = 0.0;
 #pragma unroll 1
     for (int k = lane; k < K; k += 64)
-      if (list.idx[k] >= 0 && !list.again[k]) own += an_exp(((double)list.x[k] - (double)m) * inv_t);
-    st.S = s_out + dpp_wave_sum(own);
+      if (list.idx[k] >= 0 && !list.again[k]) own += an_exp(((double)list.x[k] - (double)st.m) * inv_t);
+    st.S = s * part + dpp_wave_sum(own);
   } else {
     float vm = -INFINITY;
     bool nan = false;
@@ -127,6 +148,7 @@ __device__ __forceinline__ DistillStat an_distill_row(DistillList& list, int K, 
       st.log_q = (double)vm + log(dpp_wave_sum(sum));
     }
   }
+  const bool empty = st.m == -INFINITY;
   const double log_s = log(st.S);
   double mass = 0.0, l = 0.0;
   bool any = false;
@@ -135,7 +157,7 @@ __device__ __forceinline__ DistillStat an_distill_row(DistillList& list, int K, 
     const bool live = list.idx[k] >= 0;
     const double lq = (double)list.v[k] - st.log_q;
     const double q = live && some ? an_exp(lq) : 0.0;
-    const double lp = empty ? -INFINITY : ((double)list.x[k] - (double)m) * inv_t - log_s;
+    const double lp = empty ? -INFINITY : ((double)list.x[k] - (double)st.m) * inv_t - log_s;
     any |= live;
     mass += q;
     if (q != 0.0) l += q * (lq - lp);   // (NaN goes in)
@@ -143,18 +165,17 @@ __device__ __forceinline__ DistillStat an_distill_row(DistillList& list, int K, 
   }
   mass = dpp_wave_sum(mass);
   l = dpp_wave_sum(l);
-  double cut = 0.0;
+  double cut = 0.0;   // r / S'
   if (tail) {
     double rest = all || __ballot(any) == 0 ? 0.0 : 1.0 - mass;   // (a row without answers teaches nothing)
     if (!(rest > (double)AN_NO_REST)) rest = 0.0;
     mass += rest;
     if (rest > 0.0) {
-      if (empty) {
+      if (empty || s == 0.0) {   // nothing outside: met with probability 0, and no logit there to change
         l += INFINITY;
       } else {
-        const double P = s_out / st.S;
-        l += rest * (log(rest) - log(P));
-        cut = P > 0.0 ? rest / P : (P == 0.0 ? mass : P);
+        l += rest * (log(rest) - (((double)st.m_out - (double)st.m) * inv_t + log(s) - log_s));
+        cut = rest / s;
       }
     }
   } else if (some) {
@@ -162,7 +183,7 @@ __device__ __forceinline__ DistillStat an_distill_row(DistillList& list, int K, 
   }
   if (bad) l = mass = NAN;
   st.mass = mass;
-  st.slope = mass - cut;
+  st.slope = mass == 0.0 ? 0.0 : mass * part / st.S - cut;
   loss = l;
   return st;
 }
@@ -173,7 +194,7 @@ struct DistillShared {
   float s_max[NT / 64];
   double s_sum[2][NT / 64];
   int bad, repeats, none;
-  float mass, slope;   // over S, the slope times the gradient's scale
+  float mass, slope;   // over S; times the gradient's scale
 };
 
 // The elements of a piece whose bits are set become -inf.
@@ -239,6 +260,7 @@ __global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs 
 #pragma unroll
   for (int i = 1; i < NW; ++i) m = fmaxf(m, sh.s_max[i]);
   if (m == -INFINITY && an_block_nan<BF16, NT>(row.s)) m = NAN;
+  const float from = TAIL && m == -INFINITY ? 0.f : m;
 
   // Sums of e = 2^t and of e t; TAIL: over the classes outside the list.  One factor only: what its rounding shifts is taken
   // out of the sum below, to first order.
@@ -248,7 +270,7 @@ __global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs 
     float w = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float t = (e[j] - m) * hi;
+      const float t = (e[j] - from) * hi;
       e[j] = an_exp2(t);
       w = fmaf(e[j], an_floor(t), w);
     }
@@ -303,14 +325,13 @@ __global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs 
     S -= a.temp.delta * AN_LN2 * Wt;
     double loss;
     // (more than 1024 classes and at most 128 answers: never all of them)
-    const DistillStat st = an_distill_row(sh.list, a.K, sh.bad != 0, m, S, S, false, TAIL, a.temp.inv_t, loss);
+    const DistillStat st = an_distill_row(sh.list, a.K, sh.bad != 0, m, S, false, TAIL, a.temp.inv_t, loss);
     if (lane == 0) {
       a.row_loss[r] = (float)(a.t2 * loss);
       if (a.stats != nullptr) a.stats[r] = st;
       sh.none = an_no_gradient(st) ? 1 : 0;
-      const double inv = sh.none ? 0.0 : 1.0 / st.S;
-      sh.mass = (float)(st.mass * inv);
-      sh.slope = (float)(st.slope * inv) * a.scale;
+      sh.mass = (float)(st.mass / st.S);
+      sh.slope = (float)st.slope * a.scale;
     }
   }
   if (a.grad == nullptr) return;   // uniform
@@ -382,36 +403,39 @@ __global__ __launch_bounds__(64 * AN_WAVES) void distill_wave_kernel(const Disti
     list.again[k] = again;
   }
   const bool bad = __ballot(beyond) != 0, repeats = __ballot(named_again) != 0;
-  float m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < E; ++i) m = fmaxf(m, v[i]);
-  m = an_wave_row_max<E>(v, m);
   __builtin_amdgcn_wave_barrier();
   __threadfence_block();
-  double S = 0.0;   // tail: over the classes outside the list
   int outside = 0;
-  float e32[E];
+  float m = -INFINITY;   // tail: of the classes outside the list
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const int c = lane + 64 * i;
-    const double e = an_exp(((double)v[i] - (double)m) * a.temp.inv_t);
-    e32[i] = (float)e;
     const bool in = (mark[c >> 5] >> (c & 31)) & 1u;   // E <= 16: c < 1024
-    S += a.tail && in ? 0.0 : e;
     outside += c < a.C && !in ? 1 : 0;
+    if (a.tail && in) v[i] = -INFINITY;   // (their gradients are written by name)
+    m = fmaxf(m, v[i]);
+  }
+  m = a.tail ? dpp_wave_max(m) : an_wave_row_max<E>(v, m);
+  const double from = a.tail && m == -INFINITY ? 0.0 : (double)m;
+  double S = 0.0;
+  float e32[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const double e = an_exp(((double)v[i] - from) * a.temp.inv_t);
+    e32[i] = (float)e;
+    S += e;
   }
   S = dpp_wave_sum(S);
   const bool all = __ballot(outside != 0) == 0;
   double loss;
-  const DistillStat st = an_distill_row(list, a.K, bad, m, S, S, all, a.tail != 0, a.temp.inv_t, loss);
+  const DistillStat st = an_distill_row(list, a.K, bad, m, S, all, a.tail != 0, a.temp.inv_t, loss);
   if (lane == 0) {
     a.row_loss[r] = (float)(a.t2 * loss);
     if (a.stats != nullptr) a.stats[r] = st;
   }
   if (a.grad == nullptr) return;
   const bool none = an_no_gradient(st);
-  const double inv = none ? 0.0 : 1.0 / st.S;
-  const float mass = (float)(st.mass * inv), slope = (float)(st.slope * inv) * a.scale;
+  const float mass = (float)(st.mass / st.S), slope = (float)st.slope * a.scale;
   unsigned char* grow = reinterpret_cast<unsigned char*>(a.grad) + r * a.ldg * (BF16 ? 2 : 4);
 #pragma unroll
   for (int i = 0; i < E; ++i) {
@@ -422,7 +446,7 @@ __global__ __launch_bounds__(64 * AN_WAVES) void distill_wave_kernel(const Disti
   __builtin_amdgcn_wave_barrier();
   const float sc = a.scale;
   an_write_named<BF16>(list.idx, list.q, a.K, repeats, lane, 64, 0, a.C, xr, grow,
-                       [&](float x) { return none ? 0.f : sc * ((float)an_exp(((double)x - (double)m) * a.temp.inv_t) * mass); },
+                       [&](float x) { return none ? 0.f : sc * ((float)an_exp(((double)x - (double)st.m) * a.temp.inv_t) * mass); },
                        [&](float t) { return none ? 0.f : -sc * t; });
 }
 
