@@ -739,8 +739,8 @@ int vqaf_token_logprobs_bwd(const void* logits, long ld, const int64_t* targets,
  * f32: the teacher's log probabilities AT THE TEMPERATURE of the answers indices (R,K) int64 (top_logprobs /
  * top_indices of vqaf_token_logprobs); a negative index is no answer, one past the classes makes its row NaN.
  * q_k = exp(teacher_k), divided by their sum (tail 0) or as they are with the remaining mass r = 1 - sum q as one more
- * event, met by all classes outside the list together (tail 1; r <= 2^-20 is taken for the rounding it is, and a list
- * of all classes or of none has no rest).  p = softmax(x / temperature):
+ * event, met by all classes outside the list together, however little p leaves there (tail 1; r <= 2^-20 is taken for
+ * the rounding it is, and a list of all classes or of none has no rest).  p = softmax(x / temperature):
  *   row_loss = temperature^2 [ sum_k q_k (log q_k - log p_{i_k}) + r (log r - log sum_{j outside} p_j) ].
  * row_loss (R) f32.  grad, if non-NULL, receives scale * d(sum of rows)/dx in `dtype` (layout as above), formed from
  * the same read of the logits.  loss, if non-NULL, receives scale * sum of rows, added in a fixed order.  stats (R,5)

@@ -11,7 +11,7 @@ from test_gpu_answers import _check_distill, _close
 pytestmark = pytest.mark.gpu
 
 DTYPES = [torch.bfloat16, torch.float32]
-CLASSES = [17, 430, 1024]   # a wave to a row
+SHORT, LONG = [17, 430, 1024], [1025, 30522, 50265, 70001]   # a wave to a row, a workgroup to a row
 
 
 @pytest.fixture(scope="module")
@@ -44,7 +44,7 @@ def _rows(C, gap, T, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T", [0.25, 1.0, 2.0 ** -12])
 @pytest.mark.parametrize("gap", [-95, 60, 80, 87, 95, 100, 110, 300, 800])
-@pytest.mark.parametrize("C", CLASSES)
+@pytest.mark.parametrize("C", SHORT + LONG)
 def test_rest_far_below_the_list(dev, C, gap, T, dtype):
     x, v, idx = _rows(C, gap, T, dtype)
     loss, _, g, _ = ao.distill(x, v, idx, T, True)
@@ -54,7 +54,7 @@ def test_rest_far_below_the_list(dev, C, gap, T, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("C", [430])
+@pytest.mark.parametrize("C", [SHORT[1], LONG[1]])
 def test_rest_masked_by_large_numbers(dev, C, dtype):
     """Masks of -500, -1e4 and the type's lowest value in the place of -inf: the rest is shared by what they leave equal."""
     T = 0.5
@@ -66,7 +66,7 @@ def test_rest_masked_by_large_numbers(dev, C, dtype):
     _check_distill(x, x.to(dev), v, idx, T, True, dev)
 
 
-@pytest.mark.parametrize("C", [17, 430])
+@pytest.mark.parametrize("C", [SHORT[1], LONG[0], LONG[3]])
 def test_rest_of_rows_that_hold_no_numbers(dev, C):
     """NaN and infinities on either side of the list, alone and with everything else masked."""
     x, v, idx = _rows(C, 100, 1.0, torch.float32)
@@ -94,7 +94,7 @@ def test_rest_of_rows_that_hold_no_numbers(dev, C):
     _check_distill(x, x.to(dev), v, idx, 1.0, True, dev)
 
 
-@pytest.mark.parametrize("C", [11, 430])
+@pytest.mark.parametrize("C", [11, 430, 1500])
 def test_gradient_against_differences(dev, C):
     """Central differences of the 64-bit definition, a hundred temperatures between the list and the rest."""
     from vqa_amd import ops
@@ -119,7 +119,7 @@ def test_gradient_against_differences(dev, C):
 def test_replayed_graph_and_second_stream(dev):
     """The loss and both of its backward passes captured once, replayed on new rows, and beside another stream's."""
     from vqa_amd import ops
-    for C in (430, 1000):
+    for C in (430, 30522):
         x, v, idx = _rows(C, 100, 1.0, torch.float32)
         xs = [x.to(dev), _rows(C, 300, 1.0, torch.float32)[0].to(dev), x.flip(0).to(dev)]
         vd, idxd = v.to(dev), idx.to(dev)

@@ -207,19 +207,33 @@ struct RowPieces {
   }
   // The thread's largest value; NaN counts as the largest or not at all.
   __device__ __forceinline__ float max() const {
+    return max_of([](const u32x4 r, int) { return r; });
+  }
+  // ... of the pieces as f(r, c) leaves them
+  template <class F>
+  __device__ __forceinline__ float max_of(F f) const {
     if constexpr (BF16) {
       unsigned k = 0x80008000u;   // the lowest pair
-      walk_raw([&](const u32x4 r, int, int) { k = an_pkmax(k, an_pkmax(an_pkmax(r.x, r.y), an_pkmax(r.z, r.w))); });
+      walk_raw([&](const u32x4 p, int c, int) {
+        const u32x4 r = f(p, c);
+        k = an_pkmax(k, an_pkmax(an_pkmax(r.x, r.y), an_pkmax(r.z, r.w)));
+      });
       const int b = an_pkmax1(k);
       if (b >= 0) return __uint_as_float((unsigned)b << 16);
       k = 0xff80ff80u;            // -inf
-      walk_raw([&](const u32x4 r, int, int) { k = an_pkmin(k, an_pkmin(an_pkmin(r.x, r.y), an_pkmin(r.z, r.w))); });
+      walk_raw([&](const u32x4 p, int c, int) {
+        const u32x4 r = f(p, c);
+        k = an_pkmin(k, an_pkmin(an_pkmin(r.x, r.y), an_pkmin(r.z, r.w)));
+      });
       return __uint_as_float(min(k & 0xffffu, k >> 16) << 16);
     } else {
       float m = -INFINITY;
-      walk([&](const float (&v)[V], int, int) {
+      walk_raw([&](const u32x4 p, int c, int) {
+        float v[V];
+        an_unpack<BF16>(f(p, c), v);
 #pragma unroll
         for (int j = 0; j < V; ++j) m = fmaxf(m, v[j]);
+        if constexpr (E > 0) __builtin_amdgcn_sched_barrier(0);   // as in walk
       });
       return m;
     }
