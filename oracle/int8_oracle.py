@@ -23,8 +23,8 @@ def quantize_rows(x: torch.Tensor):
 
 
 def linear(x, weight, weight_scale, bias=None, out_dtype=None):
-    """(y f64, bound).  Epilogue: the integer sum to f32, times the token's scale, a fused multiply-add with the
-    channel's scale and the bias: three roundings of the product and one of the result, then the output type."""
+    """(y f64, bound).  Epilogue: the integer sum to f32, times the token's scale, times the channel's, plus the bias: three
+    roundings of the product and one of the result, then the output type."""
     q, s = quantize_rows(x)
     prod = (q @ weight.double().t()) * s[:, None] * weight_scale.double()[None, :]
     y = prod if bias is None else prod + bias.double()

@@ -1,0 +1,62 @@
+"""Linear layers in eight-bit integers at the ends of the f32 range, and with scales that lie apart."""
+import math
+
+import pytest
+import torch
+
+from oracle import int8_oracle as io
+from test_gpu_int8 import _close
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available()
+    return torch.device("cuda:0")
+
+
+# tokens of one launch, of the few-token product and of every tile size
+@pytest.mark.parametrize("M,N", [(3, 40), (50, 40), (130, 100), (2000, 2000), (4609, 1800)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_tokens_near_the_end_of_the_range(dev, M, N, dtype):
+    """The sum times the token's scale may lie past the f32 range where the channel's scale brings it back."""
+    from vqa_amd import ops
+    K = 96
+    g = torch.Generator().manual_seed(M)
+    x = torch.randn(M, K, generator=g).abs() + 0.5                 # sums of one sign: up to 2^20
+    w = (torch.randn(N, K, generator=g).abs() + 0.5) * 1e-6
+    big = torch.finfo(dtype).max / float(x.abs().amax()) / 2
+    rows = torch.arange(M) % 3
+    x[rows == 0] *= big
+    x[rows == 1] *= 2.0 ** 101                                     # scales to both sides of 2^96
+    x = x.to(dtype)
+    w[N // 2] *= 1e-30                                             # a channel of tiny weights
+    w[N - 1] *= 1e20                                               # ... and of ones whose outputs are infinite
+    wq, ws = ops.quantize_rows(w.to(dev))
+    bias = torch.linspace(-1, 1, N)
+    for b in (bias, None):
+        y = ops.int8_linear(x.to(dev), wq, ws, None if b is None else b.to(dev), out_dtype=torch.float32).cpu()
+        want, tol = io.linear(x, wq.cpu(), ws.cpu(), b, torch.float32)
+        far = want.abs() > torch.finfo(torch.float32).max
+        near = (want.abs() * (1 - 2.0 ** -20) <= torch.finfo(torch.float32).max) & \
+               (want.abs() * (1 + 2.0 ** -20) >= torch.finfo(torch.float32).max)
+        assert bool(far.any()) and not bool(far[:, 0].any())
+        assert bool(torch.isinf(y[far & ~near]).all())
+        ok = ~far & ~near
+        _close(y[ok], want[ok], tol[ok], f"{M} {N}")
+
+
+def test_rows_do_not_depend_on_their_neighbours(dev):
+    """A row of large numbers in a tile changes no other row's bits."""
+    from vqa_amd import ops
+    for M, N, K in ((4, 40, 96), (50, 40, 96), (130, 100, 200), (2000, 2000, 130), (4609, 1800, 64)):
+        g = torch.Generator().manual_seed(M)
+        x = torch.randn(M, K, generator=g)
+        wq, ws = ops.quantize_rows(torch.randn(N, K, generator=g).to(dev))
+        bias = torch.linspace(-1, 1, N, device=dev)
+        want = ops.int8_linear(x.to(dev), wq, ws, bias)
+        x[1] *= 1e37
+        got = ops.int8_linear(x.to(dev), wq, ws, bias)
+        keep = torch.arange(M) != 1
+        assert torch.equal(got[keep.to(dev)], want[keep.to(dev)])

@@ -4,7 +4,7 @@
 //   s_m = max(max_k |x_mk| / 127, 2^-126),   q_mk = round-half-even(x_mk / s_m),   y_mn = (sum_k q_mk w_nk) s_m s_n + b_n
 //
 // The sum is exact in 32-bit integers (127^2 K < 2^31 for K up to 131072); the two scales, the bias and the rounding to
-// the output type follow in f32, in the epilogue.  The quotient is rounded as if it were exact: next to a border the
+// the output type follow in f32, in the epilogue, without leaving its range on the way where the result does not.  The quotient is rounded as if it were exact: next to a border the
 // sign of x - (q +- 1/2) s, one fused multiply-add, decides.  A row with NaN or an infinity gets the scale NaN, which
 // makes its outputs NaN.
 //
@@ -220,6 +220,20 @@ __device__ __forceinline__ float i8_bias(const Int8Args& g, int n) {
   return g.bias_bf16 ? bf16_to_f32(reinterpret_cast<const bf16_t*>(g.bias)[n]) : reinterpret_cast<const float*>(g.bias)[n];
 }
 
+// One output from its integer sum, (sum * token's scale) * channel's scale + bias with a rounding each.  A scale from 2^96
+// on could carry the sum (below 2^31) past the f32 range before the channel's brings it back: of such a token 2^-64 goes
+// through the products, and `back` is the 2^64 that is missing (1 of any other).
+struct I8Token {
+  float scale, back;
+};
+__device__ __forceinline__ I8Token i8_token(float scale) {
+  const bool big = scale >= 0x1p96f;
+  return I8Token{big ? scale * 0x1p-64f : scale, big ? 0x1p64f : 1.f};
+}
+__device__ __forceinline__ float i8_output(int sum, const I8Token t, float channel, float bias) {
+  return fmaf((float)sum * t.scale * channel, t.back, bias);
+}
+
 // Scales and bias of a wave's tokens and channels, asked for before the product so that they are there after it: a lane
 // has those of token 32 i + (lane & 31) and channel 32 j + (lane & 31).  The bias comes as its two halves, whatever its
 // type, so that nothing is decided, and nothing awaited, before the product.
@@ -261,6 +275,9 @@ __device__ __forceinline__ void i8_write_tile(const Int8Args& g, const I8Scales<
     chan[j * 64 + 32 + (lane & 31)] = sc.bias(g, j);
   }
   asm volatile("" ::: "memory");
+  I8Token token[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) token[i] = i8_token(sc.x[i]);
 #pragma unroll
   for (int j = 0; j < TN; ++j) {   // in place: the sums become the outputs' bits
 #pragma unroll
@@ -271,7 +288,7 @@ __device__ __forceinline__ void i8_write_tile(const Int8Args& g, const I8Scales<
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          acc[i][j][4 * r + e] = __float_as_int(fmaf((float)acc[i][j][4 * r + e] * sc.x[i], sw[e], bv[e]));
+          acc[i][j][4 * r + e] = __float_as_int(i8_output(acc[i][j][4 * r + e], token[i], sw[e], bv[e]));
     }
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -664,11 +681,11 @@ __global__ __launch_bounds__(256) void int8_few_kernel(const Int8Args g, const v
     for (int w = 1; w < 4; ++w) t += s_part[w][b][lane];
     const int m = b * 16 + (lane & 15);
     if (m < g.M) {
-      const float sx = SELF ? s_scale[m < I8_SELF ? m : 0] : g.x_scale[m];
+      const I8Token token = i8_token(SELF ? s_scale[m < I8_SELF ? m : 0] : g.x_scale[m]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int n = n0 + 4 * (lane >> 4) + e;
-        if (n < g.N) store1<OUT_BF16>(g.y, (size_t)m * g.ldy + n, fmaf((float)t[e] * sx, g.w_scale[n], i8_bias(g, n)));
+        if (n < g.N) store1<OUT_BF16>(g.y, (size_t)m * g.ldy + n, i8_output(t[e], token, g.w_scale[n], i8_bias(g, n)));
       }
     }
   }
