@@ -60,3 +60,32 @@ def test_rows_do_not_depend_on_their_neighbours(dev):
         got = ops.int8_linear(x.to(dev), wq, ws, bias)
         keep = torch.arange(M) != 1
         assert torch.equal(got[keep.to(dev)], want[keep.to(dev)])
+
+
+def _next_to_borders(steps):
+    """Rows whose scale is an odd multiple of 2^-149 below 2^-125, of the values that f32 has next to the borders between
+    two steps: down to half a unit (2^-150) to either side."""
+    x = torch.zeros(len(steps), 254)
+    for r, k in enumerate(steps):                     # the scale is k 2^-149
+        border = [(2 * q + 1) * k // 2 for q in range(-63, 63)]          # (q + 1/2) k, rounded down
+        vals = [127 * k] + border + [b + 1 for b in border] + [0]
+        x[r] = torch.tensor(vals, dtype=torch.float64).mul(2.0 ** -149).float()
+    return x
+
+
+def test_borders_of_subnormal_steps(dev):
+    """The quotient is rounded as if it were exact also where half a step is no f32 number."""
+    from vqa_amd import ops
+    x = _next_to_borders([2 ** 23 + 1, 2 ** 23 + 7, 2 ** 23 + 12345, 2 ** 24 - 1, 2 ** 24 - 4321])
+    want_q, want_s = io.quantize_rows(x)
+    assert bool((want_s < 2.0 ** -125).all())
+    half = (x.double() / want_s[:, None]).abs() % 1 - 0.5
+    assert bool((half[:, 1:253] != 0).all()) and float(half[:, 1:253].abs().max()) < 2.0 ** -18    # next to a tie, never one
+    q, s = ops.quantize_rows(x.to(dev))
+    assert torch.equal(s.cpu().double(), want_s) and torch.equal(q.cpu().double(), want_q)
+    # one token quantised in the product's own launch
+    w = torch.eye(254, 256, dtype=torch.int8, device=dev)[:, :254]
+    ones = torch.full((254,), 2.0 ** 100, device=dev)
+    for m in range(x.shape[0]):
+        y = ops.int8_linear(x[m:m + 1].to(dev), w, ones)
+        assert torch.equal(torch.round(y.cpu().double() / (want_s[m] * 2.0 ** 100)), want_q[m:m + 1])

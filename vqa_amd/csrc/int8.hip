@@ -32,6 +32,10 @@ constexpr int I8_ROW = 128;   // rows of quantised tokens are whole multiples of
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ int i8_round(float x, float s, float inv) {
   float q = rintf(x * inv);
+  if (s < 0x1p-100f) {   // half a step may be finer than f32's smallest number: both 2^64 times as large, exactly
+    x *= 0x1p64f;
+    s *= 0x1p64f;
+  }
   const float up = fmaf(-(q + 0.5f), s, x), down = fmaf(-(q - 0.5f), s, x);   // exact signs
   const bool odd = ((int)q) & 1;
   if (up > 0.f || (up == 0.f && odd)) q += 1.f;
