@@ -89,3 +89,27 @@ def test_borders_of_subnormal_steps(dev):
     for m in range(x.shape[0]):
         y = ops.int8_linear(x[m:m + 1].to(dev), w, ones)
         assert torch.equal(torch.round(y.cpu().double() / (want_s[m] * 2.0 ** 100)), want_q[m:m + 1])
+
+
+@pytest.mark.parametrize("M", [3, 40, 200])
+def test_strided_scales(dev, M, monkeypatch):
+    """Scales that lie apart, while other allocations take whatever is free between the call's preparation and its launch
+    (another thread's, on the same stream)."""
+    from vqa_amd import ops
+    K, N = 100, 70
+    g = torch.Generator().manual_seed(M)
+    x = torch.randn(M, K, generator=g).to(dev)
+    wq, ws = ops.quantize_rows(torch.randn(N, K, generator=g).to(dev))
+    bias = torch.linspace(-1, 1, N, device=dev)
+    apart, wide = torch.stack([ws, ws + 1], 1)[:, 0], torch.stack([bias, bias], 1)[:, 1]
+    shared = ws[:1].expand(N)
+    want, want_shared = ops.int8_linear(x, wq, ws, bias), ops.int8_linear(x, wq, shared.contiguous(), bias)
+    real, taken = ops._launch, []
+
+    def launch(device, entry, *args):
+        taken.extend(torch.full((n,), math.nan, device=dev) for n in (N, N, 128, 128))
+        return real(device, entry, *args)
+    monkeypatch.setattr(ops, "_launch", launch)
+    assert not apart.is_contiguous() and not wide.is_contiguous() and not shared.is_contiguous()
+    assert torch.equal(ops.int8_linear(x, wq, apart, wide), want)
+    assert torch.equal(ops.int8_linear(x, wq, shared, bias), want_shared)

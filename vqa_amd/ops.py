@@ -1268,6 +1268,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     code = _lib.BF16 if dt == torch.bfloat16 else _lib.F32
     if dt not in (torch.float32, torch.bfloat16):
         raise TypeError(f"out_dtype has to be float32 or bfloat16, got {dt}")
+    weight_scale = weight_scale.contiguous()   # (a copy has to outlive the launch)
     if bias is not None:
         dtype_code(bias)
         bias = bias.contiguous()
@@ -1287,7 +1288,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         need = load().vqaf_int8_linear_workspace_bytes(M, K)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         _launch(x.device, "vqaf_int8_linear", x2.data_ptr(), ld, dtype_code(x2), weight.data_ptr(), ldw,
-                weight_scale.contiguous().data_ptr(), _addr(bias), dtype_code(bias) if bias is not None else 0, M, N, K,
+                weight_scale.data_ptr(), _addr(bias), dtype_code(bias) if bias is not None else 0, M, N, K,
                 y.data_ptr(), N, code, _addr(ws), need)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
