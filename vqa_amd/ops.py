@@ -10,6 +10,7 @@ import weakref
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -854,6 +855,14 @@ def _first_order(backward):
     return run
 
 
+def _has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a forward-mode derivative comes with any of them.  These operators have none: autograd's function refuses
+    it, so a tensor that carries one takes that way whether gradients are recorded or not."""
+    if getattr(forward_ad, "_current_level", 0) < 0:   # no level is open (asking a tensor costs 0.7 us)
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _answer_rows(logits: torch.Tensor):
     """(logits as (R,C) with unit inner stride, its row pitch)."""
     if logits.dim() < 1 or logits.shape[-1] < 1:
@@ -965,8 +974,8 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     logits (..., C) f32 or bf16.  targets (...) or (..., T) int64, at most 128 for each row: a negative one is none
     (log probability 0, no gradient), one past the classes gives NaN.  Results are f32 with the leading dimensions of
     `logits`; alternatives come in falling order, ties by the lowest index.  The log probabilities and the entropy are
-    differentiable.  Rows of nothing but -inf have log probabilities -inf, entropy 0 and no gradient; a NaN or +inf
-    makes its row NaN."""
+    differentiable, once and in reverse mode.  Rows of nothing but -inf have log probabilities -inf, entropy 0 and no
+    gradient; a NaN or +inf makes its row NaN."""
     x, ld = _answer_rows(logits)
     R, C = x.shape
     lead = logits.shape[:-1]
@@ -994,7 +1003,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
         ti = torch.empty((*lead, top), dtype=torch.int64, device=x.device) if top else None
         return TokenLogprobs(lp, ent, tl, ti)
     call = (ld, lead, T, top, temperature, bool(entropy))
-    if x.requires_grad and torch.is_grad_enabled():
+    if (x.requires_grad and torch.is_grad_enabled()) or _has_tangent(x):
         return TokenLogprobs(*_TokenLogprobs.apply(x, tg, call))
     return TokenLogprobs(*_logprobs_forward(x, tg, call, False)[:4])
 
@@ -1088,7 +1097,7 @@ def distill_loss(logits: torch.Tensor, teacher: torch.Tensor, indices: torch.Ten
     if len(lead) != 1:
         v, idx = v.reshape(R, K), idx.reshape(R, K)
     scale = 1.0 / R if reduction == "mean" else 1.0 if reduction == "sum" else None
-    if x.requires_grad and torch.is_grad_enabled():
+    if (x.requires_grad and torch.is_grad_enabled()) or _has_tangent(x):
         out = _Distill.apply(x, ld, v, idx, temperature, int(bool(tail)), scale)
     else:
         out = _distill_forward(x, ld, v, idx, temperature, int(bool(tail)), scale, False)[0]
@@ -1246,9 +1255,9 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     f32 from `quantize_rows`, bias (N) f32 or bf16 or None; the tokens are quantised row by row on the way in
     (vqaf_int8_linear).  Returns (..., N) in out_dtype (default: x's).  Weights in rows that are not whole 16-byte
     pieces are copied into such rows first.  There is no gradient: an input that requires one is refused while
-    gradients are recorded."""
-    if (x.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad)) and \
-            torch.is_grad_enabled():
+    gradients are recorded, and one with a forward-mode tangent always."""
+    if ((x.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad)) and
+            torch.is_grad_enabled()) or _has_tangent(x, weight_scale, bias):
         raise RuntimeError("int8_linear has no gradient: call it under torch.no_grad(), or train the layer in bf16")
     x2, ld = _int8_rows(x, "int8_linear")
     if weight.dim() != 2 or weight.dtype != torch.int8:
