@@ -234,3 +234,15 @@ def test_distillation_with_a_common_module(dev):
     modes.clear()
     loops.distill(a, a, _loader(1, 5, 4, 3, 2), torch.optim.SGD(a.parameters(), lr=0.1), dev, top=2)
     assert modes == [(False, False), (True, True)]
+
+
+def test_adapters_of_a_quantised_stack_do_not_merge(dev):
+    """The plain weights are gone: the call says so, and works as before on a stack that has them."""
+    from vqa_amd.encoders import BertConfig, BertModel, add_lora, merged_lora_weights, quantize_int8
+    stack = BertModel(BertConfig(vocab_size=50, hidden_size=64, num_hidden_layers=1, num_attention_heads=1,
+                                 intermediate_size=128, max_position_embeddings=16))
+    add_lora(stack)
+    assert set(merged_lora_weights(stack)) == {f"encoder.layer.0.attention.self.{t}.weight" for t in ("query", "value")}
+    stack = quantize_int8(stack.to(dev).eval())
+    with pytest.raises(RuntimeError, match="quantize_int8"):
+        merged_lora_weights(stack)

@@ -889,6 +889,8 @@ def merged_lora_weights(stack: "BertModel") -> dict:
     for i, lyr in enumerate(stack.encoder.layer):
         if lyr.lora is None:
             continue
+        if lyr.attention.self.packed is not None:
+            raise RuntimeError("adapters cannot be merged after quantize_int8: the plain weights are gone; merge first")
         for t in lyr.lora.targets:
             pair, lin = lyr.lora.adapters[t], getattr(lyr.attention.self, t)
             out[f"encoder.layer.{i}.attention.self.{t}.weight"] = (
