@@ -62,3 +62,19 @@ def test_entry_points_refuse_bad_arguments():
     def db(step=0, up=p, g=p, ldg=8):
         return lib.vqaf_distill_bwd(p, 8, p, p, 2, 8, 2, 0, 1.0, p, up, step, 0, 1.0, g, ldg, None)
     assert db(step=2) == -1 and db(up=None) == -5 and db(ldg=10) == -3 and db(g=p + 4) == -3
+
+
+def test_module_loads_without_torch_s_private_names():
+    """A torch without the quick ways to the current device and stream: the module imports and checks its arguments."""
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+    code = ("import torch\n"
+            "for n in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):\n"
+            "    if hasattr(torch._C, n): delattr(torch._C, n)\n"
+            "from vqa_amd import ops\n"
+            "try: ops.token_logprobs(torch.zeros(2, 5))\n"
+            "except RuntimeError as e: print(e)\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "GPU only" in r.stdout, r.stderr

@@ -828,8 +828,9 @@ class TokenLogprobs(NamedTuple):
     top_indices: Optional[torch.Tensor]
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index, without building a stream object
-_current_device = torch._C._cuda_getDevice
+# Of a device index without building a stream object, where torch has it (a build without GPU support does not)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _launch(device: torch.device, entry: str, *args) -> None:
