@@ -257,7 +257,8 @@ def adv_swap_(top: torch.Tensor, bottom: torch.Tensor, pos: torch.Tensor, src: t
     B, K = top.shape
     R = bottom.shape[1]
     k_adv = pos.shape[1]
-    check(load().vqaf_adv_swap(ptr(top), ptr(bottom), ptr(pos.contiguous()), ptr(src.contiguous()),
+    pos, src = pos.contiguous(), src.contiguous()   # (copies have to outlive the launch)
+    check(load().vqaf_adv_swap(ptr(top), ptr(bottom), ptr(pos), ptr(src),
                                B, K, R, k_adv, stream_ptr(top.device)), "vqaf_adv_swap")
 
 
@@ -762,7 +763,8 @@ class _MeanCE(torch.autograd.Function):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("cross_entropy_mean: run one step eagerly before capturing a HIP graph")
             ticket = _ce_tickets[dev] = torch.zeros(1, dtype=torch.int32, device=dev)
-        check(load().vqaf_ce_mean(ptr(lg), ptr(targets.to(torch.int64).contiguous()), B, C, dtype_code(lg), ptr(loss),
+        tg = targets.to(torch.int64).contiguous()   # (a copy has to outlive the launch)
+        check(load().vqaf_ce_mean(ptr(lg), ptr(tg), B, C, dtype_code(lg), ptr(loss),
                                   ptr(buf), ldg, dtype_code(buf), 1.0 / B, ptr(mean), ptr(ticket), stream_ptr(dev)),
               "vqaf_ce_mean")
         ctx.buf = buf  # the unit-gradient backward hands on a view of it (its base stays this object)
