@@ -78,3 +78,13 @@ def test_module_loads_without_torch_s_private_names():
             "except RuntimeError as e: print(e)\n")
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "GPU only" in r.stdout, r.stderr
+
+
+@pytest.mark.parametrize("top", [0, -1, 129])
+def test_distillation_needs_answers(top):
+    """Refused before anything runs: a list of no answers used to end inside the first batch, in an AttributeError."""
+    from vqa_amd import loops
+    net = torch.nn.Linear(2, 3).eval()
+    with pytest.raises(ValueError, match="top"):
+        loops.distill(net, torch.nn.Linear(2, 3), [], torch.optim.SGD(net.parameters(), 0.1), "cpu", top=top)
+    assert not net.training

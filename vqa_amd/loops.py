@@ -124,8 +124,10 @@ def distill(model: nn.Module, teacher: nn.Module, train_loader, optimizer, devic
     (ops.token_logprobs) are the targets of ops.distill_loss.  A student that has seen only another model's answers is the
     usual alternative to DP-SGD against the attacks that vqa_amd.mia scores.  hard_weight > 0 mixes the labels' mean
     cross-entropy in: (1 - hard_weight) * distillation + hard_weight * cross-entropy.  The teacher runs in eval mode
-    without gradients, also in modules that it shares with the student; held in eight bits (encoders.quantize_int8) it labels faster.  Returns (average loss, agreement of
-    the best answers in %)."""
+    without gradients, also in modules that it shares with the student; held in eight bits (encoders.quantize_int8) it
+    labels faster.  Returns (average loss, agreement of the best answers in %)."""
+    if not 1 <= top <= ops.ANSWERS_MAX:
+        raise ValueError(f"top has to be in [1, {ops.ANSWERS_MAX}], got {top}")
     if not 0.0 <= hard_weight < 1.0:
         raise ValueError(f"hard_weight has to be in [0, 1), got {hard_weight}")
     teacher.eval()
