@@ -412,8 +412,8 @@ __device__ __forceinline__ void an_write_named(const int* idx, const float* add,
 constexpr int AN_ST = 256, AN_SP = 4;   // threads, pieces per thread of a streamed segment
 constexpr int AN_NAMED = 2 * AN_TOP_MAX;
 
-// A segment of 16 KB of a row for each workgroup.  Measured, 1001 x 50265 bf16: 38 us (5.3 TB/s read and written, the rate
-// of a large copy); 511 x 50265 f32 with 100 named entries a row: 45 us (4.6 TB/s).
+// A segment of 16 KB of a row for each workgroup.  Measured, 1001 x 50265 bf16: 37 us (5.5 TB/s read and written, the rate
+// of a large copy); 511 x 50265 f32 with 100 named entries a row: 46 us (4.5 TB/s).
 template <bool BF16, class OP>
 __global__ __launch_bounds__(AN_ST) void answer_grad_block_kernel(const OP op, const void* x, long ld, long r0, long R, int C,
                                                                   int segments, void* grad, long ldg) {
@@ -451,6 +451,8 @@ __global__ __launch_bounds__(AN_ST) void answer_grad_block_kernel(const OP op, c
                        [&](float t) { return OP::term(w, t); });
 }
 
+// A wave to a row of up to 1024 classes.  Measured, log probabilities of 25000 x 430: bf16 21 us (2.0 TB/s: two bytes a lane),
+// f32 18 us (4.8 TB/s).
 template <bool BF16, int E, class OP>
 __global__ __launch_bounds__(64 * AN_WAVES) void answer_grad_wave_kernel(const OP op, const void* x, long ld, long r0, long R,
                                                                          int C, void* grad, long ldg) {

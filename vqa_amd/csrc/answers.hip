@@ -188,8 +188,8 @@ __device__ __forceinline__ float an_threshold(const float* tmax, int threads_wit
 // One read of the row into registers, its maximum (bf16: on packed pairs as integers), the sums of e and e t, and the
 // alternatives.  Those reach the K-th largest of the threads' maxima, or very nearly only they do: the threads that hold
 // such values look through their pieces once more, and the short list that results is ranked by counting.
-// Measured, 1920 rows of 30522 bf16 classes: 29 us without alternatives (4.0 TB/s), 35 us with 20 (3.3 TB/s), 41 with 64;
-// 1001 x 50265: 27 us without (3.7 TB/s).  Half of the time is vector instructions (14 for each value, 7 of them for e and e t);
+// Measured, 1920 rows of 30522 bf16 classes: 28 us without alternatives (4.2 TB/s), 36 us with 20 (3.3 TB/s), 41 with 64;
+// 1001 x 50265: 27 us without (3.7 TB/s); 511 x 70001, read again: 26 us without (2.8 TB/s), 33 with 20.  Half of the time is vector instructions (14 for each value, 7 of them for e and e t);
 // 1920 rows are one and a half rounds of what fits on the chip.
 template <bool BF16, int NT, int E, int W>
 __global__ __launch_bounds__(NT, W) void logprob_block_kernel(const LogprobArgs a) {
@@ -357,7 +357,7 @@ __device__ __forceinline__ void an_wave_select(const unsigned (&key)[E], unsigne
   }
 }
 
-// Measured, 430 f32 classes: 1024 rows with a target 2.8 us, with three alternatives 4.1, with 20 5 us; 25000 rows with a
+// Measured, 430 f32 classes: 1024 rows with a target 3.4 us, with three alternatives 4.6, with 20 5.7 us; 25000 rows with a
 // target and 20 alternatives 25 us, with 64 54 us: a row is some 300 instructions of one wave, most of them for the
 // alternatives.
 template <bool BF16, int E>
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(64 * AN_WAVES, E <= 8 ? 8 : 5) void logprob_wave_ke
 // ---------------------------------------------------------------------------------------------
 // Taken from 8192 rows on, for up to eight alternatives.  With many rows the instructions of the reductions and of the
 // alternatives count, and here four rows share them; with few the latency does, and a whole wave to a row has less of it.
-// Measured, 430 f32 classes with a target and 0 / 3 / 8 alternatives: 25000 rows 11.2 / 15.4 / 18.2 us (3.8 TB/s without
+// Measured (the shortest of many launches, both sides in one run), 430 f32 classes with a target and 0 / 3 / 8 alternatives: 25000 rows 11.2 / 15.4 / 18.2 us (3.8 TB/s without
 // alternatives) against 13.1 / 19.6 / 23.0 with a wave to a row, 8192 rows 5.9 / 8.0 / 9.4 against 6.8 / 9.4 / 10.8, 4096
 // rows 4.4 / 6.3 / 7.6 against 4.7 / 6.4 / 7.1, 1024 rows 3.4 / 5.3 / 6.4 against 2.8 / 4.1 / 4.4; 25000 rows of 430 bf16
 // classes 10.3 / 14.8 / 17.4 against 15.6 / 21.4 / 24.5.  Loads are 16-byte pieces as in the longer rows: single elements

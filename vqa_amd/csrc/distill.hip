@@ -221,9 +221,10 @@ __device__ __forceinline__ u32x4 an_drop(u32x4 r, unsigned bits) {
 // HOLD: the exponentials stay in registers for the gradient (f32: in the place of the logits; bf16: in twice the
 // registers, only for short rows); otherwise they are formed again.
 // Measured, 1920 rows of 30522 bf16 classes, 64 answers, with the rest as an event and the gradient: 65 us (3.6 TB/s read
-// and written; 45 us without the gradient); 511 x 50265 f32, 100 answers, loss only: 35 us (2.9 TB/s: two workgroups to
-// a CU hold all the rows at once, so that loads, sums and reductions of a row follow one another).  25 vector instructions a
-// value take two thirds of that.
+// and written; 45 us without the gradient); 511 x 50265 f32, 100 answers, without a gradient: 37 us with the statistics for
+// one, 31 without (2.8 and 3.3 TB/s: two workgroups to a CU hold all the rows at once, so that loads, sums and reductions
+// of a row follow one another); 511 x 70001 bf16, read again, with the gradient: 49 us.  25 vector instructions a value take
+// two thirds of the first.
 template <bool BF16, int NT, int E, bool TAIL, bool HOLD, int W>
 __global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs a) {
   constexpr int V = Piece<BF16>::V, NW = NT / 64;
@@ -376,8 +377,8 @@ __global__ __launch_bounds__(NT, W) void distill_block_kernel(const DistillArgs 
                        [&](float q) { return none ? 0.f : -sc * q; });
 }
 
-// One wave per row of up to 1024 classes.  Measured, 64 x 430 bf16 and 1024 x 430 f32 with gradient: 7 us, a chain of
-// reductions and f64 logarithms.
+// One wave per row of up to 1024 classes.  Measured with the gradient, 64 x 430 bf16 8 us and 1024 x 430 f32 9 us, a chain of
+// reductions and f64 logarithms; 25000 x 430 bf16 46 us, with the rest as an event 50 us: f64 arithmetic, 0.9 TB/s.
 template <bool BF16, int E>
 __global__ __launch_bounds__(64 * AN_WAVES) void distill_wave_kernel(const DistillArgs a) {
   __shared__ DistillList s_list[AN_WAVES];

@@ -4,9 +4,9 @@
 //   s_m = max(max_k |x_mk| / 127, 2^-126),   q_mk = round-half-even(x_mk / s_m),   y_mn = (sum_k q_mk w_nk) s_m s_n + b_n
 //
 // The sum is exact in 32-bit integers (127^2 K < 2^31 for K up to 131072); the two scales, the bias and the rounding to
-// the output type follow in f32, in the epilogue, without leaving its range on the way where the result does not.  The quotient is rounded as if it were exact: next to a border the
-// sign of x - (q +- 1/2) s, one fused multiply-add, decides.  A row with NaN or an infinity gets the scale NaN, which
-// makes its outputs NaN.
+// the output type follow in f32, in the epilogue, without leaving its range on the way where the result does not.  The
+// quotient is rounded as if it were exact: next to a border the sign of x - (q +- 1/2) s, one fused multiply-add, decides.  A
+// row with NaN or an infinity gets the scale NaN, which makes its outputs NaN.
 //
 // Many tokens: one pass writes the rows as integers, bound by its bytes, and a matrix product on 32x32x32 integer MFMAs
 // reads them through a ring of stages in shared memory.  Up to 64 tokens: the product is bound by the weights' bytes and
@@ -156,7 +156,8 @@ __device__ __forceinline__ unsigned i8_amax_bits(unsigned top) {   // as the bit
 }
 
 // One wave per row: E x 512 columns in registers, or (E = 0) the row read twice.  Writes zeros up to the row's pitch.
-// Measured, bf16: 8191 x 4096 23 us (4.4 TB/s read and written), 12608 x 768 10 us (2.9 TB/s: a row is only 1.5 KB).
+// Measured, bf16: 8191 x 4096 24 us (4.2 TB/s read and written), 12608 x 768 10 us (2.9 TB/s: a row is only 1.5 KB); f32:
+// 38 us (4.4 TB/s), 10 us.
 template <bool BF16, bool VEC, int E>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const QuantArgs a) {
   const int lane = threadIdx.x & 63;
@@ -340,12 +341,13 @@ __device__ __forceinline__ void i8_write_tile(const Int8Args& g, const I8Scales<
 // The product: output tiles of 32 TM WM tokens x 32 TN WN channels, a workgroup of WM x WN waves of 32 TM x 32 TN each.
 // k-steps of 64 values go through a ring of STAGES stages in shared memory, all but the one being read in flight, one
 // barrier a step.  A wave reads the operands of a half step under the products of the half before.
-// Measured: 8191 x 4096 x 4096 135 us (2.04 P operations/s), 8192 x 8192 x 8192 490 us (2.24 P; the library's product
-// 2.06), where the chip's power sets the pace (1.8 GHz; the same with zeros 415 us at 2.3 GHz; matrix instructions alone, on
-// random operands in registers, 3.5 P).  12608 x 768 x 2304 37 us (1.21 P: twelve k-steps, then 128 KB of output a
-// workgroup that nothing overlaps, in two rounds of tiles of which the second is three quarters full), 1920 x 768 x 768 on
-// 64 x 64 tiles 7.8 us, 500 x 4096 x 1024 13 us.  With each half step's operands awaited before its products it was 145, 42,
-// 9.2 and 16.7 us; scales and bias asked for after the product cost 4 us of the second.
+// Measured: 8191 x 4096 x 4096 145 us on average and 133 to 157 from launch to launch (1.9 P operations/s), 8192 x 8192 x
+// 8192 498 us (2.2 P; the library's product 2.1), where the chip's power sets the pace (1.8 GHz; the same with zeros 415 us
+// at 2.3 GHz; matrix instructions alone, on random operands in registers, 3.5 P).  12608 x 768 x 2304 36 us (1.25 P: twelve
+// k-steps, then 128 KB of output a workgroup that nothing overlaps, in two rounds of tiles of which the second is three
+// quarters full; 43 us with f32 outputs), 1920 x 768 x 768 on 64 x 64 tiles 7.7 us, 500 x 4096 x 1024 12 us.  With each half
+// step's operands awaited before its products they took 7 to 28 percent longer; scales and bias asked for after the
+// product cost 4 us of the third.
 constexpr int I8_BK = 64;
 
 // piece c (16 values) of row r of a [rows][64] image lies at position c ^ i8_swz(r): sixteen rows on sixteen slots
@@ -593,7 +595,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void int8_tile_kernel(const Int8
 
 // ---------------------------------------------------------------------------------------------
 // Few tokens: 16 output channels per workgroup, the contraction cut among its four waves.  Measured: one token, 768 x 2304
-// 4.2 us and 4096 x 4096 6.7 us (2.5 TB/s of weights), the quantiser and the launch included
+// 5.0 us and 4096 x 4096 8.0 us (2.1 TB/s of weights), the quantiser and the launch included; 5, 16 and 64 tokens of 768 x 2304
+// 4.0, 4.1 and 5.9 us behind a quantiser of 2.8, 3.4 and 4.3 us
 // ---------------------------------------------------------------------------------------------
 constexpr int I8_SELF = 4;          // tokens whose rows the workgroups quantise themselves
 constexpr int I8_SELF_K = 8192;     // and the columns up to which they do
@@ -763,11 +766,12 @@ int i8_launch_tile(Int8Args& g, hipStream_t st) {
 
 template <bool YB>
 int i8_launch_tiles(Int8Args& g, hipStream_t st) {
-  // 256 x 256 tiles, one workgroup of eight waves per CU, once they nearly fill the chip (12608 x 768 x 2304: 450 tiles,
-  // 37 us against 42 us on 128 x 128; 2048 x 4096 x 4096: 128 tiles, 54 against 49 us); 128 x 128 tiles, two
-  // workgroups per CU, down to one for each CU (1920 x 768 x 2304: 270 tiles, 13 us against 16.5 us on 64 x 64;
-  // 500 x 4096 x 1024: 32 tiles, 20 against 13 us); then 64 x 64 in a ring twice as deep, where few workgroups have to
-  // hide the latency by themselves.
+  // 256 x 256 tiles, one workgroup of eight waves per CU, once they nearly fill the chip (quantiser included, 12608 x 768 x
+  // 2304: 450 tiles, 49 us against 52 on 128 x 128, and 8191 x 4096 x 4096 156 against 194; 2048 x 4096 x 4096: 128 tiles, 64
+  // against 57 us); 128 x 128 tiles, two workgroups per CU, down to one for each CU (1920 x 768 x 2304: 270 tiles, 16.7 us
+  // against 19.3 us on 64 x 64; 500 x 4096 x 1024: 32 tiles, 28 against 20 us); then 64 x 64 in a ring twice as deep, where
+  // few workgroups have to hide the latency by themselves.  The channels that a tile lacks are not weighed: of 37000 tokens
+  // of 768, 8 channels take 38 us on 256 x 256 against 32 on 64 x 64, 430 channels 80 against 68 on 128 x 128.
   const long t256 = (long)((g.M + 255) / 256) * ((g.N + 255) / 256), t128 = (long)((g.M + 127) / 128) * ((g.N + 127) / 128);
   if (t256 >= 144) return i8_launch_tile<YB, 4, 2, 2, 4, 4, 2>(g, st);
   if (t128 >= 256) return i8_launch_tile<YB, 2, 2, 2, 2, 4, 2>(g, st);
